@@ -109,6 +109,56 @@ int sal_rope_rows_f16(void *q, const void *k, const void *v, const void *cos, co
                       int heads, int kv_heads, int hd, int max_len, void *stream);
 int sal_causal_softmax_f16(void *scores, int heads, int m, int T, int first, float scale, void *stream);
 
+/* A cache of keys and values in 4 bits, for sequences of different lengths (hd 64, 128 or 256; others return SAL_E_UNSUPPORTED).
+ *
+ * Pages of SAL_KV4_PAGE positions: pool uint8 [pages][kv_heads][64 * (hd + hd / 8)] per layer, 16-byte aligned.  table int32
+ * [batch][max_pages] names the pages of each sequence in order; entries outside 0..pages-1 are pages that do not exist: nothing is
+ * stored there and nothing seen.  The record of a page and kv head: codes of K [64][hd / 2], codes of V, parameters of K as fp16
+ * [64][hd / 64][2], parameters of V.  64 neighbouring numbers of a row are a group with a scale and a lowest value:
+ *     low = min, scale = half((max - min) / 15), code = min(15, rint((x - low) * (1 / scale))), value = low + scale * code,
+ * steps in 32-bit arithmetic.  A group with a number that is not finite reads back as NaN.  Byte j of a group's 32 bytes holds numbers
+ * 2j (low half) and 2j + 1; group g of position p lies in block g ^ f(p) of its row, f(p) = s(p) for hd 256, s(p) >> 1 for 128, 0 for 64,
+ * s(p) = (p & 3) ^ ((p >> 1) & 2).  A page costs kv_heads * 64 * (hd + hd / 8) bytes: 72 bytes for 128 numbers.
+ *
+ * Rows: `m` new rows of each of `batch` sequences, batch * m <= SAL_KV4_MAX_ROWS.  Row i of sequence b stands at position pos[b] + i
+ * (pos int64, on the device); rows int32 [batch] (may be NULL: all) says how many of the m rows there are, what the others have is neither
+ * read nor written.
+ *
+ * sal_rope_kv4_write_f16: q [batch][m][heads][hd] is rotated into q_out (may be q), k [batch][m][kv_heads][hd] rotated, quantised and stored,
+ * v quantised and stored.  A rotated number is the exact a * cos - b * sin rounded to 32 and then to 16 bits.  cos/sin: fp32
+ * [max_len][hd / 2].  Nothing is written for rows outside 0..min(max_len, 64 * max_pages)-1.
+ * sal_read_kv4: the values of m positions from pos[b] on, k_out and v_out [batch][m][kv_heads][hd], fp32 (out_f32) or fp16; zero for
+ * positions without a page.
+ * sal_attention_kv4_f16: q [batch][m][heads][hd] (rotated), out likewise; row i of sequence b sees positions 0..pos[b] + i as far as their
+ * pages exist (a row that sees none gets zeros).  Scores and sums in fp32.  workspace: sal_attention_kv4_workspace_bytes of scratch, zero-filled
+ * once, 16-byte aligned, not shared between streams.
+ * sal_copy_kv4_pages: page dst[i] becomes a copy of page src[i], in all of `layers` layers (pool [layers][pages][page_bytes]).  src and dst
+ * are HOST arrays, which the call has done with when it returns; no page may be written twice, or written and read (SAL_E_SHAPE). */
+#define SAL_KV4_PAGE 64
+#define SAL_KV4_MAX_ROWS 65535
+int sal_rope_kv4_write_f16(const void *q, const void *k, const void *v, const void *cos, const void *sin, const int64_t *pos,
+                           const int32_t *rows, const int32_t *table, void *pool, void *q_out, int batch, int m, int heads, int kv_heads,
+                           int hd, int max_len, int max_pages, int pages, void *stream);
+int sal_read_kv4(const void *pool, const int32_t *table, const int64_t *pos, void *k_out, void *v_out, int out_f32, int batch, int m,
+                 int kv_heads, int hd, int max_pages, int pages, void *stream);
+size_t sal_attention_kv4_workspace_bytes(int batch, int m, int heads, int kv_heads, int hd);
+int sal_attention_kv4_f16(const void *q, const void *pool, const int32_t *table, const int64_t *pos, const int32_t *rows, void *out, int batch,
+                          int m, int heads, int kv_heads, int hd, int max_pages, int pages, float scale, void *workspace,
+                          size_t workspace_bytes, void *stream);
+int sal_copy_kv4_pages(void *pool, const int32_t *src, const int32_t *dst, int count, int layers, int pages, size_t page_bytes, void *stream);
+
+/* The next token of each of `rows` sequences, drawn from its logits (fp32 if logits_f32, else fp16; [rows][vocab], vocab <= 262144) with the
+ * random number u[row] (fp32): a token's weight is exp((logit - largest) / temperature); in the order of falling logits, equal ones by
+ * index, the first top_k tokens stay (<= 0: all), of these those in front of which less than top_p of their weights lies (>= 1: all;
+ * the first always stays), of these those with a weight of at least min_p (the largest is 1; <= 0: all).  The token is the first, by index,
+ * at which the running sum of the weights that stayed exceeds u times their total.  temperature <= 0 takes the largest logit, the first of
+ * equal ones.  NaN and -infinity are never chosen; a row of nothing else gives 0.  temperature, top_k, top_p, min_p: device arrays [rows],
+ * or NULL for the one value of all rows that stands in the argument of that name with _all.  Weights are summed in whole numbers of 2**-44:
+ * equal inputs give equal tokens. */
+int sal_sample_token(const void *logits, int logits_f32, int rows, int vocab, const void *u, const void *temperature, const int32_t *top_k,
+                     const void *top_p, const void *min_p, float temperature_all, int top_k_all, float top_p_all, float min_p_all,
+                     int64_t *token, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,6 +23,9 @@ SAL_MAX_PEERS = 8
 SAL_MAX_M = 64
 SAL_MAX_ROWS = 4096   # rows of one tensor-core product (sal_lutgemm_rows)
 
+SAL_KV4_PAGE = 64        # positions of a page of the 4-bit cache
+SAL_KV4_MAX_ROWS = 65535
+
 _vp, _i, _u, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint, ctypes.c_size_t
 
 
@@ -90,6 +93,12 @@ SIGNATURES = {
     "sal_residual_rmsnorm_rows_f16": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, ctypes.c_float, _vp]),
     "sal_rope_attention_decode_batch": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, ctypes.c_float, _vp,
                                             ctypes.c_size_t, _vp]),
+    "sal_rope_kv4_write_f16": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "sal_read_kv4": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "sal_attention_kv4_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "sal_attention_kv4_f16": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, ctypes.c_float, _vp, _sz, _vp]),
+    "sal_copy_kv4_pages": (_i, [_vp, _vp, _vp, _i, _i, _i, _sz, _vp]),
+    "sal_sample_token": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, ctypes.c_float, _i, ctypes.c_float, ctypes.c_float, _vp, _vp]),
 }
 
 _lib = None

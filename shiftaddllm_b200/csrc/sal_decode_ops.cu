@@ -508,23 +508,6 @@ __global__ void __launch_bounds__(128) causal_softmax_kernel(__half *scores, int
     }
 }
 
-// All helpers are launched with the programmatic-stream-serialization attribute (see pdl_prologue).
-template <typename... KArgs, typename... Args>
-int launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, void *stream, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...) == cudaSuccess ? SAL_OK : SAL_E_LAUNCH;
-}
-
-
 // Single-query attention split over the cached positions ("flash decoding"): CTA (kv head, slice) handles
 // the slice's positions for the G query heads that share the kv head, so a K or V row is read once per
 // group.  A row of hd halves is read by hd/8 lanes with 16-byte loads (a warp covers 32/(hd/8) positions
@@ -965,7 +948,7 @@ int launch_attention_variant(size_t smem, const void *q, const void *k_cache, co
                    ? SAL_OK
                    : SAL_E_LAUNCH;
     }
-    return launch_pdl(attention_split_kernel<G, STAGE_V, ROPE, CLUSTER>, dim3(kv_heads, nsplit, batch), dim3(ATTN_WARPS * 32), smem, stream, q,
+    return sal_launch_pdl(attention_split_kernel<G, STAGE_V, ROPE, CLUSTER>, dim3(kv_heads, nsplit, batch), dim3(ATTN_WARPS * 32), smem, stream, q,
                       reinterpret_cast<__half *>(const_cast<void *>(k_cache)), reinterpret_cast<__half *>(const_cast<void *>(v_cache)),
                       pos, reinterpret_cast<__half *>(out),
                       reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + ATTN_WS_HEADER),
@@ -1065,7 +1048,7 @@ int sal_residual_rmsnorm_f16(const void *x, const void *delta, const void *weigh
     if (!x || !weight || !out) return SAL_E_NULL;
     if (n < 1 || n > 12000 /* the row is staged in shared memory, 48 KB with the reduction scratch */) return SAL_E_SHAPE;
     const int threads = n >= 1024 ? 1024 : ((n + 31) / 32) * 32;
-    return launch_pdl(residual_rmsnorm_kernel, dim3(1), dim3(threads), (size_t)n * sizeof(float), stream,
+    return sal_launch_pdl(residual_rmsnorm_kernel, dim3(1), dim3(threads), (size_t)n * sizeof(float), stream,
                       reinterpret_cast<const __half *>(x), reinterpret_cast<const __half *>(delta),
                       reinterpret_cast<const __half *>(weight), reinterpret_cast<__half *>(out),
                       reinterpret_cast<__half *>(x_out), n, eps);
@@ -1076,7 +1059,7 @@ int sal_rope_kv_write_f16(void *q, const void *k, const void *v, const void *cos
     if (!q || !k || !v || !cos || !sin || !pos || !k_cache || !v_cache) return SAL_E_NULL;
     if (heads < 1 || kv_heads < 1 || hd < 2 || (hd & 1) || max_len < 1) return SAL_E_SHAPE;
     const int total = heads * (hd / 2) + kv_heads * (hd / 2) + kv_heads * hd;
-    return launch_pdl(rope_kv_write_kernel, dim3((total + 255) / 256), dim3(256), 0, stream, reinterpret_cast<__half *>(q),
+    return sal_launch_pdl(rope_kv_write_kernel, dim3((total + 255) / 256), dim3(256), 0, stream, reinterpret_cast<__half *>(q),
                       reinterpret_cast<const __half *>(k), reinterpret_cast<const __half *>(v),
                       reinterpret_cast<const float *>(cos), reinterpret_cast<const float *>(sin), pos,
                       reinterpret_cast<__half *>(k_cache), reinterpret_cast<__half *>(v_cache), heads, kv_heads, hd, max_len);
@@ -1090,7 +1073,7 @@ int sal_residual_rmsnorm_fixedacc(const void *x, void *delta_acc, const void *we
     // one CTA for the norm, plus one per 16 K extra accumulator words to clear (at most 32)
     int zero_ctas = (zero_a_n + zero_b_n + 16383) / 16384;
     if (zero_ctas > 32) zero_ctas = 32;
-    return launch_pdl(residual_rmsnorm_acc_kernel, dim3(1 + zero_ctas), dim3(threads), (size_t)n * sizeof(float), stream,
+    return sal_launch_pdl(residual_rmsnorm_acc_kernel, dim3(1 + zero_ctas), dim3(threads), (size_t)n * sizeof(float), stream,
                       reinterpret_cast<const __half *>(x), reinterpret_cast<acc_t *>(delta_acc),
                       reinterpret_cast<const __half *>(weight), reinterpret_cast<__half *>(out), reinterpret_cast<__half *>(x_out),
                       n, eps, reinterpret_cast<acc_t *>(zero_a), zero_a_n, reinterpret_cast<acc_t *>(zero_b), zero_b_n);
@@ -1102,7 +1085,7 @@ int sal_rope_kv_write_fixedacc(void *q_acc, void *k_acc, void *v_acc, void *q_ou
     if (!q_acc || !k_acc || !v_acc || !q_out || !cos || !sin || !pos || !k_cache || !v_cache) return SAL_E_NULL;
     if (heads < 1 || kv_heads < 1 || hd < 2 || (hd & 1) || max_len < 1) return SAL_E_SHAPE;
     const int total = heads * (hd / 2) + kv_heads * (hd / 2) + kv_heads * hd;
-    return launch_pdl(rope_kv_write_acc_kernel, dim3((total + 255) / 256), dim3(256), 0, stream, reinterpret_cast<acc_t *>(q_acc),
+    return sal_launch_pdl(rope_kv_write_acc_kernel, dim3((total + 255) / 256), dim3(256), 0, stream, reinterpret_cast<acc_t *>(q_acc),
                       reinterpret_cast<acc_t *>(k_acc), reinterpret_cast<acc_t *>(v_acc), reinterpret_cast<__half *>(q_out),
                       reinterpret_cast<const float *>(cos), reinterpret_cast<const float *>(sin), pos,
                       reinterpret_cast<__half *>(k_cache), reinterpret_cast<__half *>(v_cache), heads, kv_heads, hd, max_len);
@@ -1124,7 +1107,7 @@ int sal_attention_decode_f16(const void *q, const void *k_cache, const void *v_c
             configured[dev] = true;
         }
     }
-    return launch_pdl(attention_decode_kernel, dim3(heads), dim3(1024), smem, stream, reinterpret_cast<const __half *>(q),
+    return sal_launch_pdl(attention_decode_kernel, dim3(heads), dim3(1024), smem, stream, reinterpret_cast<const __half *>(q),
                       reinterpret_cast<const __half *>(k_cache), reinterpret_cast<const __half *>(v_cache), pos,
                       reinterpret_cast<__half *>(out), heads, kv_heads, hd, max_len, scale);
 }
@@ -1166,7 +1149,7 @@ int sal_residual_rmsnorm_rows_f16(const void *x, const void *delta, const void *
     if (!x || !weight || !out) return SAL_E_NULL;
     if (rows < 1 || rows > 65535 || n < 1 || n > 12000) return SAL_E_SHAPE;
     const int threads = n >= 1024 ? 1024 : ((n + 31) / 32) * 32;
-    return launch_pdl(residual_rmsnorm_kernel, dim3(rows), dim3(threads), (size_t)n * sizeof(float), stream,
+    return sal_launch_pdl(residual_rmsnorm_kernel, dim3(rows), dim3(threads), (size_t)n * sizeof(float), stream,
                       reinterpret_cast<const __half *>(x), reinterpret_cast<const __half *>(delta), reinterpret_cast<const __half *>(weight),
                       reinterpret_cast<__half *>(out), reinterpret_cast<__half *>(x_out), n, eps);
 }
@@ -1175,7 +1158,7 @@ int sal_greedy_token_f16(const void *logits_f16, void *logits_f32, int vocab, in
     if (!logits_f16 || !token || !pos) return SAL_E_NULL;
     if (vocab < 8 || vocab % 8 != 0) return SAL_E_SHAPE;
     if ((reinterpret_cast<uintptr_t>(logits_f16) & 15) || (reinterpret_cast<uintptr_t>(logits_f32) & 15)) return SAL_E_ALIGN;
-    return launch_pdl(greedy_token_kernel, dim3(1), dim3(1024), 0, stream, reinterpret_cast<const __half *>(logits_f16),
+    return sal_launch_pdl(greedy_token_kernel, dim3(1), dim3(1024), 0, stream, reinterpret_cast<const __half *>(logits_f16),
                       reinterpret_cast<float *>(logits_f32), vocab, token, pos);
 }
 
@@ -1183,9 +1166,9 @@ int sal_silu_mul_f16(const void *gate, const void *up, void *out, int n, void *s
     if (!gate || !up || !out) return SAL_E_NULL;
     if (n < 1) return SAL_E_SHAPE;
     if (n % 8 == 0 && ((reinterpret_cast<uintptr_t>(gate) | reinterpret_cast<uintptr_t>(up) | reinterpret_cast<uintptr_t>(out)) & 15) == 0)
-        return launch_pdl(silu_mul_vec_kernel, dim3((n / 8 + 255) / 256), dim3(256), 0, stream, reinterpret_cast<const uint4 *>(gate),
+        return sal_launch_pdl(silu_mul_vec_kernel, dim3((n / 8 + 255) / 256), dim3(256), 0, stream, reinterpret_cast<const uint4 *>(gate),
                           reinterpret_cast<const uint4 *>(up), reinterpret_cast<uint4 *>(out), n / 8);
-    return launch_pdl(silu_mul_kernel, dim3((n + 255) / 256), dim3(256), 0, stream, reinterpret_cast<const __half *>(gate),
+    return sal_launch_pdl(silu_mul_kernel, dim3((n + 255) / 256), dim3(256), 0, stream, reinterpret_cast<const __half *>(gate),
                       reinterpret_cast<const __half *>(up), reinterpret_cast<__half *>(out), n);
 }
 
@@ -1197,7 +1180,7 @@ int sal_rope_rows_f16(void *q, const void *k, const void *v, const void *cos, co
          reinterpret_cast<uintptr_t>(v_cache)) & 15)
         return SAL_E_ALIGN;
     const int total = (heads + kv_heads) * (hd / 16) + kv_heads * (hd / 8);
-    return launch_pdl(rope_rows_kernel, dim3((total + 255) / 256, m), dim3(256), 0, stream, reinterpret_cast<__half *>(q),
+    return sal_launch_pdl(rope_rows_kernel, dim3((total + 255) / 256, m), dim3(256), 0, stream, reinterpret_cast<__half *>(q),
                       reinterpret_cast<const __half *>(k), reinterpret_cast<const __half *>(v), reinterpret_cast<const float *>(cos),
                       reinterpret_cast<const float *>(sin), pos0, reinterpret_cast<__half *>(k_cache), reinterpret_cast<__half *>(v_cache), heads,
                       kv_heads, hd);
@@ -1209,8 +1192,8 @@ int sal_causal_softmax_f16(void *scores, int heads, int m, int T, int first, flo
     const int rows = heads * m;
     __half *p = reinterpret_cast<__half *>(scores);
     if (T % 8 == 0 && (reinterpret_cast<uintptr_t>(scores) & 15) == 0)
-        return launch_pdl(causal_softmax_kernel<8>, dim3((rows + 3) / 4), dim3(128), 0, stream, p, rows, m, T, first, scale);
-    return launch_pdl(causal_softmax_kernel<1>, dim3((rows + 3) / 4), dim3(128), 0, stream, p, rows, m, T, first, scale);
+        return sal_launch_pdl(causal_softmax_kernel<8>, dim3((rows + 3) / 4), dim3(128), 0, stream, p, rows, m, T, first, scale);
+    return sal_launch_pdl(causal_softmax_kernel<1>, dim3((rows + 3) / 4), dim3(128), 0, stream, p, rows, m, T, first, scale);
 }
 
 }  // extern "C"

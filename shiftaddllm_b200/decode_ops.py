@@ -3,6 +3,10 @@ batch-1 decode step.  Tensors must be contiguous CUDA tensors; launches go to to
 stream and are CUDA-graph capturable (the position is read from a device tensor)."""
 from __future__ import annotations
 
+import contextlib
+import ctypes
+import math
+
 import torch
 
 from . import _lib
@@ -10,6 +14,14 @@ from . import _lib
 
 def _stream(t):
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """Makes `device` the current one for a launch, where it is not."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def residual_rmsnorm(x, delta, weight, out, x_out, eps: float):
@@ -150,3 +162,156 @@ def causal_softmax(scores, first: int, scale: float):
     lib = _lib.load()
     _lib.check(lib.sal_causal_softmax_f16(scores.data_ptr(), scores.shape[0], scores.shape[1], scores.shape[2], int(first), float(scale),
                                           _stream(scores)), "sal_causal_softmax_f16")
+
+
+# ---- a cache in 4 bits, in pages, for sequences of different lengths ----------------------------------------------------
+
+KV4_PAGE = _lib.SAL_KV4_PAGE
+
+
+def _want(what, name, t, dtype, shape, device):
+    """`t` is a contiguous tensor of this dtype on this device; `shape`: so many numbers in all, so many in its last dimension."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{what}: {name} must be a torch.Tensor")
+    if t.device != device or t.dtype != dtype or not t.is_contiguous() or t.numel() != math.prod(shape) or (t.dim() > 0 and t.shape[-1] != shape[-1]):
+        raise RuntimeError(f"{what}: {name} must be a contiguous {dtype} tensor {list(shape)} on {device}, got {list(t.shape)} {t.dtype} on {t.device}")
+
+
+def _kv4_pool_check(what, pool, table, pos, rows, kv_heads, hd):
+    """Checks what every call on a layer's pool takes; returns (device, batch, max_pages, pages)."""
+    if not isinstance(pool, torch.Tensor) or not pool.is_cuda:
+        raise RuntimeError(f"{what}: pool must be a CUDA tensor (there is no CPU path)")
+    record = kv4_record_bytes(hd)
+    if pool.dim() != 3 or pool.shape[1] != kv_heads or pool.shape[2] != record or pool.dtype != torch.uint8 or not pool.is_contiguous():
+        raise RuntimeError(f"{what}: pool must be a contiguous uint8 tensor [pages, {kv_heads}, {record}], got {tuple(pool.shape)} {pool.dtype}")
+    device, batch = pool.device, pos.numel()
+    _want(what, "pos", pos, torch.int64, (batch,), device)
+    if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.shape[0] != batch or table.shape[1] < 1:
+        raise RuntimeError(f"{what}: table must be an int32 tensor [{batch}, pages of a sequence]")
+    _want(what, "table", table, torch.int32, table.shape, device)
+    if rows is not None:
+        _want(what, "rows", rows, torch.int32, (batch,), device)
+    return device, batch, table.shape[1], pool.shape[0]
+
+
+def _rows_per_sequence(what, name, t, batch, width):
+    """m of a tensor [batch, m, width] (or [batch * m, width])."""
+    if not isinstance(t, torch.Tensor) or batch < 1 or t.numel() == 0 or t.numel() % (batch * width):
+        raise RuntimeError(f"{what}: {name} must hold the same number of rows of {width} numbers for each of {batch} sequences")
+    return t.numel() // (batch * width)
+
+
+def kv4_record_bytes(hd: int) -> int:
+    """Bytes of a page and kv head: 64 positions of codes and parameters, keys and values."""
+    if hd not in (64, 128, 256):
+        raise RuntimeError(f"the 4-bit cache takes heads of 64, 128 or 256 numbers, got {hd}")
+    return KV4_PAGE * (hd + hd // 8)
+
+
+def kv4_pool(layers: int, pages: int, kv_heads: int, hd: int, device) -> torch.Tensor:
+    """Zero-filled pages for `layers` layers: uint8 [layers, pages, kv_heads, record]; a layer's pool is `pool[layer]`."""
+    return torch.zeros(layers, pages, kv_heads, kv4_record_bytes(hd), dtype=torch.uint8, device=device)
+
+
+def rope_kv4_write(q, k, v, cos, sin, pos, table, pool, q_out, heads, kv_heads, hd, rows=None):
+    """Rotary step of m new rows of each of `batch` sequences, and their keys and values into a 4-bit cache (the format, and what is left
+    unwritten, stand in include/sal_decode_ops.h).  q, q_out fp16 [batch, m, heads * hd] (q_out may be q), k, v fp16 [batch, m, kv_heads * hd],
+    cos, sin fp32 [max_len, hd / 2], pos int64 [batch]: position of each sequence's first new row, table int32 [batch, pages of a sequence],
+    pool: one layer's uint8 [pages, kv_heads, record].  rows int32 [batch]: how many of the m rows there are (None: all)."""
+    device, batch, max_pages, pages = _kv4_pool_check("rope_kv4_write", pool, table, pos, rows, kv_heads, hd)
+    m = _rows_per_sequence("rope_kv4_write", "q", q, batch, heads * hd)
+    for name, t, width in (("q", q, heads), ("q_out", q_out, heads), ("k", k, kv_heads), ("v", v, kv_heads)):
+        _want("rope_kv4_write", name, t, torch.float16, (batch, m, width * hd), device)
+    _want("rope_kv4_write", "cos", cos, torch.float32, (cos.numel() // (hd // 2), hd // 2), device)
+    _want("rope_kv4_write", "sin", sin, torch.float32, (cos.shape[0], hd // 2), device)
+    lib = _lib.load()
+    with _on(device):
+        _lib.check(lib.sal_rope_kv4_write_f16(q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos.data_ptr(),
+                                              None if rows is None else rows.data_ptr(), table.data_ptr(), pool.data_ptr(), q_out.data_ptr(),
+                                              batch, m, heads, kv_heads, hd, cos.shape[0], max_pages, pages, _stream(q)), "sal_rope_kv4_write_f16")
+
+
+def read_kv4(pool, table, pos, k_out, v_out, kv_heads, hd):
+    """The values of m positions of each sequence, from pos[b] on: k_out and v_out [batch, m, kv_heads, hd] in float32 (as they are) or
+    float16 (rounded); zeros where a sequence has no page."""
+    device, batch, max_pages, pages = _kv4_pool_check("read_kv4", pool, table, pos, None, kv_heads, hd)
+    m = _rows_per_sequence("read_kv4", "k_out", k_out, batch, kv_heads * hd)
+    if k_out.dtype not in (torch.float32, torch.float16):
+        raise RuntimeError(f"read_kv4: k_out must be float32 or float16, got {k_out.dtype}")
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        _want("read_kv4", name, t, k_out.dtype, (batch, m, kv_heads, hd), device)
+    lib = _lib.load()
+    with _on(device):
+        _lib.check(lib.sal_read_kv4(pool.data_ptr(), table.data_ptr(), pos.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
+                                    1 if k_out.dtype == torch.float32 else 0, batch, m, kv_heads, hd, max_pages, pages, _stream(pool)), "sal_read_kv4")
+
+
+def attention_kv4_workspace(batch: int, m: int, heads: int, kv_heads: int, hd: int, device) -> torch.Tensor:
+    """Zero-filled scratch for attention_kv4 calls of up to this size (one per stream that uses it)."""
+    lib = _lib.load()
+    need = lib.sal_attention_kv4_workspace_bytes(int(batch), int(m), int(heads), int(kv_heads), int(hd))
+    if need == 0:
+        raise RuntimeError(f"attention_kv4_workspace: no such shape: batch {batch}, {m} rows, {heads} heads over {kv_heads}, {hd} numbers")
+    return torch.zeros(need, dtype=torch.uint8, device=device)
+
+
+def attention_kv4(q, pool, table, pos, out, heads, kv_heads, hd, scale: float, workspace, rows=None):
+    """Attention of m rows of each of `batch` sequences over a 4-bit cache: row i of sequence b sees the positions 0 .. pos[b] + i as far as
+    their pages exist (none: zeros).  q (rotated) and out fp16 [batch, m, heads * hd]; the other arguments as rope_kv4_write takes them."""
+    device, batch, max_pages, pages = _kv4_pool_check("attention_kv4", pool, table, pos, rows, kv_heads, hd)
+    m = _rows_per_sequence("attention_kv4", "q", q, batch, heads * hd)
+    for name, t in (("q", q), ("out", out)):
+        _want("attention_kv4", name, t, torch.float16, (batch, m, heads * hd), device)
+    _want("attention_kv4", "workspace", workspace, torch.uint8, workspace.shape, device)
+    lib = _lib.load()
+    with _on(device):
+        _lib.check(lib.sal_attention_kv4_f16(q.data_ptr(), pool.data_ptr(), table.data_ptr(), pos.data_ptr(),
+                                             None if rows is None else rows.data_ptr(), out.data_ptr(), batch, m, heads, kv_heads, hd, max_pages,
+                                             pages, float(scale), workspace.data_ptr(), workspace.numel(), _stream(q)), "sal_attention_kv4_f16")
+
+
+def copy_kv4_pages(pool, src, dst):
+    """Page dst[i] of `pool` (uint8 [layers, pages, ..]) becomes a copy of page src[i], in every layer.  src and dst are sequences of whole
+    numbers on the host; no page may be written twice, or written and read in the same call."""
+    if not isinstance(pool, torch.Tensor) or not pool.is_cuda or pool.dtype != torch.uint8 or pool.dim() < 3 or not pool.is_contiguous():
+        raise RuntimeError("copy_kv4_pages: pool must be a contiguous uint8 CUDA tensor [layers, pages, ..]")
+    n = len(src)
+    if len(dst) != n:
+        raise RuntimeError(f"copy_kv4_pages: {n} pages to copy, {len(dst)} places")
+    if n == 0:
+        return
+    lib = _lib.load()
+    pages = (ctypes.c_int32 * (2 * n))(*src, *dst)
+    with _on(pool.device):
+        _lib.check(lib.sal_copy_kv4_pages(pool.data_ptr(), ctypes.addressof(pages), ctypes.addressof(pages) + 4 * n, n, pool.shape[0], pool.shape[1],
+                                          pool[0, 0].numel(), _stream(pool)), "sal_copy_kv4_pages (no page twice, none both read and written)")
+
+
+# ---- the next token ---------------------------------------------------------------------------------------------------
+
+
+def sample_token(logits, u, token, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """token[r] (int64) = the next token of row r of logits (fp16 or fp32 [rows, vocab]), drawn with the random number u[r] (fp32, in [0, 1)).
+    temperature, top_k, top_p and min_p are one number for all rows or a tensor of one per row (float32; top_k int32).  What each filter keeps,
+    and in which order they apply, stands in include/sal_decode_ops.h."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dtype not in (torch.float16, torch.float32) or not logits.is_contiguous() \
+            or logits.numel() == 0:
+        raise RuntimeError("sample_token: logits must be a contiguous float16 or float32 CUDA tensor [rows, vocab]")
+    vocab = logits.shape[-1]
+    rows, device = logits.numel() // vocab, logits.device
+    _want("sample_token", "u", u, torch.float32, (rows,), device)
+    _want("sample_token", "token", token, torch.int64, (rows,), device)
+    ptr, one = [], []
+    for name, v, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                           ("min_p", min_p, torch.float32)):
+        if isinstance(v, torch.Tensor):
+            _want("sample_token", name, v, dtype, (rows,), device)
+            ptr.append(v.data_ptr())
+            one.append(0)
+        else:
+            ptr.append(None)
+            one.append(v)
+    lib = _lib.load()
+    with _on(device):
+        _lib.check(lib.sal_sample_token(logits.data_ptr(), 1 if logits.dtype == torch.float32 else 0, rows, vocab, u.data_ptr(), *ptr, float(one[0]),
+                                        int(one[1]), float(one[2]), float(one[3]), token.data_ptr(), _stream(logits)), "sal_sample_token")
