@@ -15,17 +15,12 @@ namespace {
 constexpr int PAGE = 64;          // positions of a page
 constexpr int GROUP = 64;         // numbers that share a scale
 constexpr int POS_LIMIT = 1 << 30;
+constexpr int MAX_PAGES = 1 << 20;   // of a sequence
 
 __device__ __forceinline__ void pdl_prologue() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
 // Bytes of the parts of a record (one page and kv head): codes of K, codes of V, parameters of K, parameters of V.
 template <int HD>
 struct Record {
@@ -190,65 +185,622 @@ __global__ void __launch_bounds__(256) read_kv4_kernel(CacheArgs c, const int64_
     }
 }
 
-// One thread block per query head of a row; warps over the positions, each with its own running maximum and sum.
-template <int HD>
-__global__ void __launch_bounds__(128) attention_kv4_kernel(const __half *q, CacheArgs c, const int64_t *pos, const int32_t *rows, __half *out, int m,
-                                                            int heads, float scale) {
-    constexpr int G = HD / GROUP, NW = 4;
-    __shared__ float s_m[NW], s_l[NW], s_o[NW][HD];
+// ---- attention on the tensor cores -----------------------------------------------------------------------------------------------
+//
+// A score is scale * sum_g (s_g * D_g + (low_g + 8 s_g) * Q_g) with D_g = sum over the group of q * (code - 8) and Q_g = sum of q; an output is
+// sum_g E_g * A_g + sum_t p_t * (low_t + 8 s_t) with A_g = sum over positions of (p * s_g / E_g) * (code - 8).  The codes less 8 are whole
+// numbers of 16-bit floats without any error, so D_g and A_g are matrix products of 16-bit operands (m16n8k16, 32-bit sums) in which only the
+// weight p * s is rounded; it goes in as the sum of two 16-bit numbers.  E_g, a power of two not below any scale so far, keeps the weights in
+// their range.  Neither keys nor values are ever formed.
+//
+// Matrix fragments hold keys (or, for the second product, dimensions) as rows and query columns as columns: a lane's part of a row are
+// 16 neighbouring codes of one group, fetched with one 8-byte load of shared memory, two codes per logic operation and one 16-bit fused
+// multiply-add or addition.  The weights pass from the first product's result to the second's operand by an 8x8 transpose in registers.
+//
+// The work of a launch is a list of (sequence and column tile, kv head, page), dealt to the thread blocks in equal contiguous runs by the blocks
+// themselves, from the positions on the device: texts of any lengths keep all SMs equally busy, and a captured launch follows the texts.  A
+// page of a head is one contiguous record, so its fetch is one bulk copy into a ring of shared memory.  Blocks that share an item leave
+// their part (maximum, sum, unnormalised output) in scratch; the last one to arrive adds them up in the order of the positions.
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Bounded wait: false after about a second.
+__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity) {
+    uint64_t t0, t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 256; ++i)
+            if (mbar_try_wait(bar, parity)) return true;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+        if (t - t0 > 1000000000ull) return false;
+    }
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) { return mbar_try_wait(bar, parity) || mbar_wait_slow(bar, parity); }
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t selector) {
+    uint32_t d;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(selector));
+    return d;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Codes in bits 0..3 and 16..19 (low), or 4..7 and 20..23 (mid), as two 16-bit floats less 8: put under the exponent of 1024 they are
+// 1024 + code and 1024 + 16 code, exactly.
+__device__ __forceinline__ uint32_t codes_low(uint32_t x) {
+    uint32_t h;
+    asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(h) : "r"(x));
+    asm("add.rn.f16x2 %0, %0, %1;" : "+r"(h) : "r"(0xe408e408u));                      // - 1032
+    return h;
+}
+__device__ __forceinline__ uint32_t codes_mid(uint32_t x) {
+    uint32_t h;
+    asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(h) : "r"(x));
+    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(h) : "r"(0x2c002c00u), "r"(0xd480d480u));   // / 16 - 72
+    return h;
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+__device__ __forceinline__ float2 as_float2(uint32_t h) { return __half22float2(*reinterpret_cast<__half2 *>(&h)); }
+
+// Scratch: status word, counter of arrivals per item, then two parts per thread block.
+constexpr int WS_HEADER = 256;
+constexpr int MAX_LIST = 1024;        // (sequence, column tile) pairs whose work is dealt out; with more, a block takes an item
+constexpr int MIN_PAGES = 2;
+constexpr float W_ONE = 8192.f;       // a weight of 1 relative to E: well inside 16 bits, and small weights keep their bits
+
+struct AttnArgs {
+    const __half *q;
+    CacheArgs c;
+    const int64_t *pos;
+    const int32_t *rows;
+    __half *out;
+    int *status;
+    unsigned *counters;
+    float *parts;
+    int batch, m, heads, rep;
+    int col_tiles;      // column tiles of a sequence
+    int whole;          // a block takes an item
+    float scale_log2;   // scale * log2(e)
+};
+
+// NT column tiles of 8 per warp, WK warps that share a page's keys, WC warps side by side in columns.  DUP: at most four columns; the other
+// four of the tile are the same queries again and carry the second parts of the weights.
+template <int HD, int NT, bool DUP, int WK, int WC>
+struct AttnShape {
+    static constexpr int COLS = DUP ? 4 : 8 * NT * WC;
+    static constexpr int WARPS = WK * WC;
+    static constexpr int THREADS = (WARPS + 1) * 32;
+    static constexpr int REC = Record<HD>::BYTES;
+    static constexpr int PART = COLS * (HD + 2);                       // floats of a part: outputs, maxima, sums
+    static constexpr int MERGE = WK * PART * 4;                        // bytes of the warps' parts
+    static constexpr int STAGES = (HD == 256 ? 3 : HD == 128 ? 4 : 6);
+    static constexpr int SMEM = STAGES * REC + MERGE + MAX_LIST * 4 + 16 + 256;
+};
+
+struct Item {
+    int b, ct, h;       // sequence, column tile, kv head
+    int pages;          // pages that some column sees
+    int last;           // last position that some column sees
+    int rows;           // rows of the sequence
+};
+
+// Rows of sequence b, and the last position that a column of tile ct sees (-1: none); false if the tile has no row.
+template <int COLS>
+__device__ __forceinline__ bool item_of(const AttnArgs &a, int b, int ct, Item &it) {
+    it.b = b, it.ct = ct, it.rows = rows_of(a.rows, b, a.m);
+    const int i0 = ct * COLS / a.rep;
+    if (i0 >= it.rows) return false;
+    const int i1 = min((ct * COLS + COLS - 1) / a.rep, it.rows - 1);
+    it.last = min(row_position(a.pos[b], i1), a.c.max_pages * PAGE - 1);
+    it.pages = it.last < 0 ? 1 : it.last / PAGE + 1;
+    return true;
+}
+
+template <int HD, int NT, bool DUP, int WK, int WC>
+__global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) attention_tiles_kernel(AttnArgs a) {
+    using S = AttnShape<HD, NT, DUP, WK, WC>;
+    using R = Record<HD>;
+    constexpr int G = R::G, COLS = S::COLS;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t *ring = smem;
+    float *merge = reinterpret_cast<float *>(smem + S::STAGES * S::REC);
+    int *list = reinterpret_cast<int *>(smem + S::STAGES * S::REC + S::MERGE);      // running number of pages in front of a pair, per kv head
+    __shared__ uint64_t bars[2 * S::STAGES];
+    __shared__ int s_valid[S::STAGES];
+    __shared__ int s_scan[33];
+    __shared__ int s_flag;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * S::STAGES;
+    if (tid == 0) {
+        for (int i = 0; i < S::STAGES; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, S::WARPS);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     pdl_prologue();
-    const int head = blockIdx.x, row = blockIdx.y, b = row / m, i = row % m;
-    if (i >= rows_of(rows, b, m)) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int last = row_position(pos[b], i);
-    if (last >= c.max_pages * PAGE) last = c.max_pages * PAGE - 1;
-    const int kvh = head / (heads / c.kv_heads);
-    float2 qf[G], o[G];
+    const int kvh = a.c.kv_heads, pairs = a.batch * a.col_tiles;
+    Item it = {};
+    int begin, end, pair;      // this block's run of the list, and the pair that it begins in
+    if (a.whole) {
+        pair = blockIdx.x / kvh;
+        it.h = blockIdx.x % kvh;
+        if (!item_of<COLS>(a, pair / a.col_tiles, pair % a.col_tiles, it)) return;
+        begin = 0, end = it.pages;
+        __syncthreads();
+    } else {
+        int total = 0;         // pages of all pairs, and in front of each
+        for (int i0 = 0; i0 < pairs; i0 += S::THREADS) {
+            const int i = i0 + tid;
+            Item x = {};
+            const int n = i < pairs && item_of<COLS>(a, i / a.col_tiles, i % a.col_tiles, x) ? x.pages : 0;
+            int run = n;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-        qf[g] = __half22float2(*reinterpret_cast<const __half2 *>(q + ((size_t)row * heads + head) * HD + g * GROUP + 2 * lane));
-        o[g] = make_float2(0.f, 0.f);
-    }
-    float mx = -INFINITY, sum = 0.f;
-    for (int p = warp; p <= last; p += NW) {
-        const uint8_t *record = record_of<HD>(c, b, p, kvh);
-        if (!record) continue;
-        float d = 0.f;
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const float2 k = row_pair<HD>(record, false, p % PAGE, g, lane);
-            d += qf[g].x * k.x + qf[g].y * k.y;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int t = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += t;
+            }
+            if (lane == 31) s_scan[warp] = run;
+            __syncthreads();
+            int front = total;
+            for (int w = 0; w <= S::WARPS; ++w) {
+                if (w < warp) front += s_scan[w];
+                total += s_scan[w];
+            }
+            if (i < pairs) list[i] = front + run - n;
+            __syncthreads();
         }
-        d = warp_sum(d) * scale;
-        if (d == -INFINITY) continue;
-        const float next = fmaxf(mx, d);
-        const float old = __expf(mx - next), w = __expf(d - next);
-        mx = next;
-        sum = sum * old + w;
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const float2 v = row_pair<HD>(record, true, p % PAGE, g, lane);
-            o[g] = make_float2(o[g].x * old + w * v.x, o[g].y * old + w * v.y);
+        if (tid == 0) list[pairs] = total;
+        __syncthreads();
+        const long long all = (long long)total * kvh;
+        long long per = (all + gridDim.x - 1) / gridDim.x;
+        if (per < MIN_PAGES) per = MIN_PAGES;
+        const long long first = per * blockIdx.x;
+        if (first >= all) return;
+        const long long stop = first + per < all ? first + per : all;
+        // the last pair whose pages (of all heads) begin at or in front of `first`; pairs without pages are passed over
+        int lo = 0, hi = pairs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if ((long long)list[mid] * kvh <= first) lo = mid;
+            else hi = mid;
         }
+        pair = lo;
+        const int in_pair = (int)(first - (long long)list[pair] * kvh);
+        item_of<COLS>(a, pair / a.col_tiles, pair % a.col_tiles, it);
+        it.h = in_pair / it.pages;
+        begin = in_pair % it.pages;
+        end = begin + (int)(stop - first);            // in pages from the item's start on; runs over into the following items
     }
-    if (lane == 0) s_m[warp] = mx, s_l[warp] = sum;
+    // moves on to the next item of the run: the next kv head, or the next pair that has pages
+    auto next_item = [&](Item &x, int &p) {
+        if (++x.h < kvh) return;
+        const int h0 = 0;
+        do ++p;
+        while (!item_of<COLS>(a, p / a.col_tiles, p % a.col_tiles, x));
+        x.h = h0;
+    };
+
+    if (warp == S::WARPS) {
+        // ---- the warp that fetches --------------------------------------------------------------------------------------------
+        int from = begin, left = end - begin, st = 0, phase = 1;
+        bool alive = true;
+        while (left > 0 && alive) {
+            const int n = min(left, it.pages - from);
+            for (int p0 = 0; p0 < n && alive; p0 += 32) {
+                // page numbers of the next 32 pages, one per lane
+                int page = -1;
+                if (p0 + lane < n && it.last >= 0) page = a.c.table[(size_t)it.b * a.c.max_pages + from + p0 + lane];
+                if (page >= a.c.pages) page = -1;
+                const int some = min(32, n - p0);
+                for (int j = 0; j < some; ++j) {
+                    const int pg = __shfl_sync(0xffffffffu, page, j);
+                    alive = mbar_wait(empty + 8 * st, phase);
+                    if (!alive) break;
+                    if (lane == 0) {
+                        s_valid[st] = pg >= 0;
+                        if (pg >= 0) {
+                            mbar_expect_tx(full + 8 * st, S::REC);
+                            bulk_copy(smem_u32(ring + st * S::REC), a.c.pool + ((size_t)pg * kvh + it.h) * S::REC, S::REC, full + 8 * st);
+                        } else {
+                            mbar_arrive(full + 8 * st);
+                        }
+                    }
+                    __syncwarp();
+                    if (++st == S::STAGES) st = 0, phase ^= 1;
+                }
+            }
+            left -= n;
+            from = 0;
+            if (left > 0) next_item(it, pair);
+        }
+        if (!alive) {   // the consumers gave up: what is on its way lands before the block ends
+            if (lane == 0) atomicExch(a.status, SAL_E_TIMEOUT);
+            for (int i = 0; i < S::STAGES; ++i) (void)mbar_wait(full + 8 * i, i < st ? phase ^ 1 : phase);
+        }
+        return;
+    }
+
+    // ---- the warps that compute ----------------------------------------------------------------------------------------------------
+    const int r = lane >> 2, c = lane & 3;
+    const int wk = warp % WK, wc = warp / WK;
+    const int krow = (r >> 1) + 4 * (r & 1);       // the key (of 8) that row r of a fragment stands for
+    int from = begin, left = end - begin, st = 0, phase = 0;
+    bool alive = true;
+    for (;;) {
+        const int n = min(left, it.pages - from);
+        const int base = from;
+        // columns of this warp: column j of the item is head j % rep of row j / rep
+        uint32_t qf[NT][HD / 16][2];
+        float qs[NT][2][G];
+        int lim[NT][2];
+        int low_lim = 0x7fffffff, top_lim = -1;     // positions up to low_lim are seen by all columns, none behind top_lim by any
+        const int cols = a.m * a.rep;
+        const int64_t first_pos = a.pos[it.b];
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-        s_o[warp][g * GROUP + 2 * lane] = o[g].x;
-        s_o[warp][g * GROUP + 2 * lane + 1] = o[g].y;
-    }
-    __syncthreads();
-    float all = s_m[0];
-    for (int w = 1; w < NW; ++w) all = fmaxf(all, s_m[w]);
-    float wgt[NW], total = 0.f;
-    for (int w = 0; w < NW; ++w) {
-        wgt[w] = s_l[w] == 0.f ? 0.f : s_m[w] == all ? 1.f : __expf(s_m[w] - all);
-        total += wgt[w] * s_l[w];
-    }
-    for (int d = threadIdx.x; d < HD; d += blockDim.x) {
-        float acc = 0.f;
-        for (int w = 0; w < NW; ++w) acc += wgt[w] * s_o[w][d];
-        out[((size_t)row * heads + head) * HD + d] = __float2half_rn(total == 0.f ? 0.f : acc / total);   // no position: zero
+        for (int nt = 0; nt < NT; ++nt) {
+            const int col0 = it.ct * COLS + (wc * NT + nt) * 8;
+            const int j = DUP ? it.ct * COLS + (r & 3) : col0 + r;
+            const int i = j / a.rep;
+            const bool there = j < cols && i < it.rows;
+            const __half *src = a.q + (((size_t)it.b * a.m + i) * a.heads + it.h * a.rep + j % a.rep) * HD + 16 * c;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+                if (there) x[0] = *reinterpret_cast<const uint4 *>(src + g * GROUP), x[1] = *reinterpret_cast<const uint4 *>(src + g * GROUP + 8);
+                float sum = 0.f;
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const uint32_t u[4] = {x[w].x, x[w].y, x[w].z, x[w].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 f = as_float2(u[e]);
+                        sum += f.x + f.y;
+                    }
+                    qf[nt][g * 4 + 2 * w][0] = prmt(u[0], u[2], 0x5410);
+                    qf[nt][g * 4 + 2 * w][1] = prmt(u[0], u[2], 0x7632);
+                    qf[nt][g * 4 + 2 * w + 1][0] = prmt(u[1], u[3], 0x5410);
+                    qf[nt][g * 4 + 2 * w + 1][1] = prmt(u[1], u[3], 0x7632);
+                }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                qs[nt][0][g] = __shfl_sync(0xffffffffu, sum, 8 * c);
+                qs[nt][1][g] = __shfl_sync(0xffffffffu, sum, 8 * c + 4);
+            }
+            const int l = there ? min(row_position(first_pos, i), a.c.max_pages * PAGE - 1) : -2;
+            low_lim = min(low_lim, (int)__reduce_min_sync(0xffffffffu, l == -2 ? 0x7fffffff : l));
+            top_lim = max(top_lim, (int)__reduce_max_sync(0xffffffffu, l));
+            lim[nt][0] = __shfl_sync(0xffffffffu, l, 8 * c);
+            lim[nt][1] = __shfl_sync(0xffffffffu, l, 8 * c + 4);
+        }
+        float acc[NT][HD / 16][4], accm[NT][2][G], mx[NT][2], sum[NT][2], big[G];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[nt][i][e] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                mx[nt][e] = -INFINITY, sum[nt][e] = 0.f;
+#pragma unroll
+                for (int g = 0; g < G; ++g) accm[nt][e][g] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) big[g] = 5.9604645e-8f;     // 2**-24, the smallest scale
+
+        for (int p = 0; p < n && alive; ++p) {
+            alive = mbar_wait(full + 8 * st, phase);
+            if (!alive) break;
+            const uint32_t rec = smem_u32(ring + st * S::REC);
+            if (s_valid[st]) {
+#pragma unroll 1
+                for (int kb = wk; kb < 4; kb += WK) {
+                    const int t0 = (base + p) * PAGE + 16 * kb;
+                    if (t0 > top_lim) break;
+                    const int key = 16 * kb + krow;
+                    // scores of 16 keys
+                    float s[NT][4];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+                    float vs[G][2], vm[G][2];      // of the two keys of this lane: scale of the values, lowest value + 8 scales
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const uint32_t at = rec + key * R::ROW + R::place(g, krow) * 32 + 8 * c;
+                        const uint2 x0 = lds64(at), x1 = lds64(at + 8 * R::ROW);
+                        const uint32_t par = rec + 2 * R::CODES + (key * G + g) * 4;
+                        const float2 k0 = as_float2(lds32(par)), k1 = as_float2(lds32(par + 8 * G * 4));
+                        const float2 v0 = as_float2(lds32(par + R::PARAMS)), v1 = as_float2(lds32(par + R::PARAMS + 8 * G * 4));
+                        vs[g][0] = v0.x, vs[g][1] = v1.x;
+                        vm[g][0] = fmaf(8.f, v0.x, v0.y), vm[g][1] = fmaf(8.f, v1.x, v1.y);
+                        float d[NT][4];
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) d[nt][e] = 0.f;
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) {
+                            const uint32_t y0 = w ? x0.y : x0.x, y1 = w ? x1.y : x1.x;
+#pragma unroll
+                            for (int t = 0; t < 2; ++t) {
+                                const uint32_t z0 = y0 >> (8 * t), z1 = y1 >> (8 * t);
+                                const uint32_t a0 = codes_low(z0), a1 = codes_low(z1), a2 = codes_mid(z0), a3 = codes_mid(z1);
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) mma16816(d[nt], a0, a1, a2, a3, qf[nt][g * 4 + 2 * w + t][0], qf[nt][g * 4 + 2 * w + t][1]);
+                            }
+                        }
+                        const float ks0 = k0.x * a.scale_log2, ks1 = k1.x * a.scale_log2;
+                        const float km0 = fmaf(8.f, k0.x, k0.y) * a.scale_log2, km1 = fmaf(8.f, k1.x, k1.y) * a.scale_log2;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            s[nt][0] += fmaf(ks0, d[nt][0], km0 * qs[nt][0][g]);
+                            s[nt][1] += fmaf(ks0, d[nt][1], km0 * qs[nt][1][g]);
+                            s[nt][2] += fmaf(ks1, d[nt][2], km1 * qs[nt][0][g]);
+                            s[nt][3] += fmaf(ks1, d[nt][3], km1 * qs[nt][1][g]);
+                        }
+                    }
+                    const bool masked = t0 + 15 > low_lim;
+                    if (masked) {      // what a column does not see weighs nothing, whatever its key and value are
+                        const int ta = t0 + krow, tb = ta + 8;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            if (ta > lim[nt][0]) s[nt][0] = -INFINITY;
+                            if (ta > lim[nt][1]) s[nt][1] = -INFINITY;
+                            if (tb > lim[nt][0]) s[nt][2] = -INFINITY;
+                            if (tb > lim[nt][1]) s[nt][3] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            if (ta > top_lim) vs[g][0] = vm[g][0] = 0.f;
+                            if (tb > top_lim) vs[g][1] = vm[g][1] = 0.f;
+                        }
+                    }
+                    // running maxima of the columns and of the scales
+                    float now[NT][2];
+                    bool moved = false;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float x = fmaxf(s[nt][e], s[nt][e + 2]);
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                            now[nt][e] = fmaxf(x, mx[nt][e]);
+                            moved |= now[nt][e] > mx[nt][e];
+                        }
+                    float grown[G];
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const float x0 = fabsf(vs[g][0]), x1 = fabsf(vs[g][1]);
+                        const float x = fmaxf(x0 <= 65504.f ? x0 : 0.f, x1 <= 65504.f ? x1 : 0.f);
+                        const uint32_t u = (__reduce_max_sync(0xffffffffu, __float_as_uint(x)) + 0x7fffffu) & 0x7f800000u;   // up to a power of two
+                        grown[g] = fmaxf(__uint_as_float(u), big[g]);
+                        moved |= grown[g] > big[g];
+                    }
+                    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float f = now[nt][e] == mx[nt][e] ? 1.f : exp2_approx(mx[nt][e] - now[nt][e]);
+                                mx[nt][e] = now[nt][e];
+                                sum[nt][e] *= f;
+#pragma unroll
+                                for (int g = 0; g < G; ++g) {
+                                    accm[nt][e][g] *= f;
+                                    const float fg = f * __fdividef(big[g], grown[g]);
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) acc[nt][4 * g + i][e] *= fg, acc[nt][4 * g + i][e + 2] *= fg;
+                                }
+                            }
+#pragma unroll
+                        for (int g = 0; g < G; ++g) big[g] = grown[g];
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float ref = mx[nt][e & 1];
+                            s[nt][e] = exp2_approx(s[nt][e] - (ref == -INFINITY ? 0.f : ref));
+                        }
+                        sum[nt][0] += s[nt][0] + s[nt][2];
+                        sum[nt][1] += s[nt][1] + s[nt][3];
+                    }
+                    // weighted values
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const float to = W_ONE / big[g];
+                        const float u0 = vs[g][0] * to, u1 = vs[g][1] * to;
+                        uint32_t b[NT][2], b2[NT][2];
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            float w[4] = {s[nt][0] * u0, s[nt][1] * u0, s[nt][2] * u1, s[nt][3] * u1};
+                            float l[4] = {s[nt][0] * vm[g][0], s[nt][1] * vm[g][0], s[nt][2] * vm[g][1], s[nt][3] * vm[g][1]};
+                            if (masked) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (s[nt][e] == 0.f) w[e] = l[e] = 0.f;
+                            }
+                            accm[nt][0][g] += l[0] + l[2];
+                            accm[nt][1][g] += l[1] + l[3];
+                            const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
+                            const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+                            const __half2 l0 = __floats2half2_rn(w[0] - f0.x, w[1] - f0.y), l1 = __floats2half2_rn(w[2] - f1.x, w[3] - f1.y);
+                            if (DUP) {
+                                b[nt][0] = transposed(as_u32(c < 2 ? h0 : l0));
+                                b[nt][1] = transposed(as_u32(c < 2 ? h1 : l1));
+                            } else {
+                                b[nt][0] = transposed(as_u32(h0)), b[nt][1] = transposed(as_u32(h1));
+                                b2[nt][0] = transposed(as_u32(l0)), b2[nt][1] = transposed(as_u32(l1));
+                            }
+                        }
+                        const uint32_t at = rec + R::CODES + (16 * kb + c) * R::ROW + 4 * r;
+                        const uint32_t pa = R::place(g, c) * 32, pb = R::place(g, c + 4) * 32;
+                        const uint32_t y0 = lds32(at + pa), y1 = lds32(at + 4 * R::ROW + pb), y2 = lds32(at + 8 * R::ROW + pa), y3 = lds32(at + 12 * R::ROW + pb);
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) {
+                            const uint32_t za = prmt(y0, y1, w ? 0x7632 : 0x5410), zb = prmt(y2, y3, w ? 0x7632 : 0x5410);
+#pragma unroll
+                            for (int t = 0; t < 2; ++t) {
+                                const uint32_t xa = za >> (8 * t), xb = zb >> (8 * t);
+                                const uint32_t a0 = codes_low(xa), a1 = codes_mid(xa), a2 = codes_low(xb), a3 = codes_mid(xb);
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    mma16816(acc[nt][4 * g + 2 * w + t], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+                                    if (!DUP) mma16816(acc[nt][4 * g + 2 * w + t], a0, a1, a2, a3, b2[nt][0], b2[nt][1]);
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + 8 * st);
+            if (++st == S::STAGES) st = 0, phase ^= 1;
+        }
+        if (!alive && lane == 0) atomicExch(a.status, SAL_E_TIMEOUT);   // and on to the end, past the same barriers
+
+        // ---- this block's part of the item: the warps' parts into shared memory, then added up -----------------------------------------
+        float *mine = merge + wk * S::PART;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float l = sum[nt][e];
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+                const int col = (wc * NT + nt) * 8 + 2 * c + e;
+                if (r == 0 && (!DUP || c < 2)) mine[COLS * HD + col] = mx[nt][e], mine[COLS * (HD + 1) + col] = l;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    float lowest = accm[nt][e][g];
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) lowest += __shfl_xor_sync(0xffffffffu, lowest, o);
+                    const float back = big[g] / W_ONE;
+                    float o8[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o8[2 * i] = acc[nt][4 * g + i][e], o8[2 * i + 1] = acc[nt][4 * g + i][e + 2];
+                    if (DUP) {      // first and second parts of the weights
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) o8[i] += __shfl_xor_sync(0xffffffffu, o8[i], 2);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o8[i] = fmaf(o8[i], back, lowest);
+                    if (!DUP || c < 2) {
+                        float4 *dst = reinterpret_cast<float4 *>(mine + col * HD + g * GROUP + 8 * r);
+                        dst[0] = make_float4(o8[0], o8[1], o8[2], o8[3]);
+                        dst[1] = make_float4(o8[4], o8[5], o8[6], o8[7]);
+                    }
+                }
+            }
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");
+        const bool all = from == 0 && n == it.pages;
+        // The blocks of an item are neighbours; a part lies in the block's first place if the item began in front of the block, else in its second.
+        float *part = a.parts + ((size_t)blockIdx.x * 2 + (from == 0 ? 1 : 0)) * S::PART;
+        for (int x = tid; x < COLS * HD; x += S::WARPS * 32) {
+            const int col = x / HD;
+            float top = merge[COLS * HD + col];
+#pragma unroll
+            for (int w = 1; w < WK; ++w) top = fmaxf(top, merge[w * S::PART + COLS * HD + col]);
+            float total = 0.f, o = 0.f;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) {
+                const float *m = merge + w * S::PART;
+                const float l = m[COLS * (HD + 1) + col];
+                const float f = l == 0.f ? 0.f : exp2_approx(m[COLS * HD + col] - top);
+                total += f * l;
+                o += l == 0.f ? 0.f : f * m[x];
+            }
+            if (all) {
+                const int j = it.ct * COLS + col;
+                if (j < cols && j / a.rep < it.rows)
+                    a.out[(((size_t)it.b * a.m + j / a.rep) * a.heads + it.h * a.rep + j % a.rep) * HD + x % HD] = __float2half_rn(total == 0.f ? 0.f : o / total);
+            } else {
+                __stcg(part + x, o);
+                if (x % HD == 0) __stcg(part + COLS * HD + col, top), __stcg(part + COLS * (HD + 1) + col, total);
+            }
+        }
+        if (!all) {
+            // first and last block that has pages of this item
+            const long long start = (long long)list[pair] * kvh + (long long)it.h * it.pages, all_pages = (long long)list[pairs] * kvh;
+            long long per = (all_pages + gridDim.x - 1) / gridDim.x;
+            if (per < MIN_PAGES) per = MIN_PAGES;
+            const int block0 = (int)(start / per), block1 = (int)((start + it.pages - 1) / per);
+            unsigned *counter = a.counters + (size_t)pair * kvh + it.h;
+            asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");
+            if (tid == 0) {
+                unsigned old;
+                asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+                s_flag = old == (unsigned)(block1 - block0);
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");
+            if (s_flag) {
+                for (int x = tid; x < COLS * HD; x += S::WARPS * 32) {
+                    const int col = x / HD, j = it.ct * COLS + col;
+                    if (j >= cols || j / a.rep >= it.rows) continue;
+                    float top = -INFINITY, total = 0.f, o = 0.f;
+                    for (int k = block0; k <= block1; ++k) {
+                        const float *m = a.parts + ((size_t)k * 2 + (k == block0 ? 1 : 0)) * S::PART;
+                        const float l = __ldcg(m + COLS * (HD + 1) + col), t = __ldcg(m + COLS * HD + col), v = __ldcg(m + x);
+                        if (l == 0.f) continue;
+                        const float next = fmaxf(top, t), f = exp2_approx(top - next), f2 = exp2_approx(t - next);
+                        top = next;
+                        total = total * f + l * f2;
+                        o = o * f + v * f2;
+                    }
+                    a.out[(((size_t)it.b * a.m + j / a.rep) * a.heads + it.h * a.rep + j % a.rep) * HD + x % HD] = __float2half_rn(total == 0.f ? 0.f : o / total);
+                }
+                if (tid == 0) *counter = 0;      // ready for the next launch
+            }
+        }
+        left -= n;
+        if (left <= 0) break;
+        from = 0;
+        next_item(it, pair);
+        asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");       // `merge` and `s_flag` are free again
     }
 }
 
@@ -271,9 +823,59 @@ bool aligned16(const void *a, const void *b = nullptr, const void *c = nullptr, 
 }
 int check_cache(int batch, int m, int kv_heads, int hd, int max_pages, int pages) {
     if (hd != 64 && hd != 128 && hd != 256) return SAL_E_UNSUPPORTED;
-    if (batch < 1 || m < 1 || kv_heads < 1 || kv_heads > 1024 || max_pages < 1 || max_pages > POS_LIMIT / PAGE || pages < 1) return SAL_E_SHAPE;
+    if (batch < 1 || m < 1 || kv_heads < 1 || kv_heads > 256 || max_pages < 1 || max_pages > MAX_PAGES || pages < 1) return SAL_E_SHAPE;
     if ((long long)batch * m > SAL_KV4_MAX_ROWS) return SAL_E_SHAPE;
     return SAL_OK;
+}
+
+enum AttnKind { FOUR_COLUMNS, EIGHT_COLUMNS, SIXTEEN_COLUMNS, MANY_COLUMNS };
+struct AttnPlan {
+    AttnKind kind;
+    int cols;          // columns of a tile
+    int col_tiles;     // of a sequence
+    int pairs;         // (sequence, column tile) pairs
+    int max_blocks;    // thread blocks that share the list
+};
+AttnPlan attention_plan(int batch, int m, int rep, int hd) {
+    const int cols = m * rep;
+    AttnPlan p = {};
+    p.kind = cols <= 4 ? FOUR_COLUMNS : cols <= 8 ? EIGHT_COLUMNS : cols <= 16 && hd < 256 ? SIXTEEN_COLUMNS : MANY_COLUMNS;
+    p.cols = p.kind == FOUR_COLUMNS ? 4 : p.kind == EIGHT_COLUMNS ? 8 : p.kind == SIXTEEN_COLUMNS ? 16 : hd < 256 ? 64 : 32;
+    p.col_tiles = (cols + p.cols - 1) / p.cols;
+    p.pairs = batch * p.col_tiles;
+    p.max_blocks = p.kind == MANY_COLUMNS ? 320 : 640;
+    return p;
+}
+
+template <int HD, int NT, bool DUP, int WK, int WC>
+int launch_tiles(const AttnArgs &a, const AttnPlan &p, void *stream) {
+    using S = AttnShape<HD, NT, DUP, WK, WC>;
+    auto kernel = attention_tiles_kernel<HD, NT, DUP, WK, WC>;
+    static std::atomic<bool> configured[64];
+    static std::atomic<int> resident[64];
+    if (sal_allow_shared_memory(kernel, configured) != cudaSuccess) return SAL_E_LAUNCH;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return SAL_E_DEVICE;
+    int blocks = resident[dev].load(std::memory_order_relaxed);
+    if (blocks == 0) {
+        int per_sm = 0, sms = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, S::THREADS, S::SMEM) != cudaSuccess || per_sm < 1) return SAL_E_LAUNCH;
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return SAL_E_LAUNCH;
+        blocks = per_sm * sms;
+        resident[dev].store(blocks, std::memory_order_relaxed);
+    }
+    const unsigned grid = a.whole ? (unsigned)p.pairs * a.c.kv_heads : (unsigned)(blocks < p.max_blocks ? blocks : p.max_blocks);
+    return sal_launch_pdl(kernel, dim3(grid), dim3(S::THREADS), S::SMEM, stream, a);
+}
+template <int HD>
+int launch_attention(const AttnArgs &a, const AttnPlan &p, void *stream) {
+    switch (p.kind) {
+        case FOUR_COLUMNS: return launch_tiles<HD, 1, true, 4, 1>(a, p, stream);
+        case EIGHT_COLUMNS: return launch_tiles<HD, 1, false, 4, 1>(a, p, stream);
+        case SIXTEEN_COLUMNS:
+            if constexpr (HD < 256) return launch_tiles<HD, 2, false, 4, 1>(a, p, stream);
+        default: return launch_tiles<HD, (HD < 256 ? 2 : 1), false, 1, 4>(a, p, stream);
+    }
 }
 
 }  // namespace
@@ -313,8 +915,9 @@ int sal_read_kv4(const void *pool, const int32_t *table, const int64_t *pos, voi
 }
 
 size_t sal_attention_kv4_workspace_bytes(int batch, int m, int heads, int kv_heads, int hd) {
-    if (batch < 1 || m < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || hd < 1) return 0;
-    return 1024;
+    if (check_cache(batch, m, kv_heads, hd, 1, 1) != SAL_OK || heads < 1 || heads > 16384 || heads % kv_heads) return 0;
+    const AttnPlan p = attention_plan(batch, m, heads / kv_heads, hd);
+    return WS_HEADER + ((size_t)(p.pairs < MAX_LIST ? p.pairs : MAX_LIST) * kv_heads * 4 + 255) / 256 * 256 + (size_t)p.max_blocks * 2 * p.cols * (hd + 2) * 4;
 }
 
 int sal_attention_kv4_f16(const void *q, const void *pool, const int32_t *table, const int64_t *pos, const int32_t *rows, void *out, int batch, int m,
@@ -326,10 +929,21 @@ int sal_attention_kv4_f16(const void *q, const void *pool, const int32_t *table,
     if (heads < 1 || heads > 16384 || heads % kv_heads) return SAL_E_SHAPE;
     if (!aligned16(q, pool, out, workspace)) return SAL_E_ALIGN;
     if (workspace_bytes < sal_attention_kv4_workspace_bytes(batch, m, heads, kv_heads, hd)) return SAL_E_WORKSPACE;
-    const CacheArgs c = {reinterpret_cast<uint8_t *>(const_cast<void *>(pool)), table, kv_heads, max_pages, pages};
-    auto kernel = hd == 64 ? attention_kv4_kernel<64> : hd == 128 ? attention_kv4_kernel<128> : attention_kv4_kernel<256>;
-    return sal_launch_pdl(kernel, dim3(heads, batch * m), dim3(128), 0, stream, reinterpret_cast<const __half *>(q), c, pos, rows,
-                          reinterpret_cast<__half *>(out), m, heads, scale);
+    const AttnPlan p = attention_plan(batch, m, heads / kv_heads, hd);
+    uint8_t *ws = reinterpret_cast<uint8_t *>(workspace);
+    AttnArgs a = {};
+    a.q = reinterpret_cast<const __half *>(q);
+    a.c = {reinterpret_cast<uint8_t *>(const_cast<void *>(pool)), table, kv_heads, max_pages, pages};
+    a.pos = pos, a.rows = rows;
+    a.out = reinterpret_cast<__half *>(out);
+    a.status = reinterpret_cast<int *>(ws);
+    a.counters = reinterpret_cast<unsigned *>(ws + WS_HEADER);
+    a.parts = reinterpret_cast<float *>(ws + WS_HEADER + ((size_t)(p.pairs < MAX_LIST ? p.pairs : MAX_LIST) * kv_heads * 4 + 255) / 256 * 256);
+    a.batch = batch, a.m = m, a.heads = heads, a.rep = heads / kv_heads;
+    a.col_tiles = p.col_tiles;
+    a.whole = p.pairs > MAX_LIST;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    return hd == 64 ? launch_attention<64>(a, p, stream) : hd == 128 ? launch_attention<128>(a, p, stream) : launch_attention<256>(a, p, stream);
 }
 
 int sal_copy_kv4_pages(void *pool, const int32_t *src, const int32_t *dst, int count, int layers, int pages, size_t page_bytes, void *stream) {
