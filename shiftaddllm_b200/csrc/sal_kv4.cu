@@ -778,20 +778,53 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
             }
             asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");
             if (s_flag) {
-                for (int x = tid; x < COLS * HD; x += S::WARPS * 32) {
+                // weight of a part: exp2(its maximum - the largest) / sum; a column's maxima and sums are read by one warp, a part per lane
+                const float *parts = a.parts + (size_t)(block0 + 1) * 2 * S::PART;      // of the blocks behind the first
+                const float *part0 = a.parts + ((size_t)block0 * 2 + 1) * S::PART;
+                const int more = block1 - block0;
+                for (int col = warp; col < COLS; col += S::WARPS) {
+                    float top = lane == 0 ? __ldcg(part0 + COLS * HD + col) : -INFINITY;
+                    for (int k = lane; k < more; k += 32) top = fmaxf(top, __ldcg(parts + (size_t)k * 2 * S::PART + COLS * HD + col));
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    float total = 0.f;
+                    for (int k = lane - 1; k < more; k += 32) {
+                        const float *m = k < 0 ? part0 : parts + (size_t)k * 2 * S::PART;
+                        const float l = __ldcg(m + COLS * (HD + 1) + col);
+                        if (l != 0.f) total += l * exp2_approx(__ldcg(m + COLS * HD + col) - top);
+                    }
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+                    if (lane == 0) merge[col] = top, merge[COLS + col] = total;
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");
+                for (int x = 4 * tid; x < COLS * HD; x += 4 * S::WARPS * 32) {
                     const int col = x / HD, j = it.ct * COLS + col;
                     if (j >= cols || j / a.rep >= it.rows) continue;
-                    float top = -INFINITY, total = 0.f, o = 0.f;
-                    for (int k = block0; k <= block1; ++k) {
-                        const float *m = a.parts + ((size_t)k * 2 + (k == block0 ? 1 : 0)) * S::PART;
-                        const float l = __ldcg(m + COLS * (HD + 1) + col), t = __ldcg(m + COLS * HD + col), v = __ldcg(m + x);
-                        if (l == 0.f) continue;
-                        const float next = fmaxf(top, t), f = exp2_approx(top - next), f2 = exp2_approx(t - next);
-                        top = next;
-                        total = total * f + l * f2;
-                        o = o * f + v * f2;
+                    const float top = merge[col], total = merge[COLS + col];
+                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int k0 = -1; k0 < more; k0 += 8) {
+                        float4 v[8];
+                        float f[8];
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {       // all loads first
+                            const int k = k0 + u;
+                            const float *m = k < 0 ? part0 : parts + (size_t)min(k, more - 1) * 2 * S::PART;
+                            v[u] = __ldcg(reinterpret_cast<const float4 *>(m + x));
+                            f[u] = __ldcg(m + COLS * HD + col);
+                        }
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            const float w = k0 + u < more ? exp2_approx(f[u] - top) : 0.f;
+                            if (w != 0.f) o.x += w * v[u].x, o.y += w * v[u].y, o.z += w * v[u].z, o.w += w * v[u].w;
+                        }
                     }
-                    a.out[(((size_t)it.b * a.m + j / a.rep) * a.heads + it.h * a.rep + j % a.rep) * HD + x % HD] = __float2half_rn(total == 0.f ? 0.f : o / total);
+                    const float inv = 1.f / total;
+                    if (total == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);      // no position: zero
+                    else o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+                    __half2 *dst = reinterpret_cast<__half2 *>(a.out + (((size_t)it.b * a.m + j / a.rep) * a.heads + it.h * a.rep + j % a.rep) * HD + x % HD);
+                    dst[0] = __floats2half2_rn(o.x, o.y);
+                    dst[1] = __floats2half2_rn(o.z, o.w);
                 }
                 if (tid == 0) *counter = 0;      // ready for the next launch
             }
