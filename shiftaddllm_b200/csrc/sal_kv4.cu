@@ -187,9 +187,8 @@ __global__ void __launch_bounds__(256) read_kv4_kernel(CacheArgs c, const int64_
 
 // ---- attention on the tensor cores -----------------------------------------------------------------------------------------------
 //
-// A score is scale * sum_g (s_g * D_g + (low_g + 8 s_g) * Q_g) with D_g = sum over the group of q * (code - 8) and Q_g = sum of q; an output is
-// sum_g E_g * A_g + sum_t p_t * (low_t + 8 s_t) with A_g = sum over positions of (p * s_g / E_g) * (code - 8).  The codes less 8 are whole
-// numbers of 16-bit floats without any error, so D_g and A_g are matrix products of 16-bit operands (m16n8k16, 32-bit sums) in which only the
+// A score is scale * sum_g (s_g * D_g + low_g * Q_g) with D_g = sum over the group of q * code and Q_g = sum of q; an output is
+// E_g * A_g + sum_t p_t * low_t with A_g = sum over positions of (p * s_g / E_g) * code.  The codes are 16-bit floats without any error, so D_g and A_g are matrix products of 16-bit operands (m16n8k16, 32-bit sums) in which only the
 // weight p * s is rounded; it goes in as the sum of two 16-bit numbers.  E_g, a power of two not below any scale so far, keeps the weights in
 // their range.  Neither keys nor values are ever formed.
 //
@@ -251,23 +250,34 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
     return v;
 }
+template <int G>
+__device__ __forceinline__ void lds_params(uint32_t (&p)[G], uint32_t a) {
+    if constexpr (G == 1) {
+        p[0] = lds32(a);
+    } else if constexpr (G == 2) {
+        const uint2 v = lds64(a);
+        p[0] = v.x, p[1] = v.y;
+    } else {
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(p[0]), "=r"(p[1]), "=r"(p[2]), "=r"(p[3]) : "r"(a));
+    }
+}
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Codes in bits 0..3 and 16..19 (low), or 4..7 and 20..23 (mid), as two 16-bit floats less 8: put under the exponent of 1024 they are
+// Codes in bits 0..3 and 16..19 (low), or 4..7 and 20..23 (mid), as two 16-bit floats: put under the exponent of 1024 they are
 // 1024 + code and 1024 + 16 code, exactly.
 __device__ __forceinline__ uint32_t codes_low(uint32_t x) {
     uint32_t h;
     asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(h) : "r"(x));
-    asm("add.rn.f16x2 %0, %0, %1;" : "+r"(h) : "r"(0xe408e408u));                      // - 1032
+    asm("add.rn.f16x2 %0, %0, %1;" : "+r"(h) : "r"(0xe400e400u));                      // - 1024
     return h;
 }
 __device__ __forceinline__ uint32_t codes_mid(uint32_t x) {
     uint32_t h;
     asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(h) : "r"(x));
-    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(h) : "r"(0x2c002c00u), "r"(0xd480d480u));   // / 16 - 72
+    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(h) : "r"(0x2c002c00u), "r"(0xd400d400u));   // / 16 - 64
     return h;
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -281,13 +291,15 @@ __device__ __forceinline__ uint32_t transposed(uint32_t a) {
     return d;
 }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+__device__ __forceinline__ __half2 as_half2(uint32_t h) { return *reinterpret_cast<__half2 *>(&h); }
 __device__ __forceinline__ float2 as_float2(uint32_t h) { return __half22float2(*reinterpret_cast<__half2 *>(&h)); }
 
 // Scratch: status word, counter of arrivals per item, then two parts per thread block.
 constexpr int WS_HEADER = 256;
 constexpr int MAX_LIST = 1024;        // (sequence, column tile) pairs whose work is dealt out; with more, a block takes an item
 constexpr int MIN_PAGES = 2;
-constexpr float W_ONE = 8192.f;       // a weight of 1 relative to E: well inside 16 bits, and small weights keep their bits
+constexpr float MOVE_AT = 8.f;        // weights stay below 2**8 ..
+constexpr float W_ONE = 64.f;         // .. and, times this, inside 16 bits; the second parts' last bit is then 2**-30 of a weight of 1
 
 struct AttnArgs {
     const __half *q;
@@ -511,7 +523,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
             lim[nt][0] = __shfl_sync(0xffffffffu, l, 8 * c);
             lim[nt][1] = __shfl_sync(0xffffffffu, l, 8 * c + 4);
         }
-        float acc[NT][HD / 16][4], accm[NT][2][G], mx[NT][2], sum[NT][2], big[G];
+        float acc[NT][HD / 16][4], accm[NT][2][G], ref[NT][2], over[NT][2], sum[NT][2], big[G], to_one[G];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -520,13 +532,16 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
                 for (int e = 0; e < 4; ++e) acc[nt][i][e] = 0.f;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                mx[nt][e] = -INFINITY, sum[nt][e] = 0.f;
+                ref[nt][e] = 0.f, over[nt][e] = -INFINITY, sum[nt][e] = 0.f;
 #pragma unroll
                 for (int g = 0; g < G; ++g) accm[nt][e][g] = 0.f;
             }
         }
 #pragma unroll
-        for (int g = 0; g < G; ++g) big[g] = 5.9604645e-8f;     // 2**-24, the smallest scale
+        for (int g = 0; g < G; ++g) big[g] = 6.1035156e-5f, to_one[g] = W_ONE / big[g];     // 2**-14
+        uint32_t big_h[(G + 1) / 2];                            // the same as pairs of 16-bit numbers
+#pragma unroll
+        for (int i = 0; i < (G + 1) / 2; ++i) big_h[i] = 0x04000400u;
 
         for (int p = 0; p < n && alive; ++p) {
             alive = mbar_wait(full + 8 * st, phase);
@@ -544,16 +559,14 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-                    float vs[G][2], vm[G][2];      // of the two keys of this lane: scale of the values, lowest value + 8 scales
+                    const uint32_t par = rec + 2 * R::CODES + key * G * 4;
+                    uint32_t k0[G], k1[G], v0[G], v1[G];      // (scale, lowest value) of the two keys of this lane
+                    lds_params<G>(k0, par), lds_params<G>(k1, par + 8 * G * 4);
+                    lds_params<G>(v0, par + R::PARAMS), lds_params<G>(v1, par + R::PARAMS + 8 * G * 4);
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
                         const uint32_t at = rec + key * R::ROW + R::place(g, krow) * 32 + 8 * c;
                         const uint2 x0 = lds64(at), x1 = lds64(at + 8 * R::ROW);
-                        const uint32_t par = rec + 2 * R::CODES + (key * G + g) * 4;
-                        const float2 k0 = as_float2(lds32(par)), k1 = as_float2(lds32(par + 8 * G * 4));
-                        const float2 v0 = as_float2(lds32(par + R::PARAMS)), v1 = as_float2(lds32(par + R::PARAMS + 8 * G * 4));
-                        vs[g][0] = v0.x, vs[g][1] = v1.x;
-                        vm[g][0] = fmaf(8.f, v0.x, v0.y), vm[g][1] = fmaf(8.f, v1.x, v1.y);
                         float d[NT][4];
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
@@ -570,104 +583,120 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
                                 for (int nt = 0; nt < NT; ++nt) mma16816(d[nt], a0, a1, a2, a3, qf[nt][g * 4 + 2 * w + t][0], qf[nt][g * 4 + 2 * w + t][1]);
                             }
                         }
-                        const float ks0 = k0.x * a.scale_log2, ks1 = k1.x * a.scale_log2;
-                        const float km0 = fmaf(8.f, k0.x, k0.y) * a.scale_log2, km1 = fmaf(8.f, k1.x, k1.y) * a.scale_log2;
+                        const float2 f0 = as_float2(k0[g]), f1 = as_float2(k1[g]);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            s[nt][0] += fmaf(ks0, d[nt][0], km0 * qs[nt][0][g]);
-                            s[nt][1] += fmaf(ks0, d[nt][1], km0 * qs[nt][1][g]);
-                            s[nt][2] += fmaf(ks1, d[nt][2], km1 * qs[nt][0][g]);
-                            s[nt][3] += fmaf(ks1, d[nt][3], km1 * qs[nt][1][g]);
+                            s[nt][0] = fmaf(f0.x, d[nt][0], fmaf(f0.y, qs[nt][0][g], s[nt][0]));
+                            s[nt][1] = fmaf(f0.x, d[nt][1], fmaf(f0.y, qs[nt][1][g], s[nt][1]));
+                            s[nt][2] = fmaf(f1.x, d[nt][2], fmaf(f1.y, qs[nt][0][g], s[nt][2]));
+                            s[nt][3] = fmaf(f1.x, d[nt][3], fmaf(f1.y, qs[nt][1][g], s[nt][3]));
                         }
                     }
                     const bool masked = t0 + 15 > low_lim;
+                    // A column's weights are powers relative to `ref`, which follows its largest score only when a weight would pass 2**8;
+                    // E likewise follows the scales.  Most blocks of keys move neither, which one vote finds out.
+                    bool moved = false;
+                    float z[NT][4];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) z[nt][e] = fmaf(s[nt][e], a.scale_log2, -ref[nt][e & 1]);
                     if (masked) {      // what a column does not see weighs nothing, whatever its key and value are
                         const int ta = t0 + krow, tb = ta + 8;
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            if (ta > lim[nt][0]) s[nt][0] = -INFINITY;
-                            if (ta > lim[nt][1]) s[nt][1] = -INFINITY;
-                            if (tb > lim[nt][0]) s[nt][2] = -INFINITY;
-                            if (tb > lim[nt][1]) s[nt][3] = -INFINITY;
+                            if (ta > lim[nt][0]) z[nt][0] = -INFINITY;
+                            if (ta > lim[nt][1]) z[nt][1] = -INFINITY;
+                            if (tb > lim[nt][0]) z[nt][2] = -INFINITY;
+                            if (tb > lim[nt][1]) z[nt][3] = -INFINITY;
                         }
 #pragma unroll
                         for (int g = 0; g < G; ++g) {
-                            if (ta > top_lim) vs[g][0] = vm[g][0] = 0.f;
-                            if (tb > top_lim) vs[g][1] = vm[g][1] = 0.f;
+                            if (ta > top_lim) v0[g] = 0;
+                            if (tb > top_lim) v1[g] = 0;
                         }
                     }
-                    // running maxima of the columns and of the scales
-                    float now[NT][2];
-                    bool moved = false;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float x = fmaxf(s[nt][e], s[nt][e + 2]);
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                            now[nt][e] = fmaxf(x, mx[nt][e]);
-                            moved |= now[nt][e] > mx[nt][e];
-                        }
-                    float grown[G];
+                        for (int e = 0; e < 4; ++e) moved |= z[nt][e] > over[nt][e & 1];
+                    if constexpr (G == 1) {
+                        moved |= !__hble2(as_half2(prmt(v0[0], v1[0], 0x5410)), as_half2(big_h[0]));
+                    } else {
 #pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        const float x0 = fabsf(vs[g][0]), x1 = fabsf(vs[g][1]);
-                        const float x = fmaxf(x0 <= 65504.f ? x0 : 0.f, x1 <= 65504.f ? x1 : 0.f);
-                        const uint32_t u = (__reduce_max_sync(0xffffffffu, __float_as_uint(x)) + 0x7fffffu) & 0x7f800000u;   // up to a power of two
-                        grown[g] = fmaxf(__uint_as_float(u), big[g]);
-                        moved |= grown[g] > big[g];
+                        for (int i = 0; i < G / 2; ++i) {
+                            const __half2 x = __hmax2_nan(as_half2(prmt(v0[2 * i], v0[2 * i + 1], 0x5410)), as_half2(prmt(v1[2 * i], v1[2 * i + 1], 0x5410)));
+                            moved |= !__hble2(x, as_half2(big_h[i]));
+                        }
                     }
                     if (__any_sync(0xffffffffu, moved)) {
+                        float fg[G];
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            const float x0 = fabsf(as_float2(v0[g]).x), x1 = fabsf(as_float2(v1[g]).x);
+                            const float x = fmaxf(x0 <= 65504.f ? x0 : 0.f, x1 <= 65504.f ? x1 : 0.f);
+                            const uint32_t u = (__reduce_max_sync(0xffffffffu, __float_as_uint(x)) + 0x7fffffu) & 0x7f800000u;   // up to a power of two
+                            const float grown = fminf(fmaxf(__uint_as_float(u), big[g]), 32768.f);
+                            fg[g] = __fdividef(big[g], grown);
+                            big[g] = grown, to_one[g] = __fdividef(W_ONE, grown);
+                            const uint32_t h = __half_as_ushort(__float2half_rn(grown));
+                            if (G == 1) big_h[0] = h * 0x10001u;
+                            else big_h[g / 2] = g & 1 ? prmt(big_h[g / 2], h, 0x5410) : prmt(big_h[g / 2], h, 0x3254);
+                        }
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                const float f = now[nt][e] == mx[nt][e] ? 1.f : exp2_approx(mx[nt][e] - now[nt][e]);
-                                mx[nt][e] = now[nt][e];
+                                float x = fmaxf(z[nt][e], z[nt][e + 2]);
+                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                                float f = 1.f;
+                                if (x > over[nt][e]) {
+                                    f = exp2_approx(-x);      // nothing was added up yet where `over` was -infinity
+                                    if (over[nt][e] == -INFINITY) f = 0.f;
+                                    ref[nt][e] += x, over[nt][e] = MOVE_AT;
+                                    if (z[nt][e] != -INFINITY) z[nt][e] = fmaf(s[nt][e], a.scale_log2, -ref[nt][e]);
+                                    if (z[nt][e + 2] != -INFINITY) z[nt][e + 2] = fmaf(s[nt][e + 2], a.scale_log2, -ref[nt][e]);
+                                }
                                 sum[nt][e] *= f;
 #pragma unroll
                                 for (int g = 0; g < G; ++g) {
                                     accm[nt][e][g] *= f;
-                                    const float fg = f * __fdividef(big[g], grown[g]);
 #pragma unroll
-                                    for (int i = 0; i < 4; ++i) acc[nt][4 * g + i][e] *= fg, acc[nt][4 * g + i][e + 2] *= fg;
+                                    for (int i = 0; i < 4; ++i) acc[nt][4 * g + i][e] *= f * fg[g], acc[nt][4 * g + i][e + 2] *= f * fg[g];
                                 }
                             }
-#pragma unroll
-                        for (int g = 0; g < G; ++g) big[g] = grown[g];
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float ref = mx[nt][e & 1];
-                            s[nt][e] = exp2_approx(s[nt][e] - (ref == -INFINITY ? 0.f : ref));
-                        }
-                        sum[nt][0] += s[nt][0] + s[nt][2];
-                        sum[nt][1] += s[nt][1] + s[nt][3];
+                        for (int e = 0; e < 4; ++e) z[nt][e] = exp2_approx(z[nt][e]);
+                        sum[nt][0] += z[nt][0] + z[nt][2];
+                        sum[nt][1] += z[nt][1] + z[nt][3];
                     }
                     // weighted values
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
-                        const float to = W_ONE / big[g];
-                        const float u0 = vs[g][0] * to, u1 = vs[g][1] * to;
+                        const float2 f0 = as_float2(v0[g]), f1 = as_float2(v1[g]);
+                        const float u0 = f0.x * to_one[g], u1 = f1.x * to_one[g];
                         uint32_t b[NT][2], b2[NT][2];
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            float w[4] = {s[nt][0] * u0, s[nt][1] * u0, s[nt][2] * u1, s[nt][3] * u1};
-                            float l[4] = {s[nt][0] * vm[g][0], s[nt][1] * vm[g][0], s[nt][2] * vm[g][1], s[nt][3] * vm[g][1]};
-                            if (masked) {
+                            float w[4] = {z[nt][0] * u0, z[nt][1] * u0, z[nt][2] * u1, z[nt][3] * u1};
+                            if (masked) {      // 0 times what is no number
 #pragma unroll
                                 for (int e = 0; e < 4; ++e)
-                                    if (s[nt][e] == 0.f) w[e] = l[e] = 0.f;
+                                    if (z[nt][e] == 0.f) w[e] = 0.f;
+                                accm[nt][0][g] += (z[nt][0] == 0.f ? 0.f : z[nt][0] * f0.y) + (z[nt][2] == 0.f ? 0.f : z[nt][2] * f1.y);
+                                accm[nt][1][g] += (z[nt][1] == 0.f ? 0.f : z[nt][1] * f0.y) + (z[nt][3] == 0.f ? 0.f : z[nt][3] * f1.y);
+                            } else {
+                                accm[nt][0][g] = fmaf(z[nt][0], f0.y, fmaf(z[nt][2], f1.y, accm[nt][0][g]));
+                                accm[nt][1][g] = fmaf(z[nt][1], f0.y, fmaf(z[nt][3], f1.y, accm[nt][1][g]));
                             }
-                            accm[nt][0][g] += l[0] + l[2];
-                            accm[nt][1][g] += l[1] + l[3];
                             const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
-                            const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
-                            const __half2 l0 = __floats2half2_rn(w[0] - f0.x, w[1] - f0.y), l1 = __floats2half2_rn(w[2] - f1.x, w[3] - f1.y);
+                            const float2 e0 = __half22float2(h0), e1 = __half22float2(h1);
+                            const __half2 l0 = __floats2half2_rn(w[0] - e0.x, w[1] - e0.y), l1 = __floats2half2_rn(w[2] - e1.x, w[3] - e1.y);
                             if (DUP) {
                                 b[nt][0] = transposed(as_u32(c < 2 ? h0 : l0));
                                 b[nt][1] = transposed(as_u32(c < 2 ? h1 : l1));
@@ -712,7 +741,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
                 const int col = (wc * NT + nt) * 8 + 2 * c + e;
-                if (r == 0 && (!DUP || c < 2)) mine[COLS * HD + col] = mx[nt][e], mine[COLS * (HD + 1) + col] = l;
+                if (r == 0 && (!DUP || c < 2)) mine[COLS * HD + col] = over[nt][e] == -INFINITY ? -INFINITY : ref[nt][e], mine[COLS * (HD + 1) + col] = l;
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
                     float lowest = accm[nt][e][g];
