@@ -266,24 +266,26 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Codes in bits 0..3 and 16..19 (low), or 4..7 and 20..23 (mid), as two 16-bit floats: put under the exponent of 1024 they are
-// 1024 + code and 1024 + 16 code, exactly.
+// Two codes of a word, in bits 4..7 and 20..23 (mid) or 0..3 and 16..19 (low), as two 16-bit floats of code * 2**-20.  The middle ones are that as
+// they stand: subnormal floats, exact, and exact in the products.  The low ones go over 1024 + code: as they stand (code * 2**-24) they would
+// cost the tensor core's sums four bits more, since it aligns a subnormal's product by its exponent and not by its first bit.
+__device__ __forceinline__ uint32_t codes_mid(uint32_t x) { return x & 0x00f000f0u; }
 __device__ __forceinline__ uint32_t codes_low(uint32_t x) {
     uint32_t h;
     asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(h) : "r"(x));
-    asm("add.rn.f16x2 %0, %0, %1;" : "+r"(h) : "r"(0xe400e400u));                      // - 1024
+    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(h) : "r"(0x00100010u), "r"(0x94009400u));   // * 2**-20 - 2**-10
     return h;
 }
-__device__ __forceinline__ uint32_t codes_mid(uint32_t x) {
-    uint32_t h;
-    asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(h) : "r"(x));
-    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(h) : "r"(0x2c002c00u), "r"(0xd400d400u));   // / 16 - 64
-    return h;
-}
+constexpr float UNIT = 1048576.f;
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
     uint32_t d;
@@ -297,7 +299,7 @@ __device__ __forceinline__ float2 as_float2(uint32_t h) { return __half22float2(
 // Scratch: status word, counter of arrivals per item, then two parts per thread block.
 constexpr int WS_HEADER = 256;
 constexpr int MAX_LIST = 1024;        // (sequence, column tile) pairs whose work is dealt out; with more, a block takes an item
-constexpr int MIN_PAGES = 2;
+constexpr int MIN_UNITS = 3;
 constexpr float MOVE_AT = 8.f;        // weights stay below 2**8 ..
 constexpr float W_ONE = 64.f;         // .. and, times this, inside 16 bits; the second parts' last bit is then 2**-30 of a weight of 1
 
@@ -313,7 +315,7 @@ struct AttnArgs {
     int batch, m, heads, rep;
     int col_tiles;      // column tiles of a sequence
     int whole;          // a block takes an item
-    float scale_log2;   // scale * log2(e)
+    float scale_log2;   // scale * log2(e) * UNIT
 };
 
 // NT column tiles of 8 per warp, WK warps that share a page's keys, WC warps side by side in columns.  DUP: at most four columns; the other
@@ -326,8 +328,10 @@ struct AttnShape {
     static constexpr int REC = Record<HD>::BYTES;
     static constexpr int PART = COLS * (HD + 2);                       // floats of a part: outputs, maxima, sums
     static constexpr int MERGE = WK * PART * 4;                        // bytes of the warps' parts
+    static constexpr bool QUERIES = WC == 1;                           // an item's queries travel with its first page
+    static constexpr int STAGE = REC + (QUERIES ? COLS * HD * 2 : 0);
     static constexpr int STAGES = (HD == 256 ? 3 : HD == 128 ? 4 : 6);
-    static constexpr int SMEM = STAGES * REC + MERGE + MAX_LIST * 4 + 16 + 256;
+    static constexpr int SMEM = STAGES * STAGE + MERGE + MAX_LIST * 4 + 16;
 };
 
 struct Item {
@@ -335,6 +339,7 @@ struct Item {
     int pages;          // pages that some column sees
     int last;           // last position that some column sees
     int rows;           // rows of the sequence
+    int first;          // position of its first row
 };
 
 // Rows of sequence b, and the last position that a column of tile ct sees (-1: none); false if the tile has no row.
@@ -344,20 +349,21 @@ __device__ __forceinline__ bool item_of(const AttnArgs &a, int b, int ct, Item &
     const int i0 = ct * COLS / a.rep;
     if (i0 >= it.rows) return false;
     const int i1 = min((ct * COLS + COLS - 1) / a.rep, it.rows - 1);
-    it.last = min(row_position(a.pos[b], i1), a.c.max_pages * PAGE - 1);
+    it.first = row_position(a.pos[b], 0);
+    it.last = min(it.first + i1, a.c.max_pages * PAGE - 1);
     it.pages = it.last < 0 ? 1 : it.last / PAGE + 1;
     return true;
 }
 
 template <int HD, int NT, bool DUP, int WK, int WC>
-__global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) attention_tiles_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD < 256 && NT == 1 ? 3 : 1)) attention_tiles_kernel(AttnArgs a) {
     using S = AttnShape<HD, NT, DUP, WK, WC>;
     using R = Record<HD>;
     constexpr int G = R::G, COLS = S::COLS;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring = smem;
-    float *merge = reinterpret_cast<float *>(smem + S::STAGES * S::REC);
-    int *list = reinterpret_cast<int *>(smem + S::STAGES * S::REC + S::MERGE);      // running number of pages in front of a pair, per kv head
+    float *merge = reinterpret_cast<float *>(smem + S::STAGES * S::STAGE);
+    int *list = reinterpret_cast<int *>(smem + S::STAGES * S::STAGE + S::MERGE);    // units in front of a pair, per kv head
     __shared__ uint64_t bars[2 * S::STAGES];
     __shared__ int s_valid[S::STAGES];
     __shared__ int s_scan[33];
@@ -371,19 +377,22 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
     pdl_prologue();
     const int kvh = a.c.kv_heads, pairs = a.batch * a.col_tiles;
     Item it = {};
-    int begin, end, pair;      // this block's run of the list, and the pair that it begins in
+    // The list counts an item as its pages and one unit more, which stands for what an item costs by itself (first page's wait, sum over
+    // the warps, output).  This block's run: `left` units from unit `at` of the item on.
+    int at, pair;
+    long long left, per = 0;
     if (a.whole) {
         pair = blockIdx.x / kvh;
         it.h = blockIdx.x % kvh;
         if (!item_of<COLS>(a, pair / a.col_tiles, pair % a.col_tiles, it)) return;
-        begin = 0, end = it.pages;
+        at = 0, left = it.pages + 1;
         __syncthreads();
     } else {
-        int total = 0;         // pages of all pairs, and in front of each
+        int total = 0;         // units of all pairs, and in front of each
         for (int i0 = 0; i0 < pairs; i0 += S::THREADS) {
             const int i = i0 + tid;
             Item x = {};
-            const int n = i < pairs && item_of<COLS>(a, i / a.col_tiles, i % a.col_tiles, x) ? x.pages : 0;
+            const int n = i < pairs && item_of<COLS>(a, i / a.col_tiles, i % a.col_tiles, x) ? x.pages + 1 : 0;
             int run = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -400,69 +409,70 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
             if (i < pairs) list[i] = front + run - n;
             __syncthreads();
         }
-        if (tid == 0) list[pairs] = total;
-        __syncthreads();
         const long long all = (long long)total * kvh;
-        long long per = (all + gridDim.x - 1) / gridDim.x;
-        if (per < MIN_PAGES) per = MIN_PAGES;
-        const long long first = per * blockIdx.x;
-        if (first >= all) return;
-        const long long stop = first + per < all ? first + per : all;
-        // the last pair whose pages (of all heads) begin at or in front of `first`; pairs without pages are passed over
+        per = (all + gridDim.x - 1) / gridDim.x;
+        if (per < MIN_UNITS) per = MIN_UNITS;
+        const long long begin = per * blockIdx.x;
+        if (begin >= all) return;
+        left = begin + per < all ? per : all - begin;
+        // the last pair whose units (of all heads) begin at or in front of `begin`: one that has some
         int lo = 0, hi = pairs;
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
-            if ((long long)list[mid] * kvh <= first) lo = mid;
+            if ((long long)list[mid] * kvh <= begin) lo = mid;
             else hi = mid;
         }
         pair = lo;
-        const int in_pair = (int)(first - (long long)list[pair] * kvh);
+        const int in_pair = (int)(begin - (long long)list[pair] * kvh);
         item_of<COLS>(a, pair / a.col_tiles, pair % a.col_tiles, it);
-        it.h = in_pair / it.pages;
-        begin = in_pair % it.pages;
-        end = begin + (int)(stop - first);            // in pages from the item's start on; runs over into the following items
+        it.h = in_pair / (it.pages + 1);
+        at = in_pair % (it.pages + 1);
     }
-    // moves on to the next item of the run: the next kv head, or the next pair that has pages
-    auto next_item = [&](Item &x, int &p) {
-        if (++x.h < kvh) return;
-        const int h0 = 0;
-        do ++p;
-        while (!item_of<COLS>(a, p / a.col_tiles, p % a.col_tiles, x));
-        x.h = h0;
+    // moves on to the next item: the next kv head, or the next pair that has rows
+    auto next_item = [&] {
+        left -= it.pages + 1 - at;
+        at = 0;
+        if (left <= 0 || ++it.h < kvh) return;
+        do ++pair;
+        while (!item_of<COLS>(a, pair / a.col_tiles, pair % a.col_tiles, it));
+        it.h = 0;
     };
+    const int cols = a.m * a.rep;
 
     if (warp == S::WARPS) {
         // ---- the warp that fetches --------------------------------------------------------------------------------------------
-        int from = begin, left = end - begin, st = 0, phase = 1;
+        int st = 0, phase = 1;
         bool alive = true;
-        while (left > 0 && alive) {
-            const int n = min(left, it.pages - from);
-            for (int p0 = 0; p0 < n && alive; p0 += 32) {
+        for (; left > 0 && alive; next_item()) {
+            const int from = max(at - 1, 0), upto = (int)min((long long)at + left, (long long)it.pages + 1) - 1;
+            for (int p0 = from; p0 < upto && alive; p0 += 32) {
                 // page numbers of the next 32 pages, one per lane
                 int page = -1;
-                if (p0 + lane < n && it.last >= 0) page = a.c.table[(size_t)it.b * a.c.max_pages + from + p0 + lane];
+                if (p0 + lane < upto && it.last >= 0) page = a.c.table[(size_t)it.b * a.c.max_pages + p0 + lane];
                 if (page >= a.c.pages) page = -1;
-                const int some = min(32, n - p0);
+                const int some = min(32, upto - p0);
                 for (int j = 0; j < some; ++j) {
                     const int pg = __shfl_sync(0xffffffffu, page, j);
                     alive = mbar_wait(empty + 8 * st, phase);
                     if (!alive) break;
+                    const uint32_t dst = smem_u32(ring + st * S::STAGE), bar = full + 8 * st;
+                    const bool queries = S::QUERIES && p0 + j == from;
+                    const int j0 = it.ct * COLS, j1 = min(min(j0 + COLS, cols), it.rows * a.rep);      // columns that are there
                     if (lane == 0) {
                         s_valid[st] = pg >= 0;
-                        if (pg >= 0) {
-                            mbar_expect_tx(full + 8 * st, S::REC);
-                            bulk_copy(smem_u32(ring + st * S::REC), a.c.pool + ((size_t)pg * kvh + it.h) * S::REC, S::REC, full + 8 * st);
-                        } else {
-                            mbar_arrive(full + 8 * st);
-                        }
+                        mbar_expect_tx(bar, (pg >= 0 ? S::REC : 0) + (queries ? (j1 - j0) * HD * 2 : 0));
+                        if (pg >= 0) bulk_copy(dst, a.c.pool + ((size_t)pg * kvh + it.h) * S::REC, S::REC, bar);
                     }
                     __syncwarp();
+                    if (queries) {      // heads of a row that share this kv head lie side by side
+                        const int i = j0 / a.rep + lane, c0 = max(i * a.rep, j0), c1 = min((i + 1) * a.rep, j1);
+                        if (c0 < c1)
+                            bulk_copy(dst + S::REC + (c0 - j0) * HD * 2, a.q + (((size_t)it.b * a.m + i) * a.heads + it.h * a.rep + (c0 - i * a.rep)) * HD,
+                                      (c1 - c0) * HD * 2, bar);
+                    }
                     if (++st == S::STAGES) st = 0, phase ^= 1;
                 }
             }
-            left -= n;
-            from = 0;
-            if (left > 0) next_item(it, pair);
         }
         if (!alive) {   // the consumers gave up: what is on its way lands before the block ends
             if (lane == 0) atomicExch(a.status, SAL_E_TIMEOUT);
@@ -475,25 +485,25 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
     const int r = lane >> 2, c = lane & 3;
     const int wk = warp % WK, wc = warp / WK;
     const int krow = (r >> 1) + 4 * (r & 1);       // the key (of 8) that row r of a fragment stands for
-    int from = begin, left = end - begin, st = 0, phase = 0;
+    int st = 0, phase = 0;
     bool alive = true;
-    for (;;) {
-        const int n = min(left, it.pages - from);
-        const int base = from;
+    for (; left > 0; next_item()) {
+        const int base = max(at - 1, 0), n = (int)min((long long)at + left, (long long)it.pages + 1) - 1 - base;
+        if (n <= 0) continue;       // the item's first unit only
+        if (S::QUERIES && alive) alive = mbar_wait(full + 8 * st, phase);
         // columns of this warp: column j of the item is head j % rep of row j / rep
         uint32_t qf[NT][HD / 16][2];
-        float qs[NT][2][G];
+        uint32_t qm[NT][(G + 1) / 2];      // sums of q over the groups, times 2**-6: first, second and third 16-bit parts in lanes c = 0, 1, 2
         int lim[NT][2];
         int low_lim = 0x7fffffff, top_lim = -1;     // positions up to low_lim are seen by all columns, none behind top_lim by any
-        const int cols = a.m * a.rep;
-        const int64_t first_pos = a.pos[it.b];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int col0 = it.ct * COLS + (wc * NT + nt) * 8;
             const int j = DUP ? it.ct * COLS + (r & 3) : col0 + r;
             const int i = j / a.rep;
             const bool there = j < cols && i < it.rows;
-            const __half *src = a.q + (((size_t)it.b * a.m + i) * a.heads + it.h * a.rep + j % a.rep) * HD + 16 * c;
+            const __half *src = S::QUERIES ? reinterpret_cast<const __half *>(ring + st * S::STAGE + S::REC) + (j - it.ct * COLS) * HD + 16 * c
+                                           : a.q + (((size_t)it.b * a.m + i) * a.heads + it.h * a.rep + j % a.rep) * HD + 16 * c;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
@@ -507,17 +517,19 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
                         const float2 f = as_float2(u[e]);
                         sum += f.x + f.y;
                     }
-                    qf[nt][g * 4 + 2 * w][0] = prmt(u[0], u[2], 0x5410);
-                    qf[nt][g * 4 + 2 * w][1] = prmt(u[0], u[2], 0x7632);
-                    qf[nt][g * 4 + 2 * w + 1][0] = prmt(u[1], u[3], 0x5410);
-                    qf[nt][g * 4 + 2 * w + 1][1] = prmt(u[1], u[3], 0x7632);
+                    qf[nt][g * 4][w] = prmt(u[0], u[2], 0x5410);
+                    qf[nt][g * 4 + 1][w] = prmt(u[0], u[2], 0x7632);
+                    qf[nt][g * 4 + 2][w] = prmt(u[1], u[3], 0x5410);
+                    qf[nt][g * 4 + 3][w] = prmt(u[1], u[3], 0x7632);
                 }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                qs[nt][0][g] = __shfl_sync(0xffffffffu, sum, 8 * c);
-                qs[nt][1][g] = __shfl_sync(0xffffffffu, sum, 8 * c + 4);
+                sum *= 0.015625f;
+                const float p1 = __half2float(__float2half_rn(sum)), p2 = __half2float(__float2half_rn(sum - p1));
+                const uint32_t h = __half_as_ushort(__float2half_rn(c == 0 ? p1 : c == 1 ? p2 : c == 2 ? sum - p1 - p2 : 0.f));
+                qm[nt][g / 2] = g & 1 ? qm[nt][g / 2] | h << 16 : h;
             }
-            const int l = there ? min(row_position(first_pos, i), a.c.max_pages * PAGE - 1) : -2;
+            const int l = there ? min(it.first + i, a.c.max_pages * PAGE - 1) : -2;
             low_lim = min(low_lim, (int)__reduce_min_sync(0xffffffffu, l == -2 ? 0x7fffffff : l));
             top_lim = max(top_lim, (int)__reduce_max_sync(0xffffffffu, l));
             lim[nt][0] = __shfl_sync(0xffffffffu, l, 8 * c);
@@ -546,50 +558,55 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
         for (int p = 0; p < n && alive; ++p) {
             alive = mbar_wait(full + 8 * st, phase);
             if (!alive) break;
-            const uint32_t rec = smem_u32(ring + st * S::REC);
+            const uint32_t rec = smem_u32(ring + st * S::STAGE);
             if (s_valid[st]) {
 #pragma unroll 1
                 for (int kb = wk; kb < 4; kb += WK) {
                     const int t0 = (base + p) * PAGE + 16 * kb;
                     if (t0 > top_lim) break;
                     const int key = 16 * kb + krow;
-                    // scores of 16 keys
-                    float s[NT][4];
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
                     const uint32_t par = rec + 2 * R::CODES + key * G * 4;
                     uint32_t k0[G], k1[G], v0[G], v1[G];      // (scale, lowest value) of the two keys of this lane
                     lds_params<G>(k0, par), lds_params<G>(k1, par + 8 * G * 4);
                     lds_params<G>(v0, par + R::PARAMS), lds_params<G>(v1, par + R::PARAMS + 8 * G * 4);
+                    // scores of 16 keys, times 2**-20: lowest values times sums of q, then group by group
+                    float s[NT][4];
+                    {
+                        const uint32_t zero = 0;
+                        const uint32_t a0 = G == 1 ? k0[0] >> 16 : prmt(k0[0], k0[G > 1], 0x7632), a1 = G == 1 ? k1[0] >> 16 : prmt(k1[0], k1[G > 1], 0x7632);
+                        const uint32_t a2 = G == 4 ? prmt(k0[2 % G], k0[3 % G], 0x7632) : zero, a3 = G == 4 ? prmt(k1[2 % G], k1[3 % G], 0x7632) : zero;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma16816_first(s[nt], a0, a1, a2, a3, qm[nt][0], G == 4 ? qm[nt][(G + 1) / 2 - 1] : zero);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[nt][e] *= 64.f / UNIT;
+                        }
+                    }
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
                         const uint32_t at = rec + key * R::ROW + R::place(g, krow) * 32 + 8 * c;
                         const uint2 x0 = lds64(at), x1 = lds64(at + 8 * R::ROW);
                         float d[NT][4];
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
+                        for (int t = 0; t < 2; ++t) {
+                            const uint32_t y0 = x0.x >> (8 * t), y1 = x1.x >> (8 * t), y2 = x0.y >> (8 * t), y3 = x1.y >> (8 * t);
+                            const uint32_t l0 = codes_low(y0), l1 = codes_low(y1), l2 = codes_low(y2), l3 = codes_low(y3);
+                            const uint32_t m0 = codes_mid(y0), m1 = codes_mid(y1), m2 = codes_mid(y2), m3 = codes_mid(y3);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) d[nt][e] = 0.f;
-#pragma unroll
-                        for (int w = 0; w < 2; ++w) {
-                            const uint32_t y0 = w ? x0.y : x0.x, y1 = w ? x1.y : x1.x;
-#pragma unroll
-                            for (int t = 0; t < 2; ++t) {
-                                const uint32_t z0 = y0 >> (8 * t), z1 = y1 >> (8 * t);
-                                const uint32_t a0 = codes_low(z0), a1 = codes_low(z1), a2 = codes_mid(z0), a3 = codes_mid(z1);
-#pragma unroll
-                                for (int nt = 0; nt < NT; ++nt) mma16816(d[nt], a0, a1, a2, a3, qf[nt][g * 4 + 2 * w + t][0], qf[nt][g * 4 + 2 * w + t][1]);
+                            for (int nt = 0; nt < NT; ++nt) {
+                                const uint32_t(&b)[2] = qf[nt][g * 4 + 2 * t], (&b2)[2] = qf[nt][g * 4 + 2 * t + 1];
+                                if (t == 0) mma16816_first(d[nt], l0, l1, l2, l3, b[0], b[1]);
+                                else mma16816(d[nt], l0, l1, l2, l3, b[0], b[1]);
+                                mma16816(d[nt], m0, m1, m2, m3, b2[0], b2[1]);
                             }
                         }
-                        const float2 f0 = as_float2(k0[g]), f1 = as_float2(k1[g]);
+                        const float f0 = as_float2(k0[g]).x, f1 = as_float2(k1[g]).x;
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            s[nt][0] = fmaf(f0.x, d[nt][0], fmaf(f0.y, qs[nt][0][g], s[nt][0]));
-                            s[nt][1] = fmaf(f0.x, d[nt][1], fmaf(f0.y, qs[nt][1][g], s[nt][1]));
-                            s[nt][2] = fmaf(f1.x, d[nt][2], fmaf(f1.y, qs[nt][0][g], s[nt][2]));
-                            s[nt][3] = fmaf(f1.x, d[nt][3], fmaf(f1.y, qs[nt][1][g], s[nt][3]));
+                            s[nt][0] = fmaf(f0, d[nt][0], s[nt][0]);
+                            s[nt][1] = fmaf(f0, d[nt][1], s[nt][1]);
+                            s[nt][2] = fmaf(f1, d[nt][2], s[nt][2]);
+                            s[nt][3] = fmaf(f1, d[nt][3], s[nt][3]);
                         }
                     }
                     const bool masked = t0 + 15 > low_lim;
@@ -747,7 +764,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
                     float lowest = accm[nt][e][g];
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) lowest += __shfl_xor_sync(0xffffffffu, lowest, o);
-                    const float back = big[g] / W_ONE;
+                    const float back = big[g] * (UNIT / W_ONE);
                     float o8[8];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o8[2 * i] = acc[nt][4 * g + i][e], o8[2 * i + 1] = acc[nt][4 * g + i][e + 2];
@@ -766,9 +783,9 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
             }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");
-        const bool all = from == 0 && n == it.pages;
+        const bool all = n == it.pages;
         // The blocks of an item are neighbours; a part lies in the block's first place if the item began in front of the block, else in its second.
-        float *part = a.parts + ((size_t)blockIdx.x * 2 + (from == 0 ? 1 : 0)) * S::PART;
+        float *part = a.parts + ((size_t)blockIdx.x * 2 + (at == 0 ? 1 : 0)) * S::PART;
         for (int x = tid; x < COLS * HD; x += S::WARPS * 32) {
             const int col = x / HD;
             float top = merge[COLS * HD + col];
@@ -794,10 +811,8 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
         }
         if (!all) {
             // first and last block that has pages of this item
-            const long long start = (long long)list[pair] * kvh + (long long)it.h * it.pages, all_pages = (long long)list[pairs] * kvh;
-            long long per = (all_pages + gridDim.x - 1) / gridDim.x;
-            if (per < MIN_PAGES) per = MIN_PAGES;
-            const int block0 = (int)(start / per), block1 = (int)((start + it.pages - 1) / per);
+            const long long start = (long long)list[pair] * kvh + (long long)it.h * (it.pages + 1);
+            const int block0 = (int)((start + 1) / per), block1 = (int)((start + it.pages) / per);
             unsigned *counter = a.counters + (size_t)pair * kvh + it.h;
             asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");
             if (tid == 0) {
@@ -809,7 +824,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
             if (s_flag) {
                 // weight of a part: exp2(its maximum - the largest) / sum; a column's maxima and sums are read by one warp, a part per lane
                 const float *parts = a.parts + (size_t)(block0 + 1) * 2 * S::PART;      // of the blocks behind the first
-                const float *part0 = a.parts + ((size_t)block0 * 2 + 1) * S::PART;
+                const float *part0 = a.parts + ((size_t)block0 * 2 + (start >= per * block0 ? 1 : 0)) * S::PART;
                 const int more = block1 - block0;
                 for (int col = warp; col < COLS; col += S::WARPS) {
                     float top = lane == 0 ? __ldcg(part0 + COLS * HD + col) : -INFINITY;
@@ -858,10 +873,6 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS) atten
                 if (tid == 0) *counter = 0;      // ready for the next launch
             }
         }
-        left -= n;
-        if (left <= 0) break;
-        from = 0;
-        next_item(it, pair);
         asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");       // `merge` and `s_flag` are free again
     }
 }
@@ -1004,7 +1015,7 @@ int sal_attention_kv4_f16(const void *q, const void *pool, const int32_t *table,
     a.batch = batch, a.m = m, a.heads = heads, a.rep = heads / kv_heads;
     a.col_tiles = p.col_tiles;
     a.whole = p.pairs > MAX_LIST;
-    a.scale_log2 = scale * 1.4426950408889634f;
+    a.scale_log2 = scale * (1.4426950408889634f * UNIT);
     return hd == 64 ? launch_attention<64>(a, p, stream) : hd == 128 ? launch_attention<128>(a, p, stream) : launch_attention<256>(a, p, stream);
 }
 
