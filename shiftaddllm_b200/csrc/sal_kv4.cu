@@ -327,7 +327,7 @@ struct AttnShape {
     static constexpr int THREADS = (WARPS + 1) * 32;
     static constexpr int REC = Record<HD>::BYTES;
     static constexpr int PART = COLS * (HD + 2);                       // floats of a part: outputs, maxima, sums
-    static constexpr int MERGE = WK * PART * 4;                        // bytes of the warps' parts
+    static constexpr int MERGE = WK > 1 ? WK * PART * 4 : 0;           // bytes of the warps' parts
     static constexpr bool QUERIES = WC == 1;                           // an item's queries travel with its first page
     static constexpr int STAGE = REC + (QUERIES ? COLS * HD * 2 : 0);
     static constexpr int STAGES = (HD == 256 ? 3 : HD == 128 ? 4 : 6);
@@ -355,6 +355,13 @@ __device__ __forceinline__ bool item_of(const AttnArgs &a, int b, int ct, Item &
     return true;
 }
 
+__device__ __forceinline__ void store_output(__half *dst, float4 o, float total) {
+    const float inv = 1.f / total;
+    if (total == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);      // no position: zeros
+    else o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+    *reinterpret_cast<uint2 *>(dst) = make_uint2(as_u32(__floats2half2_rn(o.x, o.y)), as_u32(__floats2half2_rn(o.z, o.w)));
+}
+
 template <int HD, int NT, bool DUP, int WK, int WC>
 __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD < 256 && NT == 1 ? 3 : 1)) attention_tiles_kernel(AttnArgs a) {
     using S = AttnShape<HD, NT, DUP, WK, WC>;
@@ -368,6 +375,8 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
     __shared__ int s_valid[S::STAGES];
     __shared__ int s_scan[33];
     __shared__ int s_flag;
+    __shared__ float s_top[S::COLS], s_total[S::COLS];
+    __shared__ long long s_out[S::COLS];       // where a column's output lies
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t full = smem_u32(bars), empty = full + 8 * S::STAGES;
     if (tid == 0) {
@@ -490,6 +499,11 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
     for (; left > 0; next_item()) {
         const int base = max(at - 1, 0), n = (int)min((long long)at + left, (long long)it.pages + 1) - 1 - base;
         if (n <= 0) continue;       // the item's first unit only
+        const int there = min(min(COLS, cols - it.ct * COLS), it.rows * a.rep - it.ct * COLS);      // columns of the item
+        if (tid < there) {
+            const int j = it.ct * COLS + tid;
+            s_out[tid] = (((long long)it.b * a.m + j / a.rep) * a.heads + it.h * a.rep + j % a.rep) * HD;
+        }
         if (S::QUERIES && alive) alive = mbar_wait(full + 8 * st, phase);
         // columns of this warp: column j of the item is head j % rep of row j / rep
         uint32_t qf[NT][HD / 16][2];
@@ -501,13 +515,13 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
             const int col0 = it.ct * COLS + (wc * NT + nt) * 8;
             const int j = DUP ? it.ct * COLS + (r & 3) : col0 + r;
             const int i = j / a.rep;
-            const bool there = j < cols && i < it.rows;
+            const bool real = j - it.ct * COLS < there;
             const __half *src = S::QUERIES ? reinterpret_cast<const __half *>(ring + st * S::STAGE + S::REC) + (j - it.ct * COLS) * HD + 16 * c
                                            : a.q + (((size_t)it.b * a.m + i) * a.heads + it.h * a.rep + j % a.rep) * HD + 16 * c;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-                if (there) x[0] = *reinterpret_cast<const uint4 *>(src + g * GROUP), x[1] = *reinterpret_cast<const uint4 *>(src + g * GROUP + 8);
+                if (real) x[0] = *reinterpret_cast<const uint4 *>(src + g * GROUP), x[1] = *reinterpret_cast<const uint4 *>(src + g * GROUP + 8);
                 float sum = 0.f;
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
@@ -529,7 +543,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
                 const uint32_t h = __half_as_ushort(__float2half_rn(c == 0 ? p1 : c == 1 ? p2 : c == 2 ? sum - p1 - p2 : 0.f));
                 qm[nt][g / 2] = g & 1 ? qm[nt][g / 2] | h << 16 : h;
             }
-            const int l = there ? min(it.first + i, a.c.max_pages * PAGE - 1) : -2;
+            const int l = real ? min(it.first + i, a.c.max_pages * PAGE - 1) : -2;
             low_lim = min(low_lim, (int)__reduce_min_sync(0xffffffffu, l == -2 ? 0x7fffffff : l));
             top_lim = max(top_lim, (int)__reduce_max_sync(0xffffffffu, l));
             lim[nt][0] = __shfl_sync(0xffffffffu, l, 8 * c);
@@ -748,8 +762,12 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
         }
         if (!alive && lane == 0) atomicExch(a.status, SAL_E_TIMEOUT);   // and on to the end, past the same barriers
 
-        // ---- this block's part of the item: the warps' parts into shared memory, then added up -----------------------------------------
+        // ---- this block's part of the item, into the output or into scratch ---------------------------------------------------------------
+        const bool all = n == it.pages;
+        // The blocks of an item are neighbours; a part lies in the block's first place if the item began in front of the block, else in its second.
+        float *part = a.parts + ((size_t)blockIdx.x * 2 + (at == 0 ? 1 : 0)) * S::PART;
         float *mine = merge + wk * S::PART;
+        if (WK == 1) asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");      // s_out is written
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -758,7 +776,13 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
                 const int col = (wc * NT + nt) * 8 + 2 * c + e;
-                if (r == 0 && (!DUP || c < 2)) mine[COLS * HD + col] = over[nt][e] == -INFINITY ? -INFINITY : ref[nt][e], mine[COLS * (HD + 1) + col] = l;
+                const float top = over[nt][e] == -INFINITY ? -INFINITY : ref[nt][e];
+                if (WK > 1) {
+                    if (r == 0 && (!DUP || c < 2)) mine[COLS * HD + col] = top, mine[COLS * (HD + 1) + col] = l;
+                } else if (!all && r == 0) {
+                    __stcg(part + COLS * HD + col, top), __stcg(part + COLS * (HD + 1) + col, l);
+                }
+                const float inv = 1.f / l;
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
                     float lowest = accm[nt][e][g];
@@ -774,7 +798,23 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
                     }
 #pragma unroll
                     for (int i = 0; i < 8; ++i) o8[i] = fmaf(o8[i], back, lowest);
-                    if (!DUP || c < 2) {
+                    if (WK == 1 && all) {
+                        if (col < there) {
+                            if (l == 0.f) {      // no position: zeros
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) o8[i] = 0.f;
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) o8[i] *= inv;
+                            }
+                            *reinterpret_cast<uint4 *>(a.out + s_out[col] + g * GROUP + 8 * r) =
+                                make_uint4(as_u32(__floats2half2_rn(o8[0], o8[1])), as_u32(__floats2half2_rn(o8[2], o8[3])),
+                                           as_u32(__floats2half2_rn(o8[4], o8[5])), as_u32(__floats2half2_rn(o8[6], o8[7])));
+                        }
+                    } else if (WK == 1) {
+                        float4 *dst = reinterpret_cast<float4 *>(part + col * HD + g * GROUP + 8 * r);
+                        if (col < there) __stcg(dst, make_float4(o8[0], o8[1], o8[2], o8[3])), __stcg(dst + 1, make_float4(o8[4], o8[5], o8[6], o8[7]));
+                    } else if (!DUP || c < 2) {
                         float4 *dst = reinterpret_cast<float4 *>(mine + col * HD + g * GROUP + 8 * r);
                         dst[0] = make_float4(o8[0], o8[1], o8[2], o8[3]);
                         dst[1] = make_float4(o8[4], o8[5], o8[6], o8[7]);
@@ -782,31 +822,28 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
                 }
             }
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");
-        const bool all = n == it.pages;
-        // The blocks of an item are neighbours; a part lies in the block's first place if the item began in front of the block, else in its second.
-        float *part = a.parts + ((size_t)blockIdx.x * 2 + (at == 0 ? 1 : 0)) * S::PART;
-        for (int x = tid; x < COLS * HD; x += S::WARPS * 32) {
-            const int col = x / HD;
-            float top = merge[COLS * HD + col];
+        if (WK > 1) {
+            asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");
+            for (int x = 4 * tid; x < there * HD; x += 4 * S::WARPS * 32) {
+                const int col = x / HD;
+                float t[WK], l[WK], top = -INFINITY, total = 0.f;
 #pragma unroll
-            for (int w = 1; w < WK; ++w) top = fmaxf(top, merge[w * S::PART + COLS * HD + col]);
-            float total = 0.f, o = 0.f;
+                for (int w = 0; w < WK; ++w) t[w] = merge[w * S::PART + COLS * HD + col], l[w] = merge[w * S::PART + COLS * (HD + 1) + col], top = fmaxf(top, t[w]);
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < WK; ++w) {
-                const float *m = merge + w * S::PART;
-                const float l = m[COLS * (HD + 1) + col];
-                const float f = l == 0.f ? 0.f : exp2_approx(m[COLS * HD + col] - top);
-                total += f * l;
-                o += l == 0.f ? 0.f : f * m[x];
-            }
-            if (all) {
-                const int j = it.ct * COLS + col;
-                if (j < cols && j / a.rep < it.rows)
-                    a.out[(((size_t)it.b * a.m + j / a.rep) * a.heads + it.h * a.rep + j % a.rep) * HD + x % HD] = __float2half_rn(total == 0.f ? 0.f : o / total);
-            } else {
-                __stcg(part + x, o);
-                if (x % HD == 0) __stcg(part + COLS * HD + col, top), __stcg(part + COLS * (HD + 1) + col, total);
+                for (int w = 0; w < WK; ++w) {
+                    if (l[w] == 0.f) continue;
+                    const float f = exp2_approx(t[w] - top);
+                    const float4 v = *reinterpret_cast<const float4 *>(merge + w * S::PART + x);
+                    total += f * l[w];
+                    o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+                }
+                if (all) {
+                    store_output(a.out + s_out[col] + x % HD, o, total);
+                } else {
+                    __stcg(reinterpret_cast<float4 *>(part + x), o);
+                    if (x % HD == 0) __stcg(part + COLS * HD + col, top), __stcg(part + COLS * (HD + 1) + col, total);
+                }
             }
         }
         if (!all) {
@@ -826,7 +863,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
                 const float *parts = a.parts + (size_t)(block0 + 1) * 2 * S::PART;      // of the blocks behind the first
                 const float *part0 = a.parts + ((size_t)block0 * 2 + (start >= per * block0 ? 1 : 0)) * S::PART;
                 const int more = block1 - block0;
-                for (int col = warp; col < COLS; col += S::WARPS) {
+                for (int col = warp; col < there; col += S::WARPS) {
                     float top = lane == 0 ? __ldcg(part0 + COLS * HD + col) : -INFINITY;
                     for (int k = lane; k < more; k += 32) top = fmaxf(top, __ldcg(parts + (size_t)k * 2 * S::PART + COLS * HD + col));
 #pragma unroll
@@ -839,36 +876,35 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
                     }
 #pragma unroll
                     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-                    if (lane == 0) merge[col] = top, merge[COLS + col] = total;
+                    if (lane == 0) s_top[col] = top, s_total[col] = total;
                 }
                 asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");
-                for (int x = 4 * tid; x < COLS * HD; x += 4 * S::WARPS * 32) {
-                    const int col = x / HD, j = it.ct * COLS + col;
-                    if (j >= cols || j / a.rep >= it.rows) continue;
-                    const float top = merge[col], total = merge[COLS + col];
-                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int k0 = -1; k0 < more; k0 += 8) {
-                        float4 v[8];
-                        float f[8];
+                constexpr int LOADS = 8, STEP = 4 * S::WARPS * 32;
+                for (int x = 4 * tid; x < there * HD; x += 2 * STEP) {
+                    // two pieces of four outputs, eight parts of each at a time: all loads first
+                    const bool two = x + STEP < there * HD;
+                    const int x1 = two ? x + STEP : x, col = x / HD, col1 = x1 / HD;
+                    const float top = s_top[col], top1 = s_top[col1];
+                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f), o1 = o;
+                    for (int k0 = -1; k0 < more; k0 += LOADS) {
+                        float4 v[LOADS], v1[LOADS];
+                        float f[LOADS], f1[LOADS];
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) {       // all loads first
-                            const int k = k0 + u;
-                            const float *m = k < 0 ? part0 : parts + (size_t)min(k, more - 1) * 2 * S::PART;
-                            v[u] = __ldcg(reinterpret_cast<const float4 *>(m + x));
-                            f[u] = __ldcg(m + COLS * HD + col);
+                        for (int u = 0; u < LOADS; ++u) {
+                            const int k = min(k0 + u, more - 1);
+                            const float *m = k < 0 ? part0 : parts + (size_t)k * 2 * S::PART;
+                            v[u] = __ldcg(reinterpret_cast<const float4 *>(m + x)), v1[u] = __ldcg(reinterpret_cast<const float4 *>(m + x1));
+                            f[u] = __ldcg(m + COLS * HD + col), f1[u] = __ldcg(m + COLS * HD + col1);
                         }
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) {
-                            const float w = k0 + u < more ? exp2_approx(f[u] - top) : 0.f;
+                        for (int u = 0; u < LOADS; ++u) {
+                            const float w = k0 + u < more ? exp2_approx(f[u] - top) : 0.f, w1 = k0 + u < more ? exp2_approx(f1[u] - top1) : 0.f;
                             if (w != 0.f) o.x += w * v[u].x, o.y += w * v[u].y, o.z += w * v[u].z, o.w += w * v[u].w;
+                            if (w1 != 0.f) o1.x += w1 * v1[u].x, o1.y += w1 * v1[u].y, o1.z += w1 * v1[u].z, o1.w += w1 * v1[u].w;
                         }
                     }
-                    const float inv = 1.f / total;
-                    if (total == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);      // no position: zero
-                    else o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
-                    __half2 *dst = reinterpret_cast<__half2 *>(a.out + (((size_t)it.b * a.m + j / a.rep) * a.heads + it.h * a.rep + j % a.rep) * HD + x % HD);
-                    dst[0] = __floats2half2_rn(o.x, o.y);
-                    dst[1] = __floats2half2_rn(o.z, o.w);
+                    store_output(a.out + s_out[col] + x % HD, o, s_total[col]);
+                    if (two) store_output(a.out + s_out[col1] + x1 % HD, o1, s_total[col1]);
                 }
                 if (tid == 0) *counter = 0;      // ready for the next launch
             }
@@ -912,12 +948,18 @@ struct AttnPlan {
 AttnPlan attention_plan(int batch, int m, int rep, int hd) {
     const int cols = m * rep;
     AttnPlan p = {};
-    p.kind = cols <= 4 ? FOUR_COLUMNS : cols <= 8 ? EIGHT_COLUMNS : cols <= 16 && hd < 256 ? SIXTEEN_COLUMNS : MANY_COLUMNS;
+    p.kind = cols <= 4 ? FOUR_COLUMNS : cols <= (hd < 256 ? 8 : 32) ? EIGHT_COLUMNS : cols <= 64 && hd < 256 ? SIXTEEN_COLUMNS : MANY_COLUMNS;
     p.cols = p.kind == FOUR_COLUMNS ? 4 : p.kind == EIGHT_COLUMNS ? 8 : p.kind == SIXTEEN_COLUMNS ? 16 : hd < 256 ? 64 : 32;
     p.col_tiles = (cols + p.cols - 1) / p.cols;
     p.pairs = batch * p.col_tiles;
     p.max_blocks = p.kind == MANY_COLUMNS ? 320 : 640;
     return p;
+}
+
+// Counters of the items that can be shared.  Fewer rows a sequence need no more: up to four narrow tiles stand where a wide one does.
+size_t counter_bytes(const AttnPlan &p, int batch, int kv_heads) {
+    const long long pairs = p.pairs > 4LL * batch ? p.pairs : 4LL * batch;
+    return ((size_t)(pairs < MAX_LIST ? pairs : MAX_LIST) * kv_heads * 4 + 255) / 256 * 256;
 }
 
 template <int HD, int NT, bool DUP, int WK, int WC>
@@ -990,7 +1032,7 @@ int sal_read_kv4(const void *pool, const int32_t *table, const int64_t *pos, voi
 size_t sal_attention_kv4_workspace_bytes(int batch, int m, int heads, int kv_heads, int hd) {
     if (check_cache(batch, m, kv_heads, hd, 1, 1) != SAL_OK || heads < 1 || heads > 16384 || heads % kv_heads) return 0;
     const AttnPlan p = attention_plan(batch, m, heads / kv_heads, hd);
-    return WS_HEADER + ((size_t)(p.pairs < MAX_LIST ? p.pairs : MAX_LIST) * kv_heads * 4 + 255) / 256 * 256 + (size_t)p.max_blocks * 2 * p.cols * (hd + 2) * 4;
+    return WS_HEADER + counter_bytes(p, batch, kv_heads) + (size_t)p.max_blocks * 2 * p.cols * (hd + 2) * 4;
 }
 
 int sal_attention_kv4_f16(const void *q, const void *pool, const int32_t *table, const int64_t *pos, const int32_t *rows, void *out, int batch, int m,
@@ -1011,7 +1053,7 @@ int sal_attention_kv4_f16(const void *q, const void *pool, const int32_t *table,
     a.out = reinterpret_cast<__half *>(out);
     a.status = reinterpret_cast<int *>(ws);
     a.counters = reinterpret_cast<unsigned *>(ws + WS_HEADER);
-    a.parts = reinterpret_cast<float *>(ws + WS_HEADER + ((size_t)(p.pairs < MAX_LIST ? p.pairs : MAX_LIST) * kv_heads * 4 + 255) / 256 * 256);
+    a.parts = reinterpret_cast<float *>(ws + WS_HEADER + counter_bytes(p, batch, kv_heads));
     a.batch = batch, a.m = m, a.heads = heads, a.rep = heads / kv_heads;
     a.col_tiles = p.col_tiles;
     a.whole = p.pairs > MAX_LIST;
