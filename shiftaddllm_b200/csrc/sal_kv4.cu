@@ -35,6 +35,7 @@ struct Record {
         const int f = (p & 3) ^ ((p >> 1) & 2);
         return G == 4 ? g ^ f : G == 2 ? g ^ (f >> 1) : 0;
     }
+    static constexpr int FOUR_ON = G / 2;            // place(g, p + 4) = place(g ^ FOUR_ON, p), place(g, p + 8) = place(g, p)
 };
 
 // a * c - b * s to the nearest 32-bit number of the exact sum (products split into value and error), then to 16 bits: the same
@@ -363,7 +364,7 @@ __device__ __forceinline__ void store_output(__half *dst, float4 o, float total)
 }
 
 template <int HD, int NT, bool DUP, int WK, int WC>
-__global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD < 256 && NT == 1 ? 3 : 1)) attention_tiles_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD < 256 && NT == 1 ? 3 : 2)) attention_tiles_kernel(AttnArgs a) {
     using S = AttnShape<HD, NT, DUP, WK, WC>;
     using R = Record<HD>;
     constexpr int G = R::G, COLS = S::COLS;
@@ -494,6 +495,9 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
     const int r = lane >> 2, c = lane & 3;
     const int wk = warp % WK, wc = warp / WK;
     const int krow = (r >> 1) + 4 * (r & 1);       // the key (of 8) that row r of a fragment stands for
+    // where this lane's codes and parameters lie in a record; group g of a key's or value's row: that address ^ 32 g, rows being aligned
+    const uint32_t k_lane = (16 * wk + krow) * R::ROW + R::place(0, krow) * 32 + 8 * c, p_lane = 2 * R::CODES + (16 * wk + krow) * G * 4;
+    const uint32_t v_lane = R::CODES + (16 * wk + c) * R::ROW + R::place(0, c) * 32 + 4 * r;
     int st = 0, phase = 0;
     bool alive = true;
     for (; left > 0; next_item()) {
@@ -575,11 +579,11 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
             const uint32_t rec = smem_u32(ring + st * S::STAGE);
             if (s_valid[st]) {
 #pragma unroll 1
-                for (int kb = wk; kb < 4; kb += WK) {
-                    const int t0 = (base + p) * PAGE + 16 * kb;
+                for (int i = 0; i < 4 / WK; ++i) {
+                    const int t0 = (base + p) * PAGE + 16 * (wk + WK * i);
                     if (t0 > top_lim) break;
-                    const int key = 16 * kb + krow;
-                    const uint32_t par = rec + 2 * R::CODES + key * G * 4;
+                    const uint32_t k_at = rec + k_lane + i * (16 * WK * R::ROW), v_at = rec + v_lane + i * (16 * WK * R::ROW);
+                    const uint32_t par = rec + p_lane + i * (16 * WK * G * 4);
                     uint32_t k0[G], k1[G], v0[G], v1[G];      // (scale, lowest value) of the two keys of this lane
                     lds_params<G>(k0, par), lds_params<G>(k1, par + 8 * G * 4);
                     lds_params<G>(v0, par + R::PARAMS), lds_params<G>(v1, par + R::PARAMS + 8 * G * 4);
@@ -598,7 +602,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
                     }
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
-                        const uint32_t at = rec + key * R::ROW + R::place(g, krow) * 32 + 8 * c;
+                        const uint32_t at = k_at ^ (32 * g);
                         const uint2 x0 = lds64(at), x1 = lds64(at + 8 * R::ROW);
                         float d[NT][4];
 #pragma unroll
@@ -736,9 +740,8 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
                                 b2[nt][0] = transposed(as_u32(l0)), b2[nt][1] = transposed(as_u32(l1));
                             }
                         }
-                        const uint32_t at = rec + R::CODES + (16 * kb + c) * R::ROW + 4 * r;
-                        const uint32_t pa = R::place(g, c) * 32, pb = R::place(g, c + 4) * 32;
-                        const uint32_t y0 = lds32(at + pa), y1 = lds32(at + 4 * R::ROW + pb), y2 = lds32(at + 8 * R::ROW + pa), y3 = lds32(at + 12 * R::ROW + pb);
+                        const uint32_t at = v_at ^ (32 * g), at4 = v_at ^ (32 * (g ^ R::FOUR_ON));
+                        const uint32_t y0 = lds32(at), y1 = lds32(at4 + 4 * R::ROW), y2 = lds32(at + 8 * R::ROW), y3 = lds32(at4 + 12 * R::ROW);
 #pragma unroll
                         for (int w = 0; w < 2; ++w) {
                             const uint32_t za = prmt(y0, y1, w ? 0x7632 : 0x5410), zb = prmt(y2, y3, w ? 0x7632 : 0x5410);
