@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <new>
+#include <type_traits>
 
 #include "sal_decode_ops.h"
 #include "sal_launch.h"
@@ -207,7 +208,6 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm vo
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -241,25 +241,16 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t select
     asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(selector));
     return d;
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-    return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-    return v;
-}
 template <int G>
-__device__ __forceinline__ void lds_params(uint32_t (&p)[G], uint32_t a) {
+__device__ __forceinline__ void load_params(uint32_t (&p)[G], const uint8_t *a) {
     if constexpr (G == 1) {
-        p[0] = lds32(a);
+        p[0] = *reinterpret_cast<const uint32_t *>(a);
     } else if constexpr (G == 2) {
-        const uint2 v = lds64(a);
+        const uint2 v = *reinterpret_cast<const uint2 *>(a);
         p[0] = v.x, p[1] = v.y;
     } else {
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(p[0]), "=r"(p[1]), "=r"(p[2]), "=r"(p[3]) : "r"(a));
+        const uint4 v = *reinterpret_cast<const uint4 *>(a);
+        p[0] = v.x, p[1] = v.y, p[2] = v.z, p[3] = v.w;
     }
 }
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -279,18 +270,18 @@ __device__ __forceinline__ uint32_t codes_low(uint32_t x) {
 }
 constexpr float UNIT = 1048576.f;
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {
     uint32_t d;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
@@ -299,9 +290,10 @@ __device__ __forceinline__ float2 as_float2(uint32_t h) { return __half22float2(
 
 // Scratch: status word, counter of arrivals per item, then two parts per thread block.
 constexpr int WS_HEADER = 256;
-constexpr int MAX_LIST = 1024;        // (sequence, column tile) pairs whose work is dealt out; with more, a block takes an item
+constexpr int CHUNK = 128;             // units of a block's run that are looked up at once
+constexpr int MAX_LIST = 256;         // (sequence, column tile) pairs whose work is dealt out; with more, a block takes an item
 constexpr int MIN_UNITS = 3;
-constexpr float MOVE_AT = 8.f;        // weights stay below 2**8 ..
+constexpr float MOVE_AT = 256.f;      // weights stay below 2**8 ..
 constexpr float W_ONE = 64.f;         // .. and, times this, inside 16 bits; the second parts' last bit is then 2**-30 of a weight of 1
 
 struct AttnArgs {
@@ -319,20 +311,22 @@ struct AttnArgs {
     float scale_log2;   // scale * log2(e) * UNIT
 };
 
-// NT column tiles of 8 per warp, WK warps that share a page's keys, WC warps side by side in columns.  DUP: at most four columns; the other
-// four of the tile are the same queries again and carry the second parts of the weights.
-template <int HD, int NT, bool DUP, int WK, int WC>
+// NT column tiles of 8 per warp, WK warps that share a page's keys, PG pages that are worked on side by side, WC warps side by side in
+// columns.  DUP: at most four columns; the other four of the tile are the same queries again and carry the second parts of the weights.
+template <int HD, int NT, bool DUP, int WK, int PG, int WC>
 struct AttnShape {
     static constexpr int COLS = DUP ? 4 : 8 * NT * WC;
-    static constexpr int WARPS = WK * WC;
-    static constexpr int THREADS = (WARPS + 1) * 32;
+    static constexpr int WARPS = WK * PG * WC;
+    static constexpr int THREADS = WARPS * 32;
+    static constexpr int PARTS = WK * PG;                              // warps that share a column
     static constexpr int REC = Record<HD>::BYTES;
     static constexpr int PART = COLS * (HD + 2);                       // floats of a part: outputs, maxima, sums
-    static constexpr int MERGE = WK > 1 ? WK * PART * 4 : 0;           // bytes of the warps' parts
+    static constexpr int MERGE = PARTS > 1 ? PARTS * PART * 4 : 0;     // bytes of the warps' parts
     static constexpr bool QUERIES = WC == 1;                           // an item's queries travel with its first page
     static constexpr int STAGE = REC + (QUERIES ? COLS * HD * 2 : 0);
-    static constexpr int STAGES = (HD == 256 ? 3 : HD == 128 ? 4 : 6);
-    static constexpr int SMEM = STAGES * STAGE + MERGE + MAX_LIST * 4 + 16;
+    static constexpr int STAGES = HD == 64 ? 8 : 4;                    // a power of two
+    static constexpr int SMEM = STAGES * STAGE + MERGE + 2 * CHUNK * 8 + MAX_LIST * 4 + 16;
+    static constexpr int MIN_BLOCKS = HD < 256 && NT == 1 ? 3 : 2;
 };
 
 struct Item {
@@ -363,25 +357,25 @@ __device__ __forceinline__ void store_output(__half *dst, float4 o, float total)
     *reinterpret_cast<uint2 *>(dst) = make_uint2(as_u32(__floats2half2_rn(o.x, o.y)), as_u32(__floats2half2_rn(o.z, o.w)));
 }
 
-template <int HD, int NT, bool DUP, int WK, int WC>
-__global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD < 256 && NT == 1 ? 3 : 2)) attention_tiles_kernel(AttnArgs a) {
-    using S = AttnShape<HD, NT, DUP, WK, WC>;
+template <int HD, int NT, bool DUP, int WK, int PG, int WC>
+__global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, AttnShape<HD, NT, DUP, WK, PG, WC>::MIN_BLOCKS) attention_tiles_kernel(AttnArgs a) {
+    using S = AttnShape<HD, NT, DUP, WK, PG, WC>;
     using R = Record<HD>;
     constexpr int G = R::G, COLS = S::COLS;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring = smem;
     float *merge = reinterpret_cast<float *>(smem + S::STAGES * S::STAGE);
-    int *list = reinterpret_cast<int *>(smem + S::STAGES * S::STAGE + S::MERGE);    // units in front of a pair, per kv head
-    __shared__ uint64_t bars[2 * S::STAGES];
-    __shared__ int s_valid[S::STAGES];
+    int2 *sched = reinterpret_cast<int2 *>(smem + S::STAGES * S::STAGE + S::MERGE);      // of two chunks of units: (record or none, item if its first page)
+    int *list = reinterpret_cast<int *>(sched + 2 * CHUNK);                              // units in front of a pair, per kv head
+    __shared__ uint64_t bars[S::STAGES];
+    __shared__ unsigned s_done[S::STAGES];     // warps that are through with a stage, counted on
     __shared__ int s_scan[33];
     __shared__ int s_flag;
-    __shared__ float s_top[S::COLS], s_total[S::COLS];
     __shared__ long long s_out[S::COLS];       // where a column's output lies
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t full = smem_u32(bars), empty = full + 8 * S::STAGES;
+    const uint32_t full = smem_u32(bars);
     if (tid == 0) {
-        for (int i = 0; i < S::STAGES; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, S::WARPS);
+        for (int i = 0; i < S::STAGES; ++i) mbar_init(full + 8 * i, 1), s_done[i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_prologue();
@@ -396,7 +390,6 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
         it.h = blockIdx.x % kvh;
         if (!item_of<COLS>(a, pair / a.col_tiles, pair % a.col_tiles, it)) return;
         at = 0, left = it.pages + 1;
-        __syncthreads();
     } else {
         int total = 0;         // units of all pairs, and in front of each
         for (int i0 = 0; i0 < pairs; i0 += S::THREADS) {
@@ -412,13 +405,15 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
             if (lane == 31) s_scan[warp] = run;
             __syncthreads();
             int front = total;
-            for (int w = 0; w <= S::WARPS; ++w) {
+            for (int w = 0; w < S::WARPS; ++w) {
                 if (w < warp) front += s_scan[w];
                 total += s_scan[w];
             }
             if (i < pairs) list[i] = front + run - n;
             __syncthreads();
         }
+        if (tid == 0) list[pairs] = total;
+        __syncthreads();
         const long long all = (long long)total * kvh;
         per = (all + gridDim.x - 1) / gridDim.x;
         if (per < MIN_UNITS) per = MIN_UNITS;
@@ -438,6 +433,64 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
         it.h = in_pair / (it.pages + 1);
         at = in_pair % (it.pages + 1);
     }
+    const int cols = a.m * a.rep;
+
+    // ---- what the run fetches: unit by unit, a chunk at a time, one unit per thread ----------------------------------------------------
+    const long long units = left, begin = per * blockIdx.x;
+    constexpr int NOTHING = -2, NO_PAGE = -1;       // an item's own unit, or behind the run; a page that does not exist
+    const int pair0 = pair, h0 = it.h, at0 = at;
+    auto look_up = [&](int chunk) {
+        static_assert(CHUNK == S::THREADS, "a thread looks up one unit");
+        const long long u = (long long)chunk * CHUNK + tid;
+        int2 e = make_int2(NOTHING, -1);
+        if (u < units) {
+            int p = pair0, h = h0, t = at0 + (int)u;      // pair, kv head, unit of the item
+            if (!a.whole) {
+                int lo = pair0, hi = pairs;
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) / 2;
+                    if ((long long)list[mid] * kvh <= begin + u) lo = mid;
+                    else hi = mid;
+                }
+                p = lo;
+                const int in_pair = (int)(begin + u - (long long)list[p] * kvh), n = list[p + 1] - list[p];
+                h = in_pair / n, t = in_pair % n;
+            }
+            if (t > 0) {
+                const int page = a.c.table[(size_t)(p / a.col_tiles) * a.c.max_pages + t - 1];
+                e.x = page >= 0 && page < a.c.pages ? page * kvh + h : NO_PAGE;
+                if (t == 1 || u == 0) e.y = p * kvh + h;
+            }
+        }
+        sched[(chunk & 1) * CHUNK + tid] = e;
+    };
+    // one lane asks for a page, and for the item's queries if it is the first
+    auto fetch = [&](int2 e, int st) {
+        const uint32_t dst = smem_u32(ring + st * S::STAGE), bar = full + 8 * st;
+        if (S::QUERIES && e.y >= 0) {
+            const int p = e.y / kvh, h = e.y % kvh, b = p / a.col_tiles, j0 = p % a.col_tiles * COLS;
+            const int j1 = min(min(j0 + COLS, cols), rows_of(a.rows, b, a.m) * a.rep);      // columns that are there
+            mbar_expect_tx(bar, (e.x >= 0 ? S::REC : 0) + (j1 - j0) * HD * 2);
+            for (int j = j0; j < j1;) {      // heads of a row that share this kv head lie side by side
+                const int i = j / a.rep, upto = min((i + 1) * a.rep, j1);
+                bulk_copy(dst + S::REC + (j - j0) * HD * 2, a.q + (((size_t)b * a.m + i) * a.heads + h * a.rep + (j - i * a.rep)) * HD, (upto - j) * HD * 2, bar);
+                j = upto;
+            }
+        } else {
+            mbar_expect_tx(bar, e.x >= 0 ? S::REC : 0);
+        }
+        if (e.x >= 0) bulk_copy(dst, a.c.pool + (size_t)e.x * S::REC, S::REC, bar);
+    };
+    look_up(0);
+    look_up(1);
+    __syncthreads();
+    if (warp == 0) {      // all stages are filled at once
+        const int2 e = sched[lane];
+        const unsigned pages = __ballot_sync(0xffffffffu, e.x != NOTHING);
+        const int rank = __popc(pages & ((1u << lane) - 1));
+        if (e.x != NOTHING && rank < S::STAGES) fetch(e, rank);
+        __syncwarp();
+    }
     // moves on to the next item: the next kv head, or the next pair that has rows
     auto next_item = [&] {
         left -= it.pages + 1 - at;
@@ -447,58 +500,15 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
         while (!item_of<COLS>(a, pair / a.col_tiles, pair % a.col_tiles, it));
         it.h = 0;
     };
-    const int cols = a.m * a.rep;
 
-    if (warp == S::WARPS) {
-        // ---- the warp that fetches --------------------------------------------------------------------------------------------
-        int st = 0, phase = 1;
-        bool alive = true;
-        for (; left > 0 && alive; next_item()) {
-            const int from = max(at - 1, 0), upto = (int)min((long long)at + left, (long long)it.pages + 1) - 1;
-            for (int p0 = from; p0 < upto && alive; p0 += 32) {
-                // page numbers of the next 32 pages, one per lane
-                int page = -1;
-                if (p0 + lane < upto && it.last >= 0) page = a.c.table[(size_t)it.b * a.c.max_pages + p0 + lane];
-                if (page >= a.c.pages) page = -1;
-                const int some = min(32, upto - p0);
-                for (int j = 0; j < some; ++j) {
-                    const int pg = __shfl_sync(0xffffffffu, page, j);
-                    alive = mbar_wait(empty + 8 * st, phase);
-                    if (!alive) break;
-                    const uint32_t dst = smem_u32(ring + st * S::STAGE), bar = full + 8 * st;
-                    const bool queries = S::QUERIES && p0 + j == from;
-                    const int j0 = it.ct * COLS, j1 = min(min(j0 + COLS, cols), it.rows * a.rep);      // columns that are there
-                    if (lane == 0) {
-                        s_valid[st] = pg >= 0;
-                        mbar_expect_tx(bar, (pg >= 0 ? S::REC : 0) + (queries ? (j1 - j0) * HD * 2 : 0));
-                        if (pg >= 0) bulk_copy(dst, a.c.pool + ((size_t)pg * kvh + it.h) * S::REC, S::REC, bar);
-                    }
-                    __syncwarp();
-                    if (queries) {      // heads of a row that share this kv head lie side by side
-                        const int i = j0 / a.rep + lane, c0 = max(i * a.rep, j0), c1 = min((i + 1) * a.rep, j1);
-                        if (c0 < c1)
-                            bulk_copy(dst + S::REC + (c0 - j0) * HD * 2, a.q + (((size_t)it.b * a.m + i) * a.heads + it.h * a.rep + (c0 - i * a.rep)) * HD,
-                                      (c1 - c0) * HD * 2, bar);
-                    }
-                    if (++st == S::STAGES) st = 0, phase ^= 1;
-                }
-            }
-        }
-        if (!alive) {   // the consumers gave up: what is on its way lands before the block ends
-            if (lane == 0) atomicExch(a.status, SAL_E_TIMEOUT);
-            for (int i = 0; i < S::STAGES; ++i) (void)mbar_wait(full + 8 * i, i < st ? phase ^ 1 : phase);
-        }
-        return;
-    }
-
-    // ---- the warps that compute ----------------------------------------------------------------------------------------------------
+    // ---- a run's items ------------------------------------------------------------------------------------------------------------------
     const int r = lane >> 2, c = lane & 3;
-    const int wk = warp % WK, wc = warp / WK;
+    const int wk = warp % WK, pg = warp / WK % PG, wc = warp / (WK * PG);
     const int krow = (r >> 1) + 4 * (r & 1);       // the key (of 8) that row r of a fragment stands for
     // where this lane's codes and parameters lie in a record; group g of a key's or value's row: that address ^ 32 g, rows being aligned
-    const uint32_t k_lane = (16 * wk + krow) * R::ROW + R::place(0, krow) * 32 + 8 * c, p_lane = 2 * R::CODES + (16 * wk + krow) * G * 4;
-    const uint32_t v_lane = R::CODES + (16 * wk + c) * R::ROW + R::place(0, c) * 32 + 4 * r;
-    int st = 0, phase = 0;
+    const uint32_t k_lane = (32 * wk + krow) * R::ROW + R::place(0, krow) * 32 + 8 * c, p_lane = 2 * R::CODES + (32 * wk + krow) * G * 4;
+    const uint32_t v_lane = R::CODES + (32 * wk + c) * R::ROW + R::place(0, c) * 32 + 4 * r;
+    int seq = 0, next_chunk = CHUNK;               // pages of the run in front of the item
     bool alive = true;
     for (; left > 0; next_item()) {
         const int base = max(at - 1, 0), n = (int)min((long long)at + left, (long long)it.pages + 1) - 1 - base;
@@ -508,7 +518,8 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
             const int j = it.ct * COLS + tid;
             s_out[tid] = (((long long)it.b * a.m + j / a.rep) * a.heads + it.h * a.rep + j % a.rep) * HD;
         }
-        if (S::QUERIES && alive) alive = mbar_wait(full + 8 * st, phase);
+        const int st0 = seq & (S::STAGES - 1);
+        if (S::QUERIES && alive) alive = mbar_wait(full + 8 * st0, seq / S::STAGES & 1);
         // columns of this warp: column j of the item is head j % rep of row j / rep
         uint32_t qf[NT][HD / 16][2];
         uint32_t qm[NT][(G + 1) / 2];      // sums of q over the groups, times 2**-6: first, second and third 16-bit parts in lanes c = 0, 1, 2
@@ -520,7 +531,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
             const int j = DUP ? it.ct * COLS + (r & 3) : col0 + r;
             const int i = j / a.rep;
             const bool real = j - it.ct * COLS < there;
-            const __half *src = S::QUERIES ? reinterpret_cast<const __half *>(ring + st * S::STAGE + S::REC) + (j - it.ct * COLS) * HD + 16 * c
+            const __half *src = S::QUERIES ? reinterpret_cast<const __half *>(ring + st0 * S::STAGE + S::REC) + (j - it.ct * COLS) * HD + 16 * c
                                            : a.q + (((size_t)it.b * a.m + i) * a.heads + it.h * a.rep + j % a.rep) * HD + 16 * c;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
@@ -553,7 +564,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
             lim[nt][0] = __shfl_sync(0xffffffffu, l, 8 * c);
             lim[nt][1] = __shfl_sync(0xffffffffu, l, 8 * c + 4);
         }
-        float acc[NT][HD / 16][4], accm[NT][2][G], ref[NT][2], over[NT][2], sum[NT][2], big[G], to_one[G];
+        float acc[NT][HD / 16][4], accm[NT][2][G], ref[NT][2], sum[NT][2], big[G], to_one[G];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -562,7 +573,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
                 for (int e = 0; e < 4; ++e) acc[nt][i][e] = 0.f;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                ref[nt][e] = 0.f, over[nt][e] = -INFINITY, sum[nt][e] = 0.f;
+                ref[nt][e] = 0.f, sum[nt][e] = 0.f;
 #pragma unroll
                 for (int g = 0; g < G; ++g) accm[nt][e][g] = 0.f;
             }
@@ -572,104 +583,137 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
         uint32_t big_h[(G + 1) / 2];                            // the same as pairs of 16-bit numbers
 #pragma unroll
         for (int i = 0; i < (G + 1) / 2; ++i) big_h[i] = 0x04000400u;
+        bool first = true;                                      // nothing was added up yet
+        // the queries are read (a stage is filled again once its page is done with), s_out is written
+        asm volatile("bar.sync 1, %0;" ::"n"(S::THREADS) : "memory");
 
-        for (int p = 0; p < n && alive; ++p) {
-            alive = mbar_wait(full + 8 * st, phase);
-            if (!alive) break;
-            const uint32_t rec = smem_u32(ring + st * S::STAGE);
-            if (s_valid[st]) {
+        for (int p0 = 0; p0 < n; p0 += PG) {
+            const int unit0 = (int)(units - left) + base + p0 + 1 - at;
+            if (unit0 >= next_chunk) {      // two chunks are at hand: the one behind is looked up once nobody needs the one in front
+                asm volatile("bar.sync 1, %0;" ::"n"(S::THREADS) : "memory");
+                look_up(next_chunk / CHUNK + 1);
+                next_chunk += CHUNK;
+                asm volatile("bar.sync 1, %0;" ::"n"(S::THREADS) : "memory");
+            }
+            const int p = p0 + pg;
+            if (p >= n) continue;
+            const int st = (seq + p) & (S::STAGES - 1);
+            if (alive) alive = mbar_wait(full + 8 * st, (seq + p) / S::STAGES & 1);
+            const uint8_t *rec = ring + st * S::STAGE;
+            if (alive && sched[(unit0 + pg) & (2 * CHUNK - 1)].x >= 0) {
 #pragma unroll 1
-                for (int i = 0; i < 4 / WK; ++i) {
-                    const int t0 = (base + p) * PAGE + 16 * (wk + WK * i);
+                for (int i = 0; i < 2 / WK; ++i) {
+                    const int t0 = (base + p) * PAGE + 32 * (wk + WK * i);
                     if (t0 > top_lim) break;
-                    const uint32_t k_at = rec + k_lane + i * (16 * WK * R::ROW), v_at = rec + v_lane + i * (16 * WK * R::ROW);
-                    const uint32_t par = rec + p_lane + i * (16 * WK * G * 4);
-                    uint32_t k0[G], k1[G], v0[G], v1[G];      // (scale, lowest value) of the two keys of this lane
-                    lds_params<G>(k0, par), lds_params<G>(k1, par + 8 * G * 4);
-                    lds_params<G>(v0, par + R::PARAMS), lds_params<G>(v1, par + R::PARAMS + 8 * G * 4);
-                    // scores of 16 keys, times 2**-20: lowest values times sums of q, then group by group
-                    float s[NT][4];
-                    {
+                    const uint32_t k_at = k_lane + i * (32 * WK * R::ROW), v_at = v_lane + i * (32 * WK * R::ROW);
+                    const uint8_t *par = rec + p_lane + i * (32 * WK * G * 4);
+                    // 32 keys in two fragments of 16: their scores times 2**-20, lowest values times sums of q, then group by group
+                    float z[2][NT][4];
+                    uint32_t v0[2][G], v1[2][G];      // (scale, lowest value) of the values of this lane's keys
+#pragma unroll
+                    for (int f = 0; f < 2; ++f) {
+                        uint32_t k0[G], k1[G];
+                        load_params<G>(k0, par + f * 16 * G * 4), load_params<G>(k1, par + (16 * f + 8) * G * 4);
+                        load_params<G>(v0[f], par + R::PARAMS + f * 16 * G * 4), load_params<G>(v1[f], par + R::PARAMS + (16 * f + 8) * G * 4);
                         const uint32_t zero = 0;
                         const uint32_t a0 = G == 1 ? k0[0] >> 16 : prmt(k0[0], k0[G > 1], 0x7632), a1 = G == 1 ? k1[0] >> 16 : prmt(k1[0], k1[G > 1], 0x7632);
                         const uint32_t a2 = G == 4 ? prmt(k0[2 % G], k0[3 % G], 0x7632) : zero, a3 = G == 4 ? prmt(k1[2 % G], k1[3 % G], 0x7632) : zero;
+                        float s[NT][4];
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             mma16816_first(s[nt], a0, a1, a2, a3, qm[nt][0], G == 4 ? qm[nt][(G + 1) / 2 - 1] : zero);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) s[nt][e] *= 64.f / UNIT;
                         }
-                    }
-#pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        const uint32_t at = k_at ^ (32 * g);
-                        const uint2 x0 = lds64(at), x1 = lds64(at + 8 * R::ROW);
-                        float d[NT][4];
-#pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            const uint32_t y0 = x0.x >> (8 * t), y1 = x1.x >> (8 * t), y2 = x0.y >> (8 * t), y3 = x1.y >> (8 * t);
-                            const uint32_t l0 = codes_low(y0), l1 = codes_low(y1), l2 = codes_low(y2), l3 = codes_low(y3);
-                            const uint32_t m0 = codes_mid(y0), m1 = codes_mid(y1), m2 = codes_mid(y2), m3 = codes_mid(y3);
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                const uint32_t(&b)[2] = qf[nt][g * 4 + 2 * t], (&b2)[2] = qf[nt][g * 4 + 2 * t + 1];
-                                if (t == 0) mma16816_first(d[nt], l0, l1, l2, l3, b[0], b[1]);
-                                else mma16816(d[nt], l0, l1, l2, l3, b[0], b[1]);
-                                mma16816(d[nt], m0, m1, m2, m3, b2[0], b2[1]);
-                            }
-                        }
-                        const float f0 = as_float2(k0[g]).x, f1 = as_float2(k1[g]).x;
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            s[nt][0] = fmaf(f0, d[nt][0], s[nt][0]);
-                            s[nt][1] = fmaf(f0, d[nt][1], s[nt][1]);
-                            s[nt][2] = fmaf(f1, d[nt][2], s[nt][2]);
-                            s[nt][3] = fmaf(f1, d[nt][3], s[nt][3]);
-                        }
-                    }
-                    const bool masked = t0 + 15 > low_lim;
-                    // A column's weights are powers relative to `ref`, which follows its largest score only when a weight would pass 2**8;
-                    // E likewise follows the scales.  Most blocks of keys move neither, which one vote finds out.
-                    bool moved = false;
-                    float z[NT][4];
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) z[nt][e] = fmaf(s[nt][e], a.scale_log2, -ref[nt][e & 1]);
-                    if (masked) {      // what a column does not see weighs nothing, whatever its key and value are
-                        const int ta = t0 + krow, tb = ta + 8;
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            if (ta > lim[nt][0]) z[nt][0] = -INFINITY;
-                            if (ta > lim[nt][1]) z[nt][1] = -INFINITY;
-                            if (tb > lim[nt][0]) z[nt][2] = -INFINITY;
-                            if (tb > lim[nt][1]) z[nt][3] = -INFINITY;
-                        }
 #pragma unroll
                         for (int g = 0; g < G; ++g) {
-                            if (ta > top_lim) v0[g] = 0;
-                            if (tb > top_lim) v1[g] = 0;
+                            const uint8_t *at = rec + (k_at ^ (32 * g)) + f * 16 * R::ROW;
+                            const uint2 x0 = *reinterpret_cast<const uint2 *>(at), x1 = *reinterpret_cast<const uint2 *>(at + 8 * R::ROW);
+                            float d[NT][4];
+#pragma unroll
+                            for (int t = 0; t < 2; ++t) {
+                                const uint32_t y0 = x0.x >> (8 * t), y1 = x1.x >> (8 * t), y2 = x0.y >> (8 * t), y3 = x1.y >> (8 * t);
+                                const uint32_t l0 = codes_low(y0), l1 = codes_low(y1), l2 = codes_low(y2), l3 = codes_low(y3);
+                                const uint32_t m0 = codes_mid(y0), m1 = codes_mid(y1), m2 = codes_mid(y2), m3 = codes_mid(y3);
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    const uint32_t(&b)[2] = qf[nt][g * 4 + 2 * t], (&b2)[2] = qf[nt][g * 4 + 2 * t + 1];
+                                    if (t == 0) mma16816_first(d[nt], m0, m1, m2, m3, b2[0], b2[1]);
+                                    else mma16816(d[nt], m0, m1, m2, m3, b2[0], b2[1]);
+                                    mma16816(d[nt], l0, l1, l2, l3, b[0], b[1]);
+                                }
+                            }
+                            const float f0 = as_float2(k0[g]).x, f1 = as_float2(k1[g]).x;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                s[nt][0] = fmaf(f0, d[nt][0], s[nt][0]);
+                                s[nt][1] = fmaf(f0, d[nt][1], s[nt][1]);
+                                s[nt][2] = fmaf(f1, d[nt][2], s[nt][2]);
+                                s[nt][3] = fmaf(f1, d[nt][3], s[nt][3]);
+                            }
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) z[f][nt][e] = fmaf(s[nt][e], a.scale_log2, -ref[nt][e & 1]);
+                    }
+                    const bool masked = t0 + 31 > low_lim;
+                    if (masked) {      // what a column does not see weighs nothing, whatever its key and value are
+#pragma unroll
+                        for (int f = 0; f < 2; ++f) {
+                            const int ta = t0 + 16 * f + krow, tb = ta + 8;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                if (ta > lim[nt][0]) z[f][nt][0] = -INFINITY;
+                                if (ta > lim[nt][1]) z[f][nt][1] = -INFINITY;
+                                if (tb > lim[nt][0]) z[f][nt][2] = -INFINITY;
+                                if (tb > lim[nt][1]) z[f][nt][3] = -INFINITY;
+                            }
+#pragma unroll
+                            for (int g = 0; g < G; ++g) {
+                                if (ta > top_lim) v0[f][g] = 0;
+                                if (tb > top_lim) v1[f][g] = 0;
+                            }
                         }
                     }
+                    // A column's weights are powers relative to `ref`, which follows its largest score only when this lane's four would pass 2**8 in
+                    // sum; E likewise follows the scales.  Most keys move neither, which one vote finds out.
+                    float w[2][NT][4], add[NT][2];
+                    bool moved = first;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) moved |= z[nt][e] > over[nt][e & 1];
+                        for (int f = 0; f < 2; ++f)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[f][nt][e] = exp2_approx(z[f][nt][e]);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            add[nt][e] = (w[0][nt][e] + w[0][nt][e + 2]) + (w[1][nt][e] + w[1][nt][e + 2]);
+                            moved |= add[nt][e] > MOVE_AT;
+                        }
+                    }
                     if constexpr (G == 1) {
-                        moved |= !__hble2(as_half2(prmt(v0[0], v1[0], 0x5410)), as_half2(big_h[0]));
+                        const __half2 x = __hmax2_nan(as_half2(prmt(v0[0][0], v1[0][0], 0x5410)), as_half2(prmt(v0[1][0], v1[1][0], 0x5410)));
+                        moved |= !__hble2(x, as_half2(big_h[0]));
                     } else {
 #pragma unroll
-                        for (int i = 0; i < G / 2; ++i) {
-                            const __half2 x = __hmax2_nan(as_half2(prmt(v0[2 * i], v0[2 * i + 1], 0x5410)), as_half2(prmt(v1[2 * i], v1[2 * i + 1], 0x5410)));
-                            moved |= !__hble2(x, as_half2(big_h[i]));
+                        for (int i2 = 0; i2 < G / 2; ++i2) {
+                            __half2 x = as_half2(prmt(v0[0][2 * i2], v0[0][2 * i2 + 1], 0x5410));
+                            x = __hmax2_nan(x, as_half2(prmt(v1[0][2 * i2], v1[0][2 * i2 + 1], 0x5410)));
+                            x = __hmax2_nan(x, __hmax2_nan(as_half2(prmt(v0[1][2 * i2], v0[1][2 * i2 + 1], 0x5410)), as_half2(prmt(v1[1][2 * i2], v1[1][2 * i2 + 1], 0x5410))));
+                            moved |= !__hble2(x, as_half2(big_h[i2]));
                         }
                     }
                     if (__any_sync(0xffffffffu, moved)) {
                         float fg[G];
 #pragma unroll
                         for (int g = 0; g < G; ++g) {
-                            const float x0 = fabsf(as_float2(v0[g]).x), x1 = fabsf(as_float2(v1[g]).x);
-                            const float x = fmaxf(x0 <= 65504.f ? x0 : 0.f, x1 <= 65504.f ? x1 : 0.f);
+                            float x = 0.f;
+#pragma unroll
+                            for (int f = 0; f < 2; ++f) {
+                                const float x0 = fabsf(as_float2(v0[f][g]).x), x1 = fabsf(as_float2(v1[f][g]).x);
+                                x = fmaxf(x, fmaxf(x0 <= 65504.f ? x0 : 0.f, x1 <= 65504.f ? x1 : 0.f));
+                            }
                             const uint32_t u = (__reduce_max_sync(0xffffffffu, __float_as_uint(x)) + 0x7fffffu) & 0x7f800000u;   // up to a power of two
                             const float grown = fminf(fmaxf(__uint_as_float(u), big[g]), 32768.f);
                             fg[g] = __fdividef(big[g], grown);
@@ -682,95 +726,105 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                float x = fmaxf(z[nt][e], z[nt][e + 2]);
+                                float x = fmaxf(fmaxf(z[0][nt][e], z[0][nt][e + 2]), fmaxf(z[1][nt][e], z[1][nt][e + 2]));
                                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                                float f = 1.f;
-                                if (x > over[nt][e]) {
-                                    f = exp2_approx(-x);      // nothing was added up yet where `over` was -infinity
-                                    if (over[nt][e] == -INFINITY) f = 0.f;
-                                    ref[nt][e] += x, over[nt][e] = MOVE_AT;
-                                    if (z[nt][e] != -INFINITY) z[nt][e] = fmaf(s[nt][e], a.scale_log2, -ref[nt][e]);
-                                    if (z[nt][e + 2] != -INFINITY) z[nt][e + 2] = fmaf(s[nt][e + 2], a.scale_log2, -ref[nt][e]);
+                                float by = first ? 0.f : 1.f;
+                                if (x > (first ? -INFINITY : 0.f)) {
+                                    if (!first) by = exp2_approx(-x);
+                                    ref[nt][e] += x;
+#pragma unroll
+                                    for (int f = 0; f < 2; ++f)
+#pragma unroll
+                                        for (int k = 0; k < 2; ++k) w[f][nt][e + 2 * k] = exp2_approx(z[f][nt][e + 2 * k] - x);
+                                    add[nt][e] = (w[0][nt][e] + w[0][nt][e + 2]) + (w[1][nt][e] + w[1][nt][e + 2]);
                                 }
-                                sum[nt][e] *= f;
+                                sum[nt][e] *= by;
 #pragma unroll
                                 for (int g = 0; g < G; ++g) {
-                                    accm[nt][e][g] *= f;
+                                    accm[nt][e][g] *= by;
 #pragma unroll
-                                    for (int i = 0; i < 4; ++i) acc[nt][4 * g + i][e] *= f * fg[g], acc[nt][4 * g + i][e + 2] *= f * fg[g];
+                                    for (int k = 0; k < 4; ++k) acc[nt][4 * g + k][e] *= by * fg[g], acc[nt][4 * g + k][e + 2] *= by * fg[g];
                                 }
                             }
+                        first = false;
                     }
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) z[nt][e] = exp2_approx(z[nt][e]);
-                        sum[nt][0] += z[nt][0] + z[nt][2];
-                        sum[nt][1] += z[nt][1] + z[nt][3];
-                    }
+                    for (int nt = 0; nt < NT; ++nt) sum[nt][0] += add[nt][0], sum[nt][1] += add[nt][1];
                     // weighted values
 #pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        const float2 f0 = as_float2(v0[g]), f1 = as_float2(v1[g]);
-                        const float u0 = f0.x * to_one[g], u1 = f1.x * to_one[g];
-                        uint32_t b[NT][2], b2[NT][2];
+                    for (int f = 0; f < 2; ++f) {
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            float w[4] = {z[nt][0] * u0, z[nt][1] * u0, z[nt][2] * u1, z[nt][3] * u1};
-                            if (masked) {      // 0 times what is no number
+                        for (int g = 0; g < G; ++g) {
+                            const float2 f0 = as_float2(v0[f][g]), f1 = as_float2(v1[f][g]);
+                            const float u0 = f0.x * to_one[g], u1 = f1.x * to_one[g];
+                            uint32_t b[NT][2], b2[NT][2];
 #pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    if (z[nt][e] == 0.f) w[e] = 0.f;
-                                accm[nt][0][g] += (z[nt][0] == 0.f ? 0.f : z[nt][0] * f0.y) + (z[nt][2] == 0.f ? 0.f : z[nt][2] * f1.y);
-                                accm[nt][1][g] += (z[nt][1] == 0.f ? 0.f : z[nt][1] * f0.y) + (z[nt][3] == 0.f ? 0.f : z[nt][3] * f1.y);
-                            } else {
-                                accm[nt][0][g] = fmaf(z[nt][0], f0.y, fmaf(z[nt][2], f1.y, accm[nt][0][g]));
-                                accm[nt][1][g] = fmaf(z[nt][1], f0.y, fmaf(z[nt][3], f1.y, accm[nt][1][g]));
+                            for (int nt = 0; nt < NT; ++nt) {
+                                const float(&q)[4] = w[f][nt];
+                                float y[4] = {q[0] * u0, q[1] * u0, q[2] * u1, q[3] * u1};
+                                if (masked) {      // 0 times what is no number
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e)
+                                        if (q[e] == 0.f) y[e] = 0.f;
+                                    accm[nt][0][g] += (q[0] == 0.f ? 0.f : q[0] * f0.y) + (q[2] == 0.f ? 0.f : q[2] * f1.y);
+                                    accm[nt][1][g] += (q[1] == 0.f ? 0.f : q[1] * f0.y) + (q[3] == 0.f ? 0.f : q[3] * f1.y);
+                                } else {
+                                    accm[nt][0][g] = fmaf(q[0], f0.y, fmaf(q[2], f1.y, accm[nt][0][g]));
+                                    accm[nt][1][g] = fmaf(q[1], f0.y, fmaf(q[3], f1.y, accm[nt][1][g]));
+                                }
+                                const __half2 h0 = __floats2half2_rn(y[0], y[1]), h1 = __floats2half2_rn(y[2], y[3]);
+                                const float2 e0 = __half22float2(h0), e1 = __half22float2(h1);
+                                if (DUP) {      // lanes 2 and 3 carry what the others' rounding left
+                                    const float rest = c < 2 ? 0.f : 1.f;
+                                    b[nt][0] = transposed(as_u32(c < 2 ? h0 : __floats2half2_rn(fmaf(-rest, e0.x, y[0]), fmaf(-rest, e0.y, y[1]))));
+                                    b[nt][1] = transposed(as_u32(c < 2 ? h1 : __floats2half2_rn(fmaf(-rest, e1.x, y[2]), fmaf(-rest, e1.y, y[3]))));
+                                } else {
+                                    b[nt][0] = transposed(as_u32(h0)), b[nt][1] = transposed(as_u32(h1));
+                                    b2[nt][0] = transposed(as_u32(__floats2half2_rn(y[0] - e0.x, y[1] - e0.y)));
+                                    b2[nt][1] = transposed(as_u32(__floats2half2_rn(y[2] - e1.x, y[3] - e1.y)));
+                                }
                             }
-                            const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
-                            const float2 e0 = __half22float2(h0), e1 = __half22float2(h1);
-                            const __half2 l0 = __floats2half2_rn(w[0] - e0.x, w[1] - e0.y), l1 = __floats2half2_rn(w[2] - e1.x, w[3] - e1.y);
-                            if (DUP) {
-                                b[nt][0] = transposed(as_u32(c < 2 ? h0 : l0));
-                                b[nt][1] = transposed(as_u32(c < 2 ? h1 : l1));
-                            } else {
-                                b[nt][0] = transposed(as_u32(h0)), b[nt][1] = transposed(as_u32(h1));
-                                b2[nt][0] = transposed(as_u32(l0)), b2[nt][1] = transposed(as_u32(l1));
-                            }
-                        }
-                        const uint32_t at = v_at ^ (32 * g), at4 = v_at ^ (32 * (g ^ R::FOUR_ON));
-                        const uint32_t y0 = lds32(at), y1 = lds32(at4 + 4 * R::ROW), y2 = lds32(at + 8 * R::ROW), y3 = lds32(at4 + 12 * R::ROW);
+                            const uint8_t *at = rec + (v_at ^ (32 * g)) + f * 16 * R::ROW, *at4 = rec + (v_at ^ (32 * (g ^ R::FOUR_ON))) + f * 16 * R::ROW;
+                            const uint32_t y0 = *reinterpret_cast<const uint32_t *>(at), y1 = *reinterpret_cast<const uint32_t *>(at4 + 4 * R::ROW);
+                            const uint32_t y2 = *reinterpret_cast<const uint32_t *>(at + 8 * R::ROW), y3 = *reinterpret_cast<const uint32_t *>(at4 + 12 * R::ROW);
 #pragma unroll
-                        for (int w = 0; w < 2; ++w) {
-                            const uint32_t za = prmt(y0, y1, w ? 0x7632 : 0x5410), zb = prmt(y2, y3, w ? 0x7632 : 0x5410);
+                            for (int k = 0; k < 2; ++k) {
+                                const uint32_t za = prmt(y0, y1, k ? 0x7632 : 0x5410), zb = prmt(y2, y3, k ? 0x7632 : 0x5410);
 #pragma unroll
-                            for (int t = 0; t < 2; ++t) {
-                                const uint32_t xa = za >> (8 * t), xb = zb >> (8 * t);
-                                const uint32_t a0 = codes_low(xa), a1 = codes_mid(xa), a2 = codes_low(xb), a3 = codes_mid(xb);
+                                for (int t = 0; t < 2; ++t) {
+                                    const uint32_t xa = za >> (8 * t), xb = zb >> (8 * t);
+                                    const uint32_t a0 = codes_low(xa), a1 = codes_mid(xa), a2 = codes_low(xb), a3 = codes_mid(xb);
 #pragma unroll
-                                for (int nt = 0; nt < NT; ++nt) {
-                                    mma16816(acc[nt][4 * g + 2 * w + t], a0, a1, a2, a3, b[nt][0], b[nt][1]);
-                                    if (!DUP) mma16816(acc[nt][4 * g + 2 * w + t], a0, a1, a2, a3, b2[nt][0], b2[nt][1]);
+                                    for (int nt = 0; nt < NT; ++nt) {
+                                        mma16816(acc[nt][4 * g + 2 * k + t], a0, a1, a2, a3, b[nt][0], b[nt][1]);
+                                        if (!DUP) mma16816(acc[nt][4 * g + 2 * k + t], a0, a1, a2, a3, b2[nt][0], b2[nt][1]);
+                                    }
                                 }
                             }
                         }
                     }
                 }
             }
+            // the last of the warps that are through with a page asks for the one that goes into its stage
             __syncwarp();
-            if (lane == 0) mbar_arrive(empty + 8 * st);
-            if (++st == S::STAGES) st = 0, phase ^= 1;
+            unsigned done = 0;
+            if (lane == 0) asm volatile("atom.acq_rel.cta.shared::cta.add.u32 %0, [%1], 1;" : "=r"(done) : "r"(smem_u32(s_done + st)) : "memory");
+            done = __shfl_sync(0xffffffffu, done, 0);
+            if ((done + 1) % (WK * WC) == 0 && alive) {
+                const int2 e = sched[(unit0 + pg + lane) & (2 * CHUNK - 1)];
+                const unsigned pages = __ballot_sync(0xffffffffu, e.x != NOTHING);
+                if (e.x != NOTHING && __popc(pages & ((1u << lane) - 1)) == S::STAGES) fetch(e, st);
+            }
         }
-        if (!alive && lane == 0) atomicExch(a.status, SAL_E_TIMEOUT);   // and on to the end, past the same barriers
+        seq += n;
 
         // ---- this block's part of the item, into the output or into scratch ---------------------------------------------------------------
         const bool all = n == it.pages;
         // The blocks of an item are neighbours; a part lies in the block's first place if the item began in front of the block, else in its second.
         float *part = a.parts + ((size_t)blockIdx.x * 2 + (at == 0 ? 1 : 0)) * S::PART;
-        float *mine = merge + wk * S::PART;
-        if (WK == 1) asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");      // s_out is written
+        float *mine = merge + (wk + WK * pg) * S::PART;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -779,8 +833,8 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
                 const int col = (wc * NT + nt) * 8 + 2 * c + e;
-                const float top = over[nt][e] == -INFINITY ? -INFINITY : ref[nt][e];
-                if (WK > 1) {
+                const float top = l == 0.f ? -INFINITY : ref[nt][e];
+                if (S::PARTS > 1) {
                     if (r == 0 && (!DUP || c < 2)) mine[COLS * HD + col] = top, mine[COLS * (HD + 1) + col] = l;
                 } else if (!all && r == 0) {
                     __stcg(part + COLS * HD + col, top), __stcg(part + COLS * (HD + 1) + col, l);
@@ -801,7 +855,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
                     }
 #pragma unroll
                     for (int i = 0; i < 8; ++i) o8[i] = fmaf(o8[i], back, lowest);
-                    if (WK == 1 && all) {
+                    if (S::PARTS == 1 && all) {
                         if (col < there) {
                             if (l == 0.f) {      // no position: zeros
 #pragma unroll
@@ -814,7 +868,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
                                 make_uint4(as_u32(__floats2half2_rn(o8[0], o8[1])), as_u32(__floats2half2_rn(o8[2], o8[3])),
                                            as_u32(__floats2half2_rn(o8[4], o8[5])), as_u32(__floats2half2_rn(o8[6], o8[7])));
                         }
-                    } else if (WK == 1) {
+                    } else if (S::PARTS == 1) {
                         float4 *dst = reinterpret_cast<float4 *>(part + col * HD + g * GROUP + 8 * r);
                         if (col < there) __stcg(dst, make_float4(o8[0], o8[1], o8[2], o8[3])), __stcg(dst + 1, make_float4(o8[4], o8[5], o8[6], o8[7]));
                     } else if (!DUP || c < 2) {
@@ -825,16 +879,16 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
                 }
             }
         }
-        if (WK > 1) {
+        if (S::PARTS > 1) {
             asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");
             for (int x = 4 * tid; x < there * HD; x += 4 * S::WARPS * 32) {
                 const int col = x / HD;
-                float t[WK], l[WK], top = -INFINITY, total = 0.f;
+                float t[S::PARTS], l[S::PARTS], top = -INFINITY, total = 0.f;
 #pragma unroll
-                for (int w = 0; w < WK; ++w) t[w] = merge[w * S::PART + COLS * HD + col], l[w] = merge[w * S::PART + COLS * (HD + 1) + col], top = fmaxf(top, t[w]);
+                for (int w = 0; w < S::PARTS; ++w) t[w] = merge[w * S::PART + COLS * HD + col], l[w] = merge[w * S::PART + COLS * (HD + 1) + col], top = fmaxf(top, t[w]);
                 float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int w = 0; w < WK; ++w) {
+                for (int w = 0; w < S::PARTS; ++w) {
                     if (l[w] == 0.f) continue;
                     const float f = exp2_approx(t[w] - top);
                     const float4 v = *reinterpret_cast<const float4 *>(merge + w * S::PART + x);
@@ -862,57 +916,68 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, WC>::THREADS, (HD <
             }
             asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");
             if (s_flag) {
-                // weight of a part: exp2(its maximum - the largest) / sum; a column's maxima and sums are read by one warp, a part per lane
                 const float *parts = a.parts + (size_t)(block0 + 1) * 2 * S::PART;      // of the blocks behind the first
                 const float *part0 = a.parts + ((size_t)block0 * 2 + (start >= per * block0 ? 1 : 0)) * S::PART;
                 const int more = block1 - block0;
-                for (int col = warp; col < there; col += S::WARPS) {
-                    float top = lane == 0 ? __ldcg(part0 + COLS * HD + col) : -INFINITY;
-                    for (int k = lane; k < more; k += 32) top = fmaxf(top, __ldcg(parts + (size_t)k * 2 * S::PART + COLS * HD + col));
+                auto add_up = [&](auto pieces, auto at_once) {      // so many pieces of four outputs per thread, so many parts of each at a time: all loads first
+                    constexpr int T = decltype(pieces)::value, P = decltype(at_once)::value, STEP = 4 * S::THREADS;
+                    for (int x0 = 4 * tid; x0 < there * HD; x0 += T * STEP) {
+                        float4 o[T];
+                        float top[T], total[T];
 #pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    float total = 0.f;
-                    for (int k = lane - 1; k < more; k += 32) {
-                        const float *m = k < 0 ? part0 : parts + (size_t)k * 2 * S::PART;
-                        const float l = __ldcg(m + COLS * (HD + 1) + col);
-                        if (l != 0.f) total += l * exp2_approx(__ldcg(m + COLS * HD + col) - top);
-                    }
+                        for (int i = 0; i < T; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f), top[i] = -INFINITY, total[i] = 0.f;
+                        for (int k0 = -1; k0 < more; k0 += P) {
+                            float4 v[T][P];
+                            float t[T][P], l[T][P];
 #pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-                    if (lane == 0) s_top[col] = top, s_total[col] = total;
-                }
-                asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");
-                constexpr int LOADS = 8, STEP = 4 * S::WARPS * 32;
-                for (int x = 4 * tid; x < there * HD; x += 2 * STEP) {
-                    // two pieces of four outputs, eight parts of each at a time: all loads first
-                    const bool two = x + STEP < there * HD;
-                    const int x1 = two ? x + STEP : x, col = x / HD, col1 = x1 / HD;
-                    const float top = s_top[col], top1 = s_top[col1];
-                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f), o1 = o;
-                    for (int k0 = -1; k0 < more; k0 += LOADS) {
-                        float4 v[LOADS], v1[LOADS];
-                        float f[LOADS], f1[LOADS];
+                            for (int u = 0; u < P; ++u) {
+                                const int k = min(k0 + u, more - 1);
+                                const float *m = k < 0 ? part0 : parts + (size_t)k * 2 * S::PART;
 #pragma unroll
-                        for (int u = 0; u < LOADS; ++u) {
-                            const int k = min(k0 + u, more - 1);
-                            const float *m = k < 0 ? part0 : parts + (size_t)k * 2 * S::PART;
-                            v[u] = __ldcg(reinterpret_cast<const float4 *>(m + x)), v1[u] = __ldcg(reinterpret_cast<const float4 *>(m + x1));
-                            f[u] = __ldcg(m + COLS * HD + col), f1[u] = __ldcg(m + COLS * HD + col1);
+                                for (int i = 0; i < T; ++i) {
+                                    const int x = x0 + i * STEP < there * HD ? x0 + i * STEP : x0;
+                                    v[i][u] = __ldcg(reinterpret_cast<const float4 *>(m + x));
+                                    t[i][u] = __ldcg(m + COLS * HD + x / HD), l[i][u] = __ldcg(m + COLS * (HD + 1) + x / HD);
+                                }
+                            }
+#pragma unroll
+                            for (int i = 0; i < T; ++i) {
+                                float high = top[i];
+#pragma unroll
+                                for (int u = 0; u < P; ++u) {
+                                    if (k0 + u >= more) l[i][u] = 0.f;
+                                    if (l[i][u] != 0.f) high = fmaxf(high, t[i][u]);
+                                }
+                                const float old = total[i] == 0.f ? 0.f : exp2_approx(top[i] - high);
+                                top[i] = high, total[i] *= old;
+                                if (total[i] != 0.f) o[i].x *= old, o[i].y *= old, o[i].z *= old, o[i].w *= old;
+#pragma unroll
+                                for (int u = 0; u < P; ++u) {
+                                    if (l[i][u] == 0.f) continue;
+                                    const float w = exp2_approx(t[i][u] - high);
+                                    total[i] += w * l[i][u];
+                                    o[i].x += w * v[i][u].x, o[i].y += w * v[i][u].y, o[i].z += w * v[i][u].z, o[i].w += w * v[i][u].w;
+                                }
+                            }
                         }
 #pragma unroll
-                        for (int u = 0; u < LOADS; ++u) {
-                            const float w = k0 + u < more ? exp2_approx(f[u] - top) : 0.f, w1 = k0 + u < more ? exp2_approx(f1[u] - top1) : 0.f;
-                            if (w != 0.f) o.x += w * v[u].x, o.y += w * v[u].y, o.z += w * v[u].z, o.w += w * v[u].w;
-                            if (w1 != 0.f) o1.x += w1 * v1[u].x, o1.y += w1 * v1[u].y, o1.z += w1 * v1[u].z, o1.w += w1 * v1[u].w;
+                        for (int i = 0; i < T; ++i) {
+                            const int x = x0 + i * STEP;
+                            if (x < there * HD) store_output(a.out + s_out[x / HD] + x % HD, o[i], total[i]);
                         }
                     }
-                    store_output(a.out + s_out[col] + x % HD, o, s_total[col]);
-                    if (two) store_output(a.out + s_out[col1] + x1 % HD, o1, s_total[col1]);
-                }
+                };
+                if (more < 4) add_up(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
+                else if (more < 8 || there * HD > 4 * S::THREADS) add_up(std::integral_constant<int, 2>{}, std::integral_constant<int, 8>{});
+                else add_up(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
                 if (tid == 0) *counter = 0;      // ready for the next launch
             }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");       // `merge` and `s_flag` are free again
+    }
+    if (!alive) {      // a wait ran out: the run went on without its pages, past the same barriers; what is on its way lands before the block ends
+        if (lane == 0) atomicExch(a.status, SAL_E_TIMEOUT);
+        for (int i = 0; i < S::STAGES; ++i) (void)mbar_wait(full + 8 * i, 0), (void)mbar_wait(full + 8 * i, 1);
     }
 }
 
@@ -936,7 +1001,7 @@ bool aligned16(const void *a, const void *b = nullptr, const void *c = nullptr, 
 int check_cache(int batch, int m, int kv_heads, int hd, int max_pages, int pages) {
     if (hd != 64 && hd != 128 && hd != 256) return SAL_E_UNSUPPORTED;
     if (batch < 1 || m < 1 || kv_heads < 1 || kv_heads > 256 || max_pages < 1 || max_pages > MAX_PAGES || pages < 1) return SAL_E_SHAPE;
-    if ((long long)batch * m > SAL_KV4_MAX_ROWS) return SAL_E_SHAPE;
+    if ((long long)batch * m > SAL_KV4_MAX_ROWS || (long long)pages * kv_heads > 0x7fffffff) return SAL_E_SHAPE;
     return SAL_OK;
 }
 
@@ -955,7 +1020,7 @@ AttnPlan attention_plan(int batch, int m, int rep, int hd) {
     p.cols = p.kind == FOUR_COLUMNS ? 4 : p.kind == EIGHT_COLUMNS ? 8 : p.kind == SIXTEEN_COLUMNS ? 16 : hd < 256 ? 64 : 32;
     p.col_tiles = (cols + p.cols - 1) / p.cols;
     p.pairs = batch * p.col_tiles;
-    p.max_blocks = p.kind == MANY_COLUMNS ? 320 : 640;
+    p.max_blocks = p.kind == MANY_COLUMNS ? 320 : 448;
     return p;
 }
 
@@ -965,10 +1030,10 @@ size_t counter_bytes(const AttnPlan &p, int batch, int kv_heads) {
     return ((size_t)(pairs < MAX_LIST ? pairs : MAX_LIST) * kv_heads * 4 + 255) / 256 * 256;
 }
 
-template <int HD, int NT, bool DUP, int WK, int WC>
+template <int HD, int NT, bool DUP, int WK, int PG, int WC>
 int launch_tiles(const AttnArgs &a, const AttnPlan &p, void *stream) {
-    using S = AttnShape<HD, NT, DUP, WK, WC>;
-    auto kernel = attention_tiles_kernel<HD, NT, DUP, WK, WC>;
+    using S = AttnShape<HD, NT, DUP, WK, PG, WC>;
+    auto kernel = attention_tiles_kernel<HD, NT, DUP, WK, PG, WC>;
     static std::atomic<bool> configured[64];
     static std::atomic<int> resident[64];
     if (sal_allow_shared_memory(kernel, configured) != cudaSuccess) return SAL_E_LAUNCH;
@@ -988,11 +1053,11 @@ int launch_tiles(const AttnArgs &a, const AttnPlan &p, void *stream) {
 template <int HD>
 int launch_attention(const AttnArgs &a, const AttnPlan &p, void *stream) {
     switch (p.kind) {
-        case FOUR_COLUMNS: return launch_tiles<HD, 1, true, 4, 1>(a, p, stream);
-        case EIGHT_COLUMNS: return launch_tiles<HD, 1, false, 4, 1>(a, p, stream);
+        case FOUR_COLUMNS: return launch_tiles<HD, 1, true, 2, 2, 1>(a, p, stream);
+        case EIGHT_COLUMNS: return launch_tiles<HD, 1, false, 2, 2, 1>(a, p, stream);
         case SIXTEEN_COLUMNS:
-            if constexpr (HD < 256) return launch_tiles<HD, 2, false, 4, 1>(a, p, stream);
-        default: return launch_tiles<HD, (HD < 256 ? 2 : 1), false, 1, 4>(a, p, stream);
+            if constexpr (HD < 256) return launch_tiles<HD, 2, false, 2, 2, 1>(a, p, stream);
+        default: return launch_tiles<HD, (HD < 256 ? 2 : 1), false, 1, 1, 4>(a, p, stream);
     }
 }
 
