@@ -5,8 +5,16 @@
 // row needs is where each prefix ends: a logit, and how many of the tokens that have it are still in.  The token is then the first, by
 // index, at which the running sum of the kept weights exceeds u times their total.
 //
+// A row is worked on by a cluster of thread blocks, each with a slice of the row in shared memory.  The ends of the prefixes are looked for in a
+// histogram of the logits, 89 bins to a factor of two in weight: counts alone say which bin holds the k-th logit, and between which bins the weights
+// in front pass top_p of the total (a bin's weights are known to 0.8 % from its number).  If many tokens lie there, a second histogram divides those
+// bins further.  Only what lies in the last ones is gathered, in the order of the indexes, and ranked exactly by comparing each with each; what lies in front is summed exactly.  Where that
+// is everything that can be kept, one block goes on alone.  Where so many lie there that the list does not take them (equal logits), the ends are
+// found bit by bit, a pass over the slices for each.
+//
 // Weights are whole numbers in units of 2**-44 (the largest is 2**44, a sum of 2**18 of them fits 63 bits): sums do not depend on their
 // order, so the same inputs give the same token however the work is split, and the running sum meets the total exactly.
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -56,20 +64,6 @@ struct Weights {
     }
 };
 
-template <typename T>
-__device__ __forceinline__ T block_total(T v, T *red) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if (lane == 0) red[warp] = v;
-    __syncthreads();
-    T r = lane < nw ? red[lane] : T(0);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
-    return r;
-}
-
 struct SampleArgs {
     const void *logits;
     const float *u, *temperature, *top_p, *min_p;
@@ -77,148 +71,511 @@ struct SampleArgs {
     float temperature_all, top_p_all, min_p_all;
     int top_k_all;
     int vocab;
+    int slice;       // tokens of a block, a multiple of 8
     int64_t *token;
 };
 
-__device__ __forceinline__ float load_logit(const float *p, int i) { return p[i]; }
-__device__ __forceinline__ float load_logit(const __half *p, int i) { return __half2float(p[i]); }
+constexpr int THREADS = 512, WARPS = THREADS / 32;
+constexpr int BINS = 4096;
+constexpr float BIN_SCALE = 89.f;                  // bins to a factor of two: 46 factors fit, behind them a weight is 0
+constexpr int LIST = 1024;                         // tokens that can be ranked
+constexpr int ALONE = THREADS;                     // so few that one block finishes, a token per thread
+constexpr int FEW = 256;                           // a window of so many is ranked at once
+constexpr int MAX_CLUSTER = 8;
 
-// One thread block per row: the ends of the prefixes are found bit by bit, with one pass over the row for each bit.
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+
+// What the blocks of a cluster tell one another; `round` alternates the places, so that one barrier a round is enough.
+struct Told {
+    mass_t mass;
+    double bound;
+    unsigned long long best;
+    int count;
+};
+struct Found {
+    float end;          // the kept prefix: logits above `end`, and the first `ties` of those that equal it
+    int ties;
+    mass_t mass;        // of the kept prefix
+};
+struct alignas(16) SampleShared {
+    Told told[2];
+    Found found;
+    int2 windows[2][2];     // first bin and the tokens in front of it, last bin and the tokens up to it; two places in turn
+    mass_t warp_mass[WARPS];
+    double warp_bound[WARPS];
+    int warp_count[WARPS];
+    unsigned long long warp_best[WARPS];
+    mass_t block_mass;
+    int block_count;
+    uint32_t hist[BINS];
+    float list_x[LIST];
+    int list_i[LIST];
+    mass_t list_w[LIST];
+};
+
+template <typename V>
+__device__ __forceinline__ V warp_total(V v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+template <typename V>
+__device__ __forceinline__ V warp_running(V v, int lane) {      // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const V t = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += t;
+    }
+    return v;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(1024) sample_kernel(SampleArgs a) {
-    __shared__ mass_t red[32];
-    __shared__ uint32_t red32[32];
-    __shared__ mass_t s_warp[32];
-    __shared__ int s_ties[32];
-    __shared__ int s_token;
+__global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    extern __shared__ __align__(16) uint8_t smem[];
+    SampleShared &s = *reinterpret_cast<SampleShared *>(smem);
+    const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int row = blockIdx.x / blocks;
+    const int2 no_first = make_int2(0, 0), no_last = make_int2(BINS - 1, 0x7fffffff);      // where no thread finds an end
+    for (int i = tid; i < BINS; i += THREADS) s.hist[i] = 0;
+    if (tid < 2) s.windows[tid][0] = no_first, s.windows[tid][1] = no_last;
     pdl_prologue();
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const T *x = reinterpret_cast<const T *>(a.logits) + (size_t)row * a.vocab;
     const float temperature = a.temperature ? a.temperature[row] : a.temperature_all;
-    float top_p = a.top_p ? a.top_p[row] : a.top_p_all, min_p = a.min_p ? a.min_p[row] : a.min_p_all;
+    const float top_p = a.top_p ? a.top_p[row] : a.top_p_all, min_p = a.min_p ? a.min_p[row] : a.min_p_all;
     int top_k = a.top_k ? a.top_k[row] : a.top_k_all;
-    float u = a.u[row];
-    uint32_t best = 0;
-    for (int i = tid; i < a.vocab; i += blockDim.x) best = max(best, key_of(load_logit(x, i)));
-    best = __reduce_max_sync(0xffffffffu, best);
-    if (lane == 0) red32[warp] = best;
-    __syncthreads();
-    best = __reduce_max_sync(0xffffffffu, red32[lane]);
-    __syncthreads();
-    if (best == 0) {   // nothing can be chosen
-        if (tid == 0) a.token[row] = 0;
+    const float u = a.u[row];
+
+    // ---- the slice into shared memory; its largest logit, the first of equal ones ------------------------------------
+    const int n0 = rank * a.slice, n = min(a.slice, a.vocab - n0);      // may be none
+    const T *src = reinterpret_cast<const T *>(a.logits) + (size_t)row * a.vocab + n0;
+    constexpr int VEC = 16 / sizeof(T);
+    const int off = (int)(reinterpret_cast<uintptr_t>(src) & 15) / (int)sizeof(T);      // of the slice's first token in its 16 bytes
+    T *const slice = reinterpret_cast<T *>(smem + sizeof(SampleShared));
+    auto x = [&](int i) { return to_float(slice[off + i]); };
+    float top = -INFINITY;
+    int top_i = 0x7fffffff;
+#pragma unroll 4
+    for (int v = tid; v * VEC - off < n; v += THREADS) {
+        const int i0 = v * VEC - off;
+        uint4 raw;
+        T *t = reinterpret_cast<T *>(&raw);
+        if (i0 >= 0 && i0 + VEC <= n) {
+            raw = *reinterpret_cast<const uint4 *>(src + i0);
+        } else {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) t[k] = i0 + k >= 0 && i0 + k < n ? src[i0 + k] : T(-INFINITY);
+        }
+        *reinterpret_cast<uint4 *>(slice + v * VEC) = raw;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            const float f = to_float(t[k]);
+            if (f > top) top = f, top_i = n0 + i0 + k;      // never NaN or -infinity
+        }
+    }
+    {
+        unsigned long long best = top_i == 0x7fffffff ? 0ull : (unsigned long long)key_of(top) << 32 | (uint32_t)~top_i;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+        if (lane == 0) s.warp_best[warp] = best;
+        __syncthreads();
+        best = lane < WARPS ? s.warp_best[lane] : 0ull;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+        if (tid == 0) s.told[0].best = best;
+    }
+    cluster.sync();
+    unsigned long long best = lane < blocks ? cluster.map_shared_rank(&s.told[0], lane)->best : 0ull;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    const int best_i = (int)~(uint32_t)best;
+    // nothing can be chosen, or only one: 0, or the largest
+    if (best == 0 || !(temperature > 0.f) || top_k == 1 || top_p <= 0.f) {
+        if (rank == 0 && tid == 0) a.token[row] = best == 0 ? 0 : best_i;
+        cluster.sync();      // nobody leaves while its memory may be read
         return;
     }
-    const bool greedy = !(temperature > 0.f);
-    if (greedy) top_k = 1;
-    const Weights weight(logit_of(best), greedy ? 1.f : temperature);
-    uint32_t end = 1;                 // the kept prefix: keys above `end`, and the first `ties` of those that equal it
-    int ties = a.vocab;
-    if (top_k > 0 && top_k < a.vocab) {
-        uint32_t key = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t trial = key | 1u << bit;
-            int n = 0;
-            for (int i = tid; i < a.vocab; i += blockDim.x) n += key_of(load_logit(x, i)) >= trial;
-            if (block_total<int>(n, reinterpret_cast<int *>(red)) >= top_k) key = trial;
-        }
-        if (key > 0) {
-            int above = 0;
-            for (int i = tid; i < a.vocab; i += blockDim.x) above += key_of(load_logit(x, i)) > key;
-            end = key;
-            ties = top_k - block_total<int>(above, reinterpret_cast<int *>(red));
-        }
-    }
-    if (top_p < 1.f) {
-        mass_t over = 0;
-        int at = 0;
-        for (int i = tid; i < a.vocab; i += blockDim.x) {
-            const float v = load_logit(x, i);
-            const uint32_t k = key_of(v);
-            if (k > end) over += weight(v);
-            at += k == end;
-        }
-        over = block_total<mass_t>(over, red);
-        at = block_total<int>(at, reinterpret_cast<int *>(red));
-        const mass_t all = over + (mass_t)min(ties, at) * (at ? weight(logit_of(end)) : 0);
-        const double goal = (double)top_p * (double)all;
-        uint32_t key = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t trial = key | 1u << bit;
-            if (trial < end) {
-                key = trial;
-                continue;
-            }
-            mass_t s = 0;
-            for (int i = tid; i < a.vocab; i += blockDim.x) {
-                const float v = load_logit(x, i);
-                if (key_of(v) >= trial) s += weight(v);
-            }
-            s = block_total<mass_t>(s, red);
-            if (trial <= best && ((double)s >= goal)) key = trial;
-        }
-        if (key > end || (key == end && end > 1)) {
-            mass_t front = 0;
-            for (int i = tid; i < a.vocab; i += blockDim.x) {
-                const float v = load_logit(x, i);
-                if (key_of(v) > key) front += weight(v);
-            }
-            front = block_total<mass_t>(front, red);
-            const double w = (double)weight(logit_of(key));
-            const double need = ceil((goal - (double)front) / w);
-            const int n = need < 1. ? 1 : need > (double)a.vocab ? a.vocab : (int)need;
-            ties = key == end ? min(ties, n) : n;
-            end = key;
-        }
-    }
+    top = logit_of((uint32_t)(best >> 32));
+    const Weights weight(top, temperature);
+    auto coarse = [&](float v) { return v == top ? 0 : (int)fminf((top - v) * weight.c_hi * BIN_SCALE, (float)(BINS - 1)); };
+    // The histogram covers the coarse bins `from` .. `upto`, all of them at first: a token's bin, -1 in front of them and BINS behind.
+    int from = 0, upto = BINS - 1;
+    float fine = 1.f;      // bins to a coarse one
+    auto bin_of = [&](float v) {
+        const int b = coarse(v);
+        if (fine == 1.f) return b;
+        if (b < from || b > upto) return b < from ? -1 : BINS;
+        const float t = v == top ? 0.f : (top - v) * weight.c_hi * BIN_SCALE;
+        return (int)fminf(fmaxf((t - (float)from) * fine, 0.f), (float)(BINS - 1));
+    };
+    if (top_k <= 0 || top_k >= a.vocab) top_k = 0;
+    const bool has_p = top_p < 1.f;
     const double floor_w = (min_p > 0.f ? (double)fminf(min_p, 1.f) : 0.) * (double)(1ull << UNIT_BITS);
-    // total of what is kept, then the place where the running sum passes u * total
-    if (tid == 0) s_token = -1;
-    mass_t total = 0, goal = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        mass_t sum = 0;
-        int seen = 0;
-        for (int i0 = 0; i0 < a.vocab; i0 += blockDim.x) {
-            const int i = i0 + tid;
-            const float v = i < a.vocab ? load_logit(x, i) : -INFINITY;
-            const uint32_t k = i < a.vocab ? key_of(v) : 0;
-            const unsigned ballot = __ballot_sync(0xffffffffu, k == end);
-            if (lane == 0) s_ties[warp] = __popc(ballot);
-            __syncthreads();
-            int rank = seen + __popc(ballot & ((1u << lane) - 1));
-            for (int w = 0; w < 32; ++w) {
-                if (w < warp) rank += s_ties[w];
-                seen += s_ties[w];
-            }
-            mass_t w = 0;
-            if (k > end || (k == end && rank < ties)) {
-                w = weight(v);
-                if ((double)w < floor_w) w = 0;
-            }
-            mass_t run = w;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const mass_t t = __shfl_up_sync(0xffffffffu, run, o);
-                if (lane >= o) run += t;
-            }
-            if (lane == 31) s_warp[warp] = run;
-            __syncthreads();
-            mass_t in_front = sum;
-            for (int j = 0; j < 32; ++j) {
-                if (j < warp) in_front += s_warp[j];
-                sum += s_warp[j];
-            }
-            if (pass == 1 && w > 0 && in_front + run > goal && in_front + run - w <= goal) s_token = i;
-            __syncthreads();
+    int round = 1;
+    // Sum over the cluster of what the blocks tell, and over the blocks in front.  Thread 0's numbers count.
+    Told all, front;
+    auto exchange = [&](mass_t mass, int count, double bound) {
+        Told &mine = s.told[round & 1];
+        if (tid == 0) mine.mass = mass, mine.count = count, mine.bound = bound;
+        cluster.sync();
+        Told t = {};
+        if (lane < blocks) t = *cluster.map_shared_rank(&mine, lane);
+        ++round;
+        const bool before = lane < rank;
+        all.mass = warp_total(t.mass), all.count = warp_total(t.count), all.bound = warp_total(t.bound);
+        front.mass = warp_total(before ? t.mass : 0ull), front.count = warp_total(before ? t.count : 0), front.bound = warp_total(before ? t.bound : 0.);
+    };
+    // sums over the block; every thread gets them, and those of the warps in front of its own
+    mass_t warps_mass;
+    int warps_count;
+    auto block_sums = [&](mass_t mass, int count) {      // of the whole warp each
+        __syncthreads();
+        if (lane == 0) s.warp_mass[warp] = mass, s.warp_count[warp] = count;
+        __syncthreads();
+        const mass_t m = lane < WARPS ? s.warp_mass[lane] : 0ull;
+        const int c = lane < WARPS ? s.warp_count[lane] : 0;
+        warps_mass = warp_total(lane < warp ? m : 0ull), warps_count = warp_total(lane < warp ? c : 0);
+        if (warp == 0) {
+            const mass_t bm = warp_total(m);
+            const int bc = warp_total(c);
+            if (lane == 0) s.block_mass = bm, s.block_count = bc;
         }
-        if (pass == 0) {
-            total = sum;
-            u = u > 0.f ? u : 0.f;
-            const double g = (double)u * (double)total;
-            goal = g < (double)(total - 1) ? (mass_t)g : total - 1;   // u >= 1 is the last kept token
+        __syncthreads();
+    };
+    // a warp's part of the slice: neighbouring tokens, so that its order is the order of the indexes
+    const int part = ((max(n, 0) + WARPS - 1) / WARPS + 31) / 32 * 32;
+    const int w0 = min(warp * part, max(n, 0)), w1 = min(w0 + part, max(n, 0));
+
+    float end = -INFINITY;      // everything is kept, as far as it can be chosen
+    int ties = 0;
+
+    // ---- the ends bit by bit: the largest key at and above which there are `k` tokens, or weights of `goal` ----------------------------------
+    auto by_bits = [&](bool by_mass, int k, double goal) {
+        uint32_t key = 0;
+        mass_t in_front_m = 0;
+        int in_front_c = 0;
+        for (int bit = 31; bit >= -1; --bit) {
+            const uint32_t trial = bit >= 0 ? key | 1u << bit : key + 1;      // at last: what lies above the key
+            mass_t m = 0;
+            int c = 0;
+            for (int i = tid; i < n; i += THREADS) {
+                const uint32_t q = key_of(x(i));
+                if (q >= trial && q > 0) m += weight(x(i)), ++c;
+            }
+            block_sums(warp_total(m), warp_total(c));
+            exchange(s.block_mass, s.block_count, 0.);
+            if (bit < 0) in_front_m = all.mass, in_front_c = all.count;
+            else if (by_mass ? (double)all.mass >= goal && trial <= (uint32_t)(best >> 32) : all.count >= k) key = trial;
+        }
+        end = logit_of(key);
+        const mass_t w = weight(end);
+        int t;
+        if (by_mass) {
+            const double need = ceil((goal - (double)in_front_m) / (double)w);
+            t = need < 1. ? 1 : need > (double)a.vocab ? a.vocab : (int)need;
+        } else {
+            t = k - in_front_c;
+        }
+        ties = t;
+        return in_front_m + (mass_t)t * w;      // the weights of the prefix
+    };
+    // ---- tokens of the bins lo .. hi into the list of the cluster's first block, in the order of the indexes; exact weights in front ----------
+    int listed;
+    mass_t ahead;
+    auto gather = [&](int lo, int hi) {
+        mass_t m = 0;
+        int c = 0;
+        for (int i0 = w0; i0 < w1; i0 += 32) {
+            const int i = i0 + lane;
+            const float v = i < w1 ? x(i) : -INFINITY;
+            const int b = v > -INFINITY ? bin_of(v) : BINS;
+            if (b < lo) m += weight(v);
+            c += __popc(__ballot_sync(0xffffffffu, b >= lo && b <= hi));
+        }
+        block_sums(warp_total(m), c);
+        exchange(s.block_mass, s.block_count, 0.);
+        listed = all.count, ahead = all.mass;
+        if (listed > LIST) return;
+        int at = front.count + warps_count;
+        SampleShared &first = *cluster.map_shared_rank(&s, 0);
+        for (int i0 = w0; i0 < w1; i0 += 32) {
+            const int i = i0 + lane;
+            const float v = i < w1 ? x(i) : -INFINITY;
+            const int b = v > -INFINITY ? bin_of(v) : BINS;
+            const unsigned in = __ballot_sync(0xffffffffu, b >= lo && b <= hi);
+            if (in >> lane & 1) {
+                const int to = at + __popc(in & ((1u << lane) - 1));
+                first.list_x[to] = v, first.list_i[to] = n0 + i, first.list_w[to] = weight(v);
+            }
+            at += __popc(in);
+        }
+        cluster.sync();
+    };
+    // rank of a listed token, and the weights in front of it (equal logits: the lower index first)
+    auto rank_of = [&](int i, int &place, mass_t &before) {
+        const float v = s.list_x[i];
+        place = 0, before = 0;
+        for (int j = 0; j < listed; ++j) {
+            const float o = s.list_x[j];
+            if (o > v || (o == v && j < i)) ++place, before += s.list_w[j];
+        }
+    };
+    // the first block finds the last kept token of the list and tells the others
+    auto settle = [&](bool by_mass, int k, double goal) {
+        if (rank == 0) {
+            for (int i = tid; i < listed; i += THREADS) {
+                int place;
+                mass_t before;
+                rank_of(i, place, before);
+                const mass_t w = s.list_w[i];
+                // the last one kept: the k-th, or the one with which the weights pass the goal
+                const bool last = by_mass ? (double)(ahead + before) < goal && (double)(ahead + before + w) >= goal : place == k - 1;
+                if (last) {
+                    int equal = 1;
+                    for (int j = 0; j < i; ++j) equal += s.list_x[j] == s.list_x[i];
+                    const Found f = {s.list_x[i], equal, ahead + before + w};
+                    for (int b = 0; b < blocks; ++b) cluster.map_shared_rank(&s, b)->found = f;
+                }
+            }
+        }
+        cluster.sync();
+        end = s.found.end, ties = s.found.ties;
+        return s.found.mass;
+    };
+
+    bool done = false;
+    if (top_k > 0 || has_p) {
+        mass_t total = 0;
+        int before_c = 0, upto_c = 0;               // tokens of the histogram in front of this thread's bins, and with them
+        double before_b = 0., upto_b = 0., ratio = 0.;      // their weights at most; a bin's are above `ratio` of that
+        const int per = BINS / blocks / THREADS > 0 ? BINS / blocks / THREADS : 1, bin0 = rank * (BINS / blocks) + tid * per;
+        auto upper = [&](int b) { return (double)exp2f(-((float)from + (float)b / fine) / BIN_SCALE); };
+        // ---- histogram, its running sums over the cluster: a block has BINS / blocks bins, a thread a few neighbouring ones ---------------------
+        auto survey = [&](bool weights) {      // the weights in front of the bins, or of everything if these are all
+            mass_t m = 0, sum = 0;
+            for (int i = tid; i < n; i += THREADS) {
+                const float v = x(i);
+                if (v > -INFINITY) {
+                    const int b = bin_of(v);
+                    if (b >= 0 && b < BINS) atomicAdd(&s.hist[b], 1u);
+                    if (weights && (fine == 1.f || b < 0)) m += weight(v);
+                }
+            }
+            if (weights) {
+                block_sums(warp_total(m), 0);
+                exchange(s.block_mass, 0, 0.);
+                sum = all.mass;
+            } else {
+                cluster.sync();
+            }
+            int c = 0;
+            double bound = 0.;      // no weight of a bin is above its upper end's
+            for (int b = bin0; b < bin0 + per; ++b) {
+                int h = 0;
+                for (int o = 0; o < blocks; ++o) h += (int)cluster.map_shared_rank(&s, o)->hist[b];
+                c += h;
+                bound += h * upper(b);
+                if (blocks > 1) s.hist[b] = h;      // nobody else reads these of this block
+            }
+            const int run_c = warp_running(c, lane);
+            const double run_b = warp_running(bound, lane);
+            __syncthreads();
+            if (lane == 31) s.warp_count[warp] = run_c, s.warp_bound[warp] = run_b;
+            __syncthreads();
+            const int in_c = lane < WARPS ? s.warp_count[lane] : 0;
+            const double in_b = lane < WARPS ? s.warp_bound[lane] : 0.;
+            const int warps_c = warp_total(lane < warp ? in_c : 0), block_c = warp_total(in_c);
+            const double warps_b = warp_total(lane < warp ? in_b : 0.), block_b = warp_total(in_b);
+            exchange(0ull, block_c, block_b);
+            upto_c = front.count + warps_c + run_c, before_c = upto_c - c;
+            upto_b = front.bound + warps_b + run_b, before_b = upto_b - bound;
+            ratio = (double)exp2f(-1.f / (BIN_SCALE * fine)) - 4e-6;
+            return sum;
+        };
+        // Tells all blocks the first and the last bin that can hold the k-th token, or the one with which the weights pass a goal; each is found
+        // by one thread.
+        int place = 0;
+        int2 window[2];
+        auto look = [&](bool by_mass, int k, double goal) {
+            auto tell = [&](int which, int bin, int tokens) {
+                for (int o = 0; o < blocks; ++o) cluster.map_shared_rank(&s, o)->windows[place][which] = make_int2(bin, tokens);
+            };
+            place ^= 1;
+            if (tid == 0) s.windows[place ^ 1][0] = no_first, s.windows[place ^ 1][1] = no_last;      // for the next time: a barrier lies between
+            const double slack = 1e-5 * (all.bound < goal ? all.bound : goal), low = goal - slack, high = goal + slack;
+            if (by_mass ? (before_b < low && upto_b >= low) || (before_b * ratio < high && upto_b * ratio >= high) : before_c < k && upto_c >= k) {
+                int at = before_c;
+                double w = before_b;
+                for (int b = bin0; b < bin0 + per; ++b) {
+                    const int h = (int)s.hist[b];
+                    const double next = w + h * upper(b);
+                    if (by_mass ? w < low && next >= low : at < k && at + h >= k) tell(0, b, at);
+                    if (by_mass ? w * ratio < high && next * ratio >= high : at < k && at + h >= k) tell(1, b, at + h);
+                    at += h, w = next;
+                }
+            }
+            cluster.sync();
+            window[0] = s.windows[place][0], window[1] = s.windows[place][1];
+        };
+        // The same in two steps: where the window holds too many tokens to be ranked, it is surveyed again with bins that much finer.
+        auto narrow = [&](bool by_mass, int k, double goal) {
+            if (window[1].y - window[0].y <= FEW) return;
+            const int in_front = window[0].y;
+            from = window[0].x, upto = window[1].x, fine = (float)BINS / (float)(upto - from + 1);
+            __syncthreads();
+            for (int i = tid; i < BINS; i += THREADS) s.hist[i] = 0;
+            __syncthreads();
+            const mass_t ahead_of = survey(by_mass);
+            look(by_mass, k - in_front, (goal - (double)ahead_of) / (double)(1ull << UNIT_BITS));
+            window[0].y += in_front;      // tokens in front of it in all
+        };
+        total = survey(has_p);
+        if (all.count <= top_k) top_k = 0;      // no more than that can be chosen at all
+        if (top_k > 0) look(false, top_k, 0.);
+        else if (has_p) look(true, 0, (double)top_p * (double)total / (double)(1ull << UNIT_BITS));
+        if (top_k == 0 && !has_p) {
+            // nothing to look for
+        } else if (window[1].y <= ALONE) {
+            // ---- all that can be kept fits one block, a token per thread --------------------------------------------------------------------------
+            gather(0, window[1].x);
+            if (rank == 0) {
+                int place = 0x7fffffff;
+                mass_t before = 0, w = 0;
+                if (tid < listed) {
+                    rank_of(tid, place, before);
+                    if (top_k == 0 || place < top_k) w = s.list_w[tid];
+                }
+                if (has_p) {
+                    mass_t sum = total;
+                    if (top_k > 0) block_sums(warp_total(w), 0), sum = s.block_mass;
+                    if (place > 0 && !((double)before < (double)top_p * (double)sum)) w = 0;
+                }
+                if ((double)w < floor_w) w = 0;
+                const mass_t run = warp_running(w, lane);
+                block_sums(__shfl_sync(0xffffffffu, run, 31), 0);
+                const mass_t sum = s.block_mass, last = warps_mass + run;
+                const double g = (double)(u > 0.f ? u : 0.f) * (double)sum;
+                const mass_t goal = g < (double)(sum - 1) ? (mass_t)g : sum - 1;      // u >= 1 is the last kept token
+                if (w > 0 && last > goal && last - w <= goal) a.token[row] = s.list_i[tid];
+            }
+            done = true;
+        } else {
+            if (top_k > 0) {
+                narrow(false, top_k, 0.);
+                const int in_front = window[0].y;
+                gather(window[0].x, window[1].x);
+                total = listed <= LIST ? settle(false, top_k - in_front, 0.) : by_bits(false, top_k, 0.);
+            }
+            if (has_p) {
+                const float k_end = end;
+                const int k_ties = ties;
+                const double goal = (double)top_p * (double)total;
+                if (top_k > 0) {
+                    if (fine != 1.f) {      // the whole range again
+                        from = 0, upto = BINS - 1, fine = 1.f;
+                        __syncthreads();
+                        for (int i = tid; i < BINS; i += THREADS) s.hist[i] = 0;
+                        __syncthreads();
+                        survey(false);
+                    }
+                    look(true, 0, goal / (double)(1ull << UNIT_BITS));
+                }
+                narrow(true, 0, goal);
+                gather(window[0].x, window[1].x);
+                if (listed <= LIST) settle(true, 0, goal);
+                else (void)by_bits(true, 0, goal);
+                if (top_k > 0 && end == k_end) ties = min(ties, k_ties);      // the second prefix is part of the first
+            }
         }
     }
-    if (tid == 0) a.token[row] = s_token;
+
+    if (!done) {
+        // ---- what is kept, in the order of the indexes: sums of the warps, the blocks, then the place in one warp ---------------------------------
+        mass_t m = 0;
+        int c = 0;
+        for (int i = w0 + lane; i < w1; i += 32) {
+            const float v = x(i);
+            if (v > end) {
+                const mass_t w = weight(v);
+                if ((double)w >= floor_w) m += w;
+            } else if (v == end && end > -INFINITY) {
+                ++c;
+            }
+        }
+        m = warp_total(m), c = warp_total(c);
+        mass_t tie_w = end > -INFINITY ? weight(end) : 0;
+        if ((double)tie_w < floor_w) tie_w = 0;
+        block_sums(m, c);
+        exchange(s.block_mass, s.block_count, 0.);
+        // equal logits at the end: the first `ties` of them, so a block's share depends on those in front
+        mass_t sum = 0, in_front = 0;
+        for (int o = 0, seen = 0; o < blocks; ++o) {
+            const Told &t = *cluster.map_shared_rank(&s.told[(round - 1) & 1], o);
+            const mass_t all_of = t.mass + (mass_t)max(0, min(ties - seen, t.count)) * tie_w;
+            if (o < rank) in_front += all_of;
+            sum += all_of;
+            seen += t.count;
+        }
+        const double g = (double)(u > 0.f ? u : 0.f) * (double)sum;
+        const mass_t goal = g < (double)(sum - 1) ? (mass_t)g : sum - 1;      // u >= 1 is the last kept token
+        const int seen = front.count + warps_count;
+        const mass_t mine = m + (mass_t)max(0, min(ties - seen, c)) * tie_w;
+        const int seen_block = front.count;
+        const mass_t at = in_front + warps_mass + (mass_t)max(0, min(ties - seen_block, warps_count)) * tie_w;
+        if (at <= goal && at + mine > goal) {      // this warp's part holds it
+            mass_t run = at;
+            int tie = seen;
+            for (int i0 = w0; i0 < w1; i0 += 32) {
+                const int i = i0 + lane;
+                const float v = i < w1 ? x(i) : -INFINITY;
+                const unsigned equal = __ballot_sync(0xffffffffu, v == end && end > -INFINITY);
+                mass_t w = 0;
+                if (v > end) {
+                    w = weight(v);
+                    if ((double)w < floor_w) w = 0;
+                } else if ((equal >> lane & 1) && tie + __popc(equal & ((1u << lane) - 1)) < ties) {
+                    w = tie_w;
+                }
+                const mass_t upto = run + warp_running(w, lane);
+                if (w > 0 && upto > goal && upto - w <= goal) a.token[row] = n0 + i;
+                run = __shfl_sync(0xffffffffu, upto, 31);
+                tie += __popc(equal);
+                if (run > goal) break;
+            }
+        }
+    }
+    cluster.sync();      // nobody leaves while its memory may be read
+}
+
+template <typename T>
+int launch_sample(SampleArgs a, int rows, void *stream) {
+    // Blocks of a row: enough to fill the GPU with few rows, a slice of 4096 tokens or more each, as far as shared memory goes.
+    int blocks = MAX_CLUSTER;
+    while (blocks > 1 && (a.vocab / blocks < 2048 || (long long)rows * blocks > 4 * 148)) {
+        if (a.vocab / (blocks / 2) > 36000) break;
+        blocks /= 2;
+    }
+    a.slice = ((a.vocab + blocks - 1) / blocks + 7) / 8 * 8;
+    const size_t smem = sizeof(SampleShared) + ((size_t)a.slice + 16) * sizeof(T);
+    static std::atomic<bool> configured[64];
+    auto kernel = sample_kernel<T>;
+    if (sal_allow_shared_memory(kernel, configured) != cudaSuccess) return SAL_E_LAUNCH;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)rows * blocks);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)blocks;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? SAL_OK : SAL_E_LAUNCH;
 }
 
 }  // namespace
@@ -229,7 +586,6 @@ extern "C" int sal_sample_token(const void *logits, int logits_f32, int rows, in
     if (!logits || !u || !token) return SAL_E_NULL;
     if (rows < 1 || rows > 65535 || vocab < 1 || vocab > MAX_VOCAB) return SAL_E_SHAPE;
     const SampleArgs a = {logits, reinterpret_cast<const float *>(u), reinterpret_cast<const float *>(temperature), reinterpret_cast<const float *>(top_p),
-                          reinterpret_cast<const float *>(min_p), top_k, temperature_all, top_p_all, min_p_all, top_k_all, vocab, token};
-    if (logits_f32) return sal_launch_pdl(sample_kernel<float>, dim3(rows), dim3(1024), 0, stream, a);
-    return sal_launch_pdl(sample_kernel<__half>, dim3(rows), dim3(1024), 0, stream, a);
+                          reinterpret_cast<const float *>(min_p), top_k, temperature_all, top_p_all, min_p_all, top_k_all, vocab, 0, token};
+    return logits_f32 ? launch_sample<float>(a, rows, stream) : launch_sample<__half>(a, rows, stream);
 }
