@@ -49,18 +49,20 @@ struct Weights {
         c_hi = c > 1e30 ? 1e30f : (float)c;
         c_lo = c > 1e30 ? 0.f : (float)(c - (double)c_hi);
     }
-    // w in units of 2**-44.  The exponent is formed with its rounding errors (of the difference and of the product) and the error applied
-    // to the power: 1.5e-7 relative, against the 1e-6 that a 32-bit exponent of 16 would cost.
+    // w in units of 2**-44, rounded down.  The exponent is formed with its rounding errors (of the difference and of the product) and the error applied
+    // to the power: 3e-7 relative, against the 1e-6 that a 32-bit exponent of 16 would cost.
     __device__ __forceinline__ mass_t operator()(float x) const {
-        if (x == top) return 1ull << UNIT_BITS;
         const float d = x - top;
         const float bb = d - x;
         const float de = (x - (d - bb)) - (top + bb);
         const float t = d * c_hi;
-        if (!(t > -46.f)) return 0;
         const float te = fmaf(d, c_hi, -t) + fmaf(d, c_lo, de * c_hi);
-        const float w = exp2f(t);
-        return (mass_t)__float2ll_rn(fmaf(w, te * 0.69314718f, w) * 17592186044416.f);
+        float w;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(t));
+        w = t > -46.f ? fmaf(w, te * 0.69314718f, w) : 0.f;
+        const uint32_t b = __float_as_uint(w);
+        const mass_t m = (mass_t)(b & 0x7fffffu | 0x800000u) << (UNIT_BITS - 23) >> min(127u - (b >> 23), 63u);
+        return x == top ? 1ull << UNIT_BITS : m;
     }
 };
 
@@ -199,20 +201,15 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
     }
     top = logit_of((uint32_t)(best >> 32));
     const Weights weight(top, temperature);
-    auto coarse = [&](float v) { return v == top ? 0 : (int)fminf((top - v) * weight.c_hi * BIN_SCALE, (float)(BINS - 1)); };
-    // The histogram covers the coarse bins `from` .. `upto`, all of them at first: a token's bin, -1 in front of them and BINS behind.
+    // A logit's place on the scale of the bins.  The histogram covers the coarse bins `from` .. `upto`, all of them at first.
+    const float bins = weight.c_hi * BIN_SCALE;
+    auto place_of = [&](float v) { return v == top ? 0.f : fminf((top - v) * bins, (float)(BINS - 1)); };
     int from = 0, upto = BINS - 1;
     float fine = 1.f;      // bins to a coarse one
-    auto bin_of = [&](float v) {
-        const int b = coarse(v);
-        if (fine == 1.f) return b;
-        if (b < from || b > upto) return b < from ? -1 : BINS;
-        const float t = v == top ? 0.f : (top - v) * weight.c_hi * BIN_SCALE;
-        return (int)fminf(fmaxf((t - (float)from) * fine, 0.f), (float)(BINS - 1));
-    };
+    auto bin_at = [&](float t) { return fine == 1.f ? (int)t : (int)fminf((t - (float)from) * fine, (float)(BINS - 1)); };      // of a place in the range
     if (top_k <= 0 || top_k >= a.vocab) top_k = 0;
     const bool has_p = top_p < 1.f;
-    const double floor_w = (min_p > 0.f ? (double)fminf(min_p, 1.f) : 0.) * (double)(1ull << UNIT_BITS);
+    const mass_t floor_w = min_p > 0.f ? (mass_t)ceil((double)fminf(min_p, 1.f) * (double)(1ull << UNIT_BITS)) : 0;
     int round = 1;
     // Sum over the cluster of what the blocks tell, and over the blocks in front.  Thread 0's numbers count.
     Told all, front;
@@ -248,6 +245,8 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
     const int part = ((max(n, 0) + WARPS - 1) / WARPS + 31) / 32 * 32;
     const int w0 = min(warp * part, max(n, 0)), w1 = min(w0 + part, max(n, 0));
 
+    mass_t warp_front = 0, warp_kept = 0;      // of the warp's part: the weights in front of the bin `from`, and those of them that min_p keeps
+    bool front_known = false;
     float end = -INFINITY;      // everything is kept, as far as it can be chosen
     int ties = 0;
 
@@ -284,33 +283,59 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
     // ---- tokens of the bins lo .. hi into the list of the cluster's first block, in the order of the indexes; exact weights in front ----------
     int listed;
     mass_t ahead;
-    auto gather = [&](int lo, int hi) {
-        mass_t m = 0;
+    auto gather = [&](int lo, int hi, bool by_mass) {
+        // places of the bins: where the histogram is a fine one, its range first
+        const bool narrowed = fine != 1.f;
+        const float p0 = narrowed ? (float)from : (float)lo, p1 = narrowed ? (float)(upto + 1) : (float)(hi + 1);
+        auto in_window = [&](float t) {
+            const int b = bin_at(t);
+            return b >= lo && b <= hi;
+        };
+        mass_t m = 0, kept = 0;
         int c = 0;
+#pragma unroll 2
         for (int i0 = w0; i0 < w1; i0 += 32) {
             const int i = i0 + lane;
             const float v = i < w1 ? x(i) : -INFINITY;
-            const int b = v > -INFINITY ? bin_of(v) : BINS;
-            if (b < lo) m += weight(v);
-            c += __popc(__ballot_sync(0xffffffffu, b >= lo && b <= hi));
+            const float t = v > -INFINITY ? place_of(v) : (float)BINS;
+            bool in = t >= p0 && t < p1;
+            if (narrowed && in) {
+                if (bin_at(t) < lo) m += weight(v);
+                in = in_window(t);
+            } else if (!narrowed && by_mass && t < p0) {
+                const mass_t w = weight(v);
+                m += w;
+                if (w >= floor_w) kept += w;
+            }
+            c += __popc(__ballot_sync(0xffffffffu, in));
         }
-        block_sums(warp_total(m), c);
+        m = warp_total(m);
+        if (narrowed) {
+            m += warp_front;
+        } else if (by_mass) {
+            from = lo;
+            warp_front = m, warp_kept = warp_total(kept), front_known = true;
+        }
+        block_sums(m, c);
         exchange(s.block_mass, s.block_count, 0.);
         listed = all.count, ahead = all.mass;
         if (listed > LIST) return;
         int at = front.count + warps_count;
         SampleShared &first = *cluster.map_shared_rank(&s, 0);
-        for (int i0 = w0; i0 < w1; i0 += 32) {
-            const int i = i0 + lane;
-            const float v = i < w1 ? x(i) : -INFINITY;
-            const int b = v > -INFINITY ? bin_of(v) : BINS;
-            const unsigned in = __ballot_sync(0xffffffffu, b >= lo && b <= hi);
-            if (in >> lane & 1) {
-                const int to = at + __popc(in & ((1u << lane) - 1));
-                first.list_x[to] = v, first.list_i[to] = n0 + i, first.list_w[to] = weight(v);
+        if (c > 0)
+#pragma unroll 2
+            for (int i0 = w0; i0 < w1; i0 += 32) {
+                const int i = i0 + lane;
+                const float v = i < w1 ? x(i) : -INFINITY;
+                const float t = v > -INFINITY ? place_of(v) : (float)BINS;
+                const bool in = t >= p0 && t < p1 && in_window(t);
+                const unsigned all_in = __ballot_sync(0xffffffffu, in);
+                if (in) {
+                    const int to = at + __popc(all_in & ((1u << lane) - 1));
+                    first.list_x[to] = v, first.list_i[to] = n0 + i, first.list_w[to] = weight(v);
+                }
+                at += __popc(all_in);
             }
-            at += __popc(in);
-        }
         cluster.sync();
     };
     // rank of a listed token, and the weights in front of it (equal logits: the lower index first)
@@ -354,17 +379,24 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
         auto upper = [&](int b) { return (double)exp2f(-((float)from + (float)b / fine) / BIN_SCALE); };
         // ---- histogram, its running sums over the cluster: a block has BINS / blocks bins, a thread a few neighbouring ones ---------------------
         auto survey = [&](bool weights) {      // the weights in front of the bins, or of everything if these are all
-            mass_t m = 0, sum = 0;
-            for (int i = tid; i < n; i += THREADS) {
+            mass_t m = 0, kept = 0, sum = 0;
+            const float lo = (float)from, hi = (float)(upto + 1);
+#pragma unroll 2
+            for (int i = w0 + lane; i < w1; i += 32) {
                 const float v = x(i);
-                if (v > -INFINITY) {
-                    const int b = bin_of(v);
-                    if (b >= 0 && b < BINS) atomicAdd(&s.hist[b], 1u);
-                    if (weights && (fine == 1.f || b < 0)) m += weight(v);
+                if (!(v > -INFINITY)) continue;
+                const float t = place_of(v);
+                if (t >= lo && t < hi) atomicAdd(&s.hist[bin_at(t)], 1u);
+                if (weights && (fine == 1.f || t < lo)) {
+                    const mass_t w = weight(v);
+                    m += w;
+                    if (w >= floor_w) kept += w;
                 }
             }
+            m = warp_total(m);
+            if (weights && fine != 1.f) warp_front = m, warp_kept = warp_total(kept), front_known = true;
             if (weights) {
-                block_sums(warp_total(m), 0);
+                block_sums(m, 0);
                 exchange(s.block_mass, 0, 0.);
                 sum = all.mass;
             } else {
@@ -439,7 +471,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
             // nothing to look for
         } else if (window[1].y <= ALONE) {
             // ---- all that can be kept fits one block, a token per thread --------------------------------------------------------------------------
-            gather(0, window[1].x);
+            gather(0, window[1].x, false);
             if (rank == 0) {
                 int place = 0x7fffffff;
                 mass_t before = 0, w = 0;
@@ -452,7 +484,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
                     if (top_k > 0) block_sums(warp_total(w), 0), sum = s.block_mass;
                     if (place > 0 && !((double)before < (double)top_p * (double)sum)) w = 0;
                 }
-                if ((double)w < floor_w) w = 0;
+                if (w < floor_w) w = 0;
                 const mass_t run = warp_running(w, lane);
                 block_sums(__shfl_sync(0xffffffffu, run, 31), 0);
                 const mass_t sum = s.block_mass, last = warps_mass + run;
@@ -465,7 +497,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
             if (top_k > 0) {
                 narrow(false, top_k, 0.);
                 const int in_front = window[0].y;
-                gather(window[0].x, window[1].x);
+                gather(window[0].x, window[1].x, false);
                 total = listed <= LIST ? settle(false, top_k - in_front, 0.) : by_bits(false, top_k, 0.);
             }
             if (has_p) {
@@ -474,7 +506,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
                 const double goal = (double)top_p * (double)total;
                 if (top_k > 0) {
                     if (fine != 1.f) {      // the whole range again
-                        from = 0, upto = BINS - 1, fine = 1.f;
+                        from = 0, upto = BINS - 1, fine = 1.f, front_known = false;
                         __syncthreads();
                         for (int i = tid; i < BINS; i += THREADS) s.hist[i] = 0;
                         __syncthreads();
@@ -483,7 +515,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
                     look(true, 0, goal / (double)(1ull << UNIT_BITS));
                 }
                 narrow(true, 0, goal);
-                gather(window[0].x, window[1].x);
+                gather(window[0].x, window[1].x, true);
                 if (listed <= LIST) settle(true, 0, goal);
                 else (void)by_bits(true, 0, goal);
                 if (top_k > 0 && end == k_end) ties = min(ties, k_ties);      // the second prefix is part of the first
@@ -495,18 +527,21 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
         // ---- what is kept, in the order of the indexes: sums of the warps, the blocks, then the place in one warp ---------------------------------
         mass_t m = 0;
         int c = 0;
+        const float p0 = front_known ? (float)from : 0.f;
+#pragma unroll 2
         for (int i = w0 + lane; i < w1; i += 32) {
             const float v = x(i);
             if (v > end) {
+                if (place_of(v) < p0) continue;      // counted already
                 const mass_t w = weight(v);
-                if ((double)w >= floor_w) m += w;
+                if (w >= floor_w) m += w;
             } else if (v == end && end > -INFINITY) {
                 ++c;
             }
         }
-        m = warp_total(m), c = warp_total(c);
+        m = warp_total(m) + (front_known ? warp_kept : 0), c = warp_total(c);
         mass_t tie_w = end > -INFINITY ? weight(end) : 0;
-        if ((double)tie_w < floor_w) tie_w = 0;
+        if (tie_w < floor_w) tie_w = 0;
         block_sums(m, c);
         exchange(s.block_mass, s.block_count, 0.);
         // equal logits at the end: the first `ties` of them, so a block's share depends on those in front
@@ -534,7 +569,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
                 mass_t w = 0;
                 if (v > end) {
                     w = weight(v);
-                    if ((double)w < floor_w) w = 0;
+                    if (w < floor_w) w = 0;
                 } else if ((equal >> lane & 1) && tie + __popc(equal & ((1u << lane) - 1)) < ties) {
                     w = tie_w;
                 }
@@ -553,7 +588,7 @@ template <typename T>
 int launch_sample(SampleArgs a, int rows, void *stream) {
     // Blocks of a row: enough to fill the GPU with few rows, a slice of 4096 tokens or more each, as far as shared memory goes.
     int blocks = MAX_CLUSTER;
-    while (blocks > 1 && (a.vocab / blocks < 2048 || (long long)rows * blocks > 4 * 148)) {
+    while (blocks > 1 && (a.vocab / blocks < 2048 || (long long)rows * blocks > 2 * 148)) {
         if (a.vocab / (blocks / 2) > 36000) break;
         blocks /= 2;
     }
