@@ -77,11 +77,11 @@ struct SampleArgs {
     int64_t *token;
 };
 
-constexpr int THREADS = 512, WARPS = THREADS / 32;
+constexpr int MAX_WARPS = 32;
 constexpr int BINS = 4096;
 constexpr float BIN_SCALE = 89.f;                  // bins to a factor of two: 46 factors fit, behind them a weight is 0
 constexpr int LIST = 1024;                         // tokens that can be ranked
-constexpr int ALONE = THREADS;                     // so few that one block finishes, a token per thread
+constexpr int ALONE = 512;                         // so few that one block finishes, a token per thread
 constexpr int FEW = 256;                           // a window of so many is ranked at once
 constexpr int MAX_CLUSTER = 8;
 
@@ -104,16 +104,18 @@ struct alignas(16) SampleShared {
     Told told[2];
     Found found;
     int2 windows[2][2];     // first bin and the tokens in front of it, last bin and the tokens up to it; two places in turn
-    mass_t warp_mass[WARPS];
-    double warp_bound[WARPS];
-    int warp_count[WARPS];
-    unsigned long long warp_best[WARPS];
+    mass_t warp_mass[MAX_WARPS];
+    double warp_bound[MAX_WARPS];
+    int warp_count[MAX_WARPS];
+    unsigned long long warp_best[MAX_WARPS];
     mass_t block_mass;
     int block_count;
     uint32_t hist[BINS];
     float list_x[LIST];
     int list_i[LIST];
     mass_t list_w[LIST];
+    mass_t list_before[LIST];
+    int list_place[LIST];
 };
 
 template <typename V>
@@ -132,8 +134,9 @@ __device__ __forceinline__ V warp_running(V v, int lane) {      // inclusive
     return v;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleArgs a) {
+    constexpr int WARPS = THREADS / 32;
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     extern __shared__ __align__(16) uint8_t smem[];
@@ -305,10 +308,11 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
             } else if (!narrowed && by_mass && t < p0) {
                 const mass_t w = weight(v);
                 m += w;
-                if (w >= floor_w) kept += w;
+                if (floor_w > 0 && w >= floor_w) kept += w;
             }
             c += __popc(__ballot_sync(0xffffffffu, in));
         }
+        if (floor_w == 0) kept = m;
         m = warp_total(m);
         if (narrowed) {
             m += warp_front;
@@ -338,22 +342,25 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
             }
         cluster.sync();
     };
-    // rank of a listed token, and the weights in front of it (equal logits: the lower index first)
-    auto rank_of = [&](int i, int &place, mass_t &before) {
-        const float v = s.list_x[i];
-        place = 0, before = 0;
-        for (int j = 0; j < listed; ++j) {
-            const float o = s.list_x[j];
-            if (o > v || (o == v && j < i)) ++place, before += s.list_w[j];
+    // Ranks of the listed tokens and the weights in front of them (equal logits: the lower index first): a token per warp, the others over its lanes.
+    auto rank_all = [&](auto use) {
+        const int count = min(listed, LIST);
+        for (int i = warp; i < count; i += WARPS) {
+            const float v = s.list_x[i];
+            int place = 0;
+            mass_t before = 0;
+            for (int j = lane; j < count; j += 32) {
+                const float o = s.list_x[j];
+                if (o > v || (o == v && j < i)) ++place, before += s.list_w[j];
+            }
+            place = __reduce_add_sync(0xffffffffu, place), before = warp_total(before);
+            if (lane == 0) use(i, place, before);
         }
     };
-    // the first block finds the last kept token of the list and tells the others
+    // the first block finds the last kept token of the list
     auto settle = [&](bool by_mass, int k, double goal) {
         if (rank == 0) {
-            for (int i = tid; i < listed; i += THREADS) {
-                int place;
-                mass_t before;
-                rank_of(i, place, before);
+            rank_all([&](int i, int place, mass_t before) {
                 const mass_t w = s.list_w[i];
                 // the last one kept: the k-th, or the one with which the weights pass the goal
                 const bool last = by_mass ? (double)(ahead + before) < goal && (double)(ahead + before + w) >= goal : place == k - 1;
@@ -361,21 +368,23 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
                     int equal = 1;
                     for (int j = 0; j < i; ++j) equal += s.list_x[j] == s.list_x[i];
                     const Found f = {s.list_x[i], equal, ahead + before + w};
-                    for (int b = 0; b < blocks; ++b) cluster.map_shared_rank(&s, b)->found = f;
+                    s.found = f;
                 }
-            }
+            });
         }
         cluster.sync();
-        end = s.found.end, ties = s.found.ties;
-        return s.found.mass;
+        const Found f = cluster.map_shared_rank(&s, 0)->found;
+        end = f.end, ties = f.ties;
+        return f.mass;
     };
 
     bool done = false;
     if (top_k > 0 || has_p) {
         mass_t total = 0;
         int before_c = 0, upto_c = 0;               // tokens of the histogram in front of this thread's bins, and with them
-        double before_b = 0., upto_b = 0., ratio = 0.;      // their weights at most; a bin's are above `ratio` of that
-        const int per = BINS / blocks / THREADS > 0 ? BINS / blocks / THREADS : 1, bin0 = rank * (BINS / blocks) + tid * per;
+        double before_b = 0., upto_b = 0., all_b = 0., ratio = 0.;      // their weights at most; a bin's are above `ratio` of that
+        const int mine = BINS / blocks, per = mine > THREADS ? mine / THREADS : 1;      // bins of a block and of a thread (of the first threads, where there are fewer bins)
+        const int bin0 = rank * mine + min(tid * per, mine), bin1 = rank * mine + min(tid * per + per, mine);
         auto upper = [&](int b) { return (double)exp2f(-((float)from + (float)b / fine) / BIN_SCALE); };
         // ---- histogram, its running sums over the cluster: a block has BINS / blocks bins, a thread a few neighbouring ones ---------------------
         auto survey = [&](bool weights) {      // the weights in front of the bins, or of everything if these are all
@@ -390,9 +399,10 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
                 if (weights && (fine == 1.f || t < lo)) {
                     const mass_t w = weight(v);
                     m += w;
-                    if (w >= floor_w) kept += w;
+                    if (floor_w > 0 && w >= floor_w) kept += w;
                 }
             }
+            if (floor_w == 0) kept = m;
             m = warp_total(m);
             if (weights && fine != 1.f) warp_front = m, warp_kept = warp_total(kept), front_known = true;
             if (weights) {
@@ -404,7 +414,7 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
             }
             int c = 0;
             double bound = 0.;      // no weight of a bin is above its upper end's
-            for (int b = bin0; b < bin0 + per; ++b) {
+            for (int b = bin0; b < bin1; ++b) {
                 int h = 0;
                 for (int o = 0; o < blocks; ++o) h += (int)cluster.map_shared_rank(&s, o)->hist[b];
                 c += h;
@@ -423,24 +433,25 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
             exchange(0ull, block_c, block_b);
             upto_c = front.count + warps_c + run_c, before_c = upto_c - c;
             upto_b = front.bound + warps_b + run_b, before_b = upto_b - bound;
+            all_b = all.bound;
             ratio = (double)exp2f(-1.f / (BIN_SCALE * fine)) - 4e-6;
             return sum;
         };
-        // Tells all blocks the first and the last bin that can hold the k-th token, or the one with which the weights pass a goal; each is found
-        // by one thread.
+        // Finds the first and the last bin that can hold the k-th token, or the one with which the weights pass a goal; each is found
+        // by one thread, which tells the first block.
         int place = 0;
         int2 window[2];
         auto look = [&](bool by_mass, int k, double goal) {
             auto tell = [&](int which, int bin, int tokens) {
-                for (int o = 0; o < blocks; ++o) cluster.map_shared_rank(&s, o)->windows[place][which] = make_int2(bin, tokens);
+                cluster.map_shared_rank(&s, 0)->windows[place][which] = make_int2(bin, tokens);
             };
             place ^= 1;
             if (tid == 0) s.windows[place ^ 1][0] = no_first, s.windows[place ^ 1][1] = no_last;      // for the next time: a barrier lies between
-            const double slack = 1e-5 * (all.bound < goal ? all.bound : goal), low = goal - slack, high = goal + slack;
+            const double slack = 1e-5 * (all_b < goal ? all_b : goal), low = goal - slack, high = goal + slack;
             if (by_mass ? (before_b < low && upto_b >= low) || (before_b * ratio < high && upto_b * ratio >= high) : before_c < k && upto_c >= k) {
                 int at = before_c;
                 double w = before_b;
-                for (int b = bin0; b < bin0 + per; ++b) {
+                for (int b = bin0; b < bin1; ++b) {
                     const int h = (int)s.hist[b];
                     const double next = w + h * upper(b);
                     if (by_mass ? w < low && next >= low : at < k && at + h >= k) tell(0, b, at);
@@ -449,7 +460,9 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
                 }
             }
             cluster.sync();
-            window[0] = s.windows[place][0], window[1] = s.windows[place][1];
+            // one copy for all blocks: they have to agree on it, even where rounding let two threads find an end
+            const SampleShared &first = *cluster.map_shared_rank(&s, 0);
+            window[0] = first.windows[place][0], window[1] = first.windows[place][1];
         };
         // The same in two steps: where the window holds too many tokens to be ranked, it is surveyed again with bins that much finer.
         auto narrow = [&](bool by_mass, int k, double goal) {
@@ -475,8 +488,10 @@ __global__ void __launch_bounds__(THREADS) sample_kernel(SampleArgs a) {
             if (rank == 0) {
                 int place = 0x7fffffff;
                 mass_t before = 0, w = 0;
+                rank_all([&](int i, int p, mass_t b) { s.list_place[i] = p, s.list_before[i] = b; });
+                __syncthreads();
                 if (tid < listed) {
-                    rank_of(tid, place, before);
+                    place = s.list_place[tid], before = s.list_before[tid];
                     if (top_k == 0 || place < top_k) w = s.list_w[tid];
                 }
                 if (has_p) {
@@ -594,12 +609,14 @@ int launch_sample(SampleArgs a, int rows, void *stream) {
     }
     a.slice = ((a.vocab + blocks - 1) / blocks + 7) / 8 * 8;
     const size_t smem = sizeof(SampleShared) + ((size_t)a.slice + 16) * sizeof(T);
-    static std::atomic<bool> configured[64];
-    auto kernel = sample_kernel<T>;
-    if (sal_allow_shared_memory(kernel, configured) != cudaSuccess) return SAL_E_LAUNCH;
+    // Twice the threads where a block has an SM to itself and a long slice (one row of 131071, top-p: 41.5 us, 46.5 with 512; of 32000: 25.5, 22).
+    const bool wide = (long long)rows * blocks <= 148 && a.slice > 8192;
+    static std::atomic<bool> configured[2][64];
+    auto kernel = wide ? sample_kernel<T, 1024> : sample_kernel<T, 512>;
+    if (sal_allow_shared_memory(kernel, configured[wide]) != cudaSuccess) return SAL_E_LAUNCH;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * blocks);
-    cfg.blockDim = dim3(THREADS);
+    cfg.blockDim = dim3(wide ? 1024 : 512);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = reinterpret_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[2];
