@@ -69,7 +69,7 @@ def build(force: bool = False, verbose: bool = False, measure: bool = False) -> 
 
 
 EXT_DIR = os.path.join(PKG_DIR, "ext")
-EXT_SRC = os.path.join(PKG_DIR, "csrc", "lutgemm_ext.cpp")
+EXT_SRCS = [os.path.join(PKG_DIR, "csrc", name) for name in ("lutgemm_ext.cpp", "decode_ext.cpp")]
 
 
 def extension_path() -> str:
@@ -80,7 +80,15 @@ def extension_path() -> str:
 
 def extension_up_to_date() -> bool:
     out = extension_path()
-    return os.path.exists(out) and all(os.path.getmtime(p) <= os.path.getmtime(out) for p in (EXT_SRC, HDRS[0], os.path.abspath(__file__)))
+    return os.path.exists(out) and all(os.path.getmtime(p) <= os.path.getmtime(out) for p in (*EXT_SRCS, *HDRS[:2], os.path.abspath(__file__)))
+
+
+def cxx_runtime() -> list[str]:
+    """Link flags that name the C++ runtime library which torch has loaded.  A compiler whose own copy of it is a static one would put a
+    second runtime into the module, and a number in an error message would then end the process."""
+    with open("/proc/self/maps") as f:
+        loaded = sorted({line.split()[-1] for line in f if "libstdc++.so" in line})
+    return ["-nostdlib++", loaded[0]] if loaded else []
 
 
 def build_extension(force: bool = False) -> str:
@@ -106,8 +114,8 @@ def build_extension(force: bool = False) -> str:
            "-I", os.path.join(REPO_DIR, "include"), "-I", sysconfig.get_paths()["include"], "-I", os.path.join(cuda_home, "include")]
     for inc in cpp_extension.include_paths():
         cmd += ["-isystem", inc]
-    cmd += ["-o", out, EXT_SRC, LIB, "-L", torch_lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
-            "-Wl,-rpath,$ORIGIN/..", f"-Wl,-rpath,{torch_lib}"]
+    cmd += ["-o", out, *EXT_SRCS, LIB, "-L", torch_lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
+            *cxx_runtime(), "-Wl,-rpath,$ORIGIN/..", f"-Wl,-rpath,{torch_lib}"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)

@@ -243,6 +243,8 @@ torch::Tensor lut_linear(const torch::Tensor &x, const torch::Tensor &bWeight, c
 
 }  // namespace
 
+void register_decode_ops(pybind11::module_ &m);   // decode_ext.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "BCQ LUT-GEMM for NVIDIA B200 (sm_100a): drop-in for ShiftAddLLM's compiled lutgemm extension";
     namespace py = pybind11;
@@ -257,5 +259,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("nb"), py::arg("num_groups"), py::arg("pdl") = false, release());
     m.def("lut_linear", &lut_linear, "the product of LutLinear.forward: rows of x times the packed layer, bias added", py::arg("x"), py::arg("bWeight"),
           py::arg("alpha"), py::arg("bias"), py::arg("K"), py::arg("N"), py::arg("wbit"), py::arg("row_layout"), release());
+    register_decode_ops(m);
     m.def("sal_version", []() { return sal_version(); });
 }

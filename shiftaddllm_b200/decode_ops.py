@@ -6,6 +6,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import warnings
 
 import torch
 
@@ -169,6 +170,25 @@ def causal_softmax(scores, first: int, scale: float):
 KV4_PAGE = _lib.SAL_KV4_PAGE
 
 
+_compiled = None   # the compiled module with these calls; False where it has not been built or cannot be imported
+
+
+def _native():
+    """The compiled module (csrc/decode_ext.cpp), whose calls make the checks below in a few microseconds less, or False."""
+    global _compiled
+    if _compiled is None:
+        from . import lutgemm
+
+        _lib.load()   # the module links to the library by name: the one loaded here is the one it finds
+        try:
+            module = lutgemm.compiled_module()
+            _compiled = module if hasattr(module, "attention_kv4") else False
+        except (RuntimeError, ImportError, OSError) as e:   # not built, or for another interpreter or torch
+            warnings.warn(f"the compiled module cannot be imported, the 4-bit cache's calls take their steps in Python: {e}")
+            _compiled = False
+    return _compiled
+
+
 def _want(what, name, t, dtype, shape, device):
     """`t` is a contiguous tensor of this dtype on this device; `shape`: so many numbers in all, so many in its last dimension."""
     if not isinstance(t, torch.Tensor):
@@ -218,6 +238,9 @@ def rope_kv4_write(q, k, v, cos, sin, pos, table, pool, q_out, heads, kv_heads, 
     unwritten, stand in include/sal_decode_ops.h).  q, q_out fp16 [batch, m, heads * hd] (q_out may be q), k, v fp16 [batch, m, kv_heads * hd],
     cos, sin fp32 [max_len, hd / 2], pos int64 [batch]: position of each sequence's first new row, table int32 [batch, pages of a sequence],
     pool: one layer's uint8 [pages, kv_heads, record].  rows int32 [batch]: how many of the m rows there are (None: all)."""
+    native = _compiled if _compiled is not None else _native()
+    if native:
+        return native.rope_kv4_write(q, k, v, cos, sin, pos, table, pool, q_out, heads, kv_heads, hd, rows)
     device, batch, max_pages, pages = _kv4_pool_check("rope_kv4_write", pool, table, pos, rows, kv_heads, hd)
     m = _rows_per_sequence("rope_kv4_write", "q", q, batch, heads * hd)
     for name, t, width in (("q", q, heads), ("q_out", q_out, heads), ("k", k, kv_heads), ("v", v, kv_heads)):
@@ -234,6 +257,9 @@ def rope_kv4_write(q, k, v, cos, sin, pos, table, pool, q_out, heads, kv_heads, 
 def read_kv4(pool, table, pos, k_out, v_out, kv_heads, hd):
     """The values of m positions of each sequence, from pos[b] on: k_out and v_out [batch, m, kv_heads, hd] in float32 (as they are) or
     float16 (rounded); zeros where a sequence has no page."""
+    native = _compiled if _compiled is not None else _native()
+    if native:
+        return native.read_kv4(pool, table, pos, k_out, v_out, kv_heads, hd)
     device, batch, max_pages, pages = _kv4_pool_check("read_kv4", pool, table, pos, None, kv_heads, hd)
     m = _rows_per_sequence("read_kv4", "k_out", k_out, batch, kv_heads * hd)
     if k_out.dtype not in (torch.float32, torch.float16):
@@ -258,6 +284,9 @@ def attention_kv4_workspace(batch: int, m: int, heads: int, kv_heads: int, hd: i
 def attention_kv4(q, pool, table, pos, out, heads, kv_heads, hd, scale: float, workspace, rows=None):
     """Attention of m rows of each of `batch` sequences over a 4-bit cache: row i of sequence b sees the positions 0 .. pos[b] + i as far as
     their pages exist (none: zeros).  q (rotated) and out fp16 [batch, m, heads * hd]; the other arguments as rope_kv4_write takes them."""
+    native = _compiled if _compiled is not None else _native()
+    if native:
+        return native.attention_kv4(q, pool, table, pos, out, heads, kv_heads, hd, scale, workspace, rows)
     device, batch, max_pages, pages = _kv4_pool_check("attention_kv4", pool, table, pos, rows, kv_heads, hd)
     m = _rows_per_sequence("attention_kv4", "q", q, batch, heads * hd)
     for name, t in (("q", q), ("out", out)):
@@ -273,6 +302,9 @@ def attention_kv4(q, pool, table, pos, out, heads, kv_heads, hd, scale: float, w
 def copy_kv4_pages(pool, src, dst):
     """Page dst[i] of `pool` (uint8 [layers, pages, ..]) becomes a copy of page src[i], in every layer.  src and dst are sequences of whole
     numbers on the host; no page may be written twice, or written and read in the same call."""
+    native = _compiled if _compiled is not None else _native()
+    if native:
+        return native.copy_kv4_pages(pool, src, dst)
     if not isinstance(pool, torch.Tensor) or not pool.is_cuda or pool.dtype != torch.uint8 or pool.dim() < 3 or not pool.is_contiguous():
         raise RuntimeError("copy_kv4_pages: pool must be a contiguous uint8 CUDA tensor [layers, pages, ..]")
     n = len(src)
@@ -294,6 +326,9 @@ def sample_token(logits, u, token, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     """token[r] (int64) = the next token of row r of logits (fp16 or fp32 [rows, vocab]), drawn with the random number u[r] (fp32, in [0, 1)).
     temperature, top_k, top_p and min_p are one number for all rows or a tensor of one per row (float32; top_k int32).  What each filter keeps,
     and in which order they apply, stands in include/sal_decode_ops.h."""
+    native = _compiled if _compiled is not None else _native()
+    if native:
+        return native.sample_token(logits, u, token, temperature, top_k, top_p, min_p)
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dtype not in (torch.float16, torch.float32) or not logits.is_contiguous() \
             or logits.numel() == 0:
         raise RuntimeError("sample_token: logits must be a contiguous float16 or float32 CUDA tensor [rows, vocab]")

@@ -477,3 +477,20 @@ def test_refusals_leave_everything_as_it_was():
         decode_ops.read_kv4(layer, table, pos, torch.empty(2, 1, kvh, hd, device="cuda"), torch.empty(2, 1, kvh, hd, **f16), kvh, hd)
     torch.cuda.synchronize()
     assert torch.equal(pool[1], before[1]) and torch.equal(pool[0, 1:], before[0, 1:])
+
+
+def test_the_same_without_the_compiled_module(monkeypatch):
+    """The Python steps make the same checks and the same calls."""
+    monkeypatch.setattr(decode_ops, "_compiled", False)
+    rng = np.random.default_rng(11)
+    pool, table = filled(rng, 2, 2, 2, 128)
+    check_attention(rng.standard_normal((2, 2, 4 * 128)).astype(np.float16), pool, table, [100, 3], [2, 1], 4, 2, 128)
+    test_rows_are_written_bit_for_bit(128, 4, 2, 1, [0, 63, 64, 200], None, False)
+    test_pages_are_copied_in_every_layer(3, 40, 2, 128, 20)
+    test_refusals_leave_everything_as_it_was()
+    logits, u, token = torch.randn(3, 100, device="cuda"), torch.rand(3, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    decode_ops.sample_token(logits, u, token, 0.7, 20, torch.full((3,), 0.9, device="cuda"), 0.01)
+    monkeypatch.setattr(decode_ops, "_compiled", None)
+    again = torch.zeros_like(token)
+    decode_ops.sample_token(logits, u, again, 0.7, 20, torch.full((3,), 0.9, device="cuda"), 0.01)
+    assert decode_ops._compiled and torch.equal(token, again)

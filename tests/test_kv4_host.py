@@ -100,3 +100,29 @@ def test_tensors_on_the_host_are_refused():
     for hd in (32, 96, 192):
         with pytest.raises(RuntimeError):
             decode_ops.kv4_pool(1, 1, 1, hd, "cpu")
+
+
+def test_a_refusal_with_a_number_in_it_is_an_exception(lib):
+    """Numbers in the compiled module's messages: with a second C++ runtime inside the module they ended the process."""
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from shiftaddllm_b200 import _lib, build, lutgemm
+build.build_extension()
+_lib.load()
+m = lutgemm.compiled_module()
+try:
+    m.lut_linear(torch.zeros(1, 30), torch.zeros(1), torch.zeros(1), None, 32, 32, 3, True)
+except RuntimeError as e:
+    print("refused", "32, got 30" in str(e))
+"""
+    got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=build_dir())
+    assert got.returncode == 0 and "refused True" in got.stdout, got.stdout + got.stderr
+
+
+def build_dir():
+    from shiftaddllm_b200 import build
+
+    return build.REPO_DIR
