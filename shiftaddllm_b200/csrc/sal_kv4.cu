@@ -61,34 +61,6 @@ __device__ __forceinline__ int rows_of(const int32_t *rows, int b, int m) {
     return r < 0 ? 0 : r > m ? m : r;
 }
 
-// One warp stores the HD numbers of a row: lane l holds numbers 64 g + 2 l and 64 g + 2 l + 1 of every group g.
-template <int HD>
-__device__ __forceinline__ void store_row(const __half2 (&x)[HD / GROUP], uint8_t *record, bool value, int p, int lane) {
-    using R = Record<HD>;
-    uint8_t *codes = record + (value ? R::CODES : 0) + p * R::ROW;
-    __half2 *params = reinterpret_cast<__half2 *>(record + 2 * R::CODES + (value ? R::PARAMS : 0)) + p * R::G;
-#pragma unroll
-    for (int g = 0; g < R::G; ++g) {
-        const float2 v = __half22float2(x[g]);
-        float lo = fminf(v.x, v.y), hi = fmaxf(v.x, v.y);
-        const bool odd = !(fabsf(v.x) <= 65504.f && fabsf(v.y) <= 65504.f);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        }
-        const bool bad = __any_sync(0xffffffffu, odd);
-        const __half scale = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
-        const float s = __half2float(scale);
-        const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
-        int a = (int)fminf(rintf(__fmul_rn(__fsub_rn(v.x, lo), inv)), 15.f);
-        int b = (int)fminf(rintf(__fmul_rn(__fsub_rn(v.y, lo), inv)), 15.f);
-        if (bad) a = b = 0;
-        codes[R::place(g, p) * 32 + lane] = (uint8_t)(a | b << 4);
-        if (lane == 0) params[g] = bad ? __half2(__ushort_as_half(0x7fff), __ushort_as_half(0x7fff)) : __half2(scale, __float2half_rn(lo));
-    }
-}
-
 struct CacheArgs {
     uint8_t *pool;
     const int32_t *table;   // [batch][max_pages]
@@ -103,94 +75,123 @@ __device__ __forceinline__ uint8_t *record_of(const CacheArgs &c, int b, int p, 
     return c.pool + ((size_t)page * c.kv_heads + kvh) * Record<HD>::BYTES;
 }
 
-// One warp per head of a row: query heads are turned into q_out, key heads turned and stored, value heads stored.
+// Writing and reading: a thread has eight neighbouring numbers of a head, 16 bytes of 16-bit numbers or 4 bytes of codes, HD / 8 threads a head.  The
+// other numbers of its rotary pairs are HD / 16 threads on, a group is eight threads.  Bound by bytes; what counts are wide accesses and many
+// rows in flight.  Blocks go over the rows with a stride, threads of a block over the heads of a row.
+constexpr int ROW_THREADS = 256;
+
 template <int HD>
-__global__ void __launch_bounds__(256) rope_kv4_write_kernel(const __half *q, const __half *k, const __half *v, const float *cos_t, const float *sin_t,
-                                                             const int64_t *pos, const int32_t *rows, CacheArgs c, __half *q_out, int m, int heads,
-                                                             int max_len) {
-    constexpr int G = HD / GROUP;
+__global__ void __launch_bounds__(ROW_THREADS) rope_kv4_write_kernel(const __half *q, const __half *k, const __half *v, const float *cos_t, const float *sin_t,
+                                                                     const int64_t *pos, const int32_t *rows, CacheArgs c, __half *q_out, int batch_rows, int m,
+                                                                     int heads, int max_len) {
+    using R = Record<HD>;
+    constexpr int T = HD / 8;
     pdl_prologue();
-    const int lane = threadIdx.x & 31;
-    const int unit = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int row = blockIdx.y, b = row / m, i = row % m;
-    if (unit >= heads + 2 * c.kv_heads || i >= rows_of(rows, b, m)) return;
-    const int p = row_position(pos[b], i);
-    if (p < 0 || p >= max_len || p >= c.max_pages * PAGE) return;
-    const bool is_q = unit < heads, is_v = unit >= heads + c.kv_heads;
+    const int unit = blockIdx.y * (ROW_THREADS / T) + threadIdx.x / T, t = threadIdx.x % T, d = 8 * t;
+    const bool is_q = unit < heads, is_v = unit >= heads + c.kv_heads, real = unit < heads + 2 * c.kv_heads;
     const int h = is_q ? unit : is_v ? unit - heads - c.kv_heads : unit - heads;
-    const __half *src = is_q ? q + ((size_t)row * heads + h) * HD : (is_v ? v : k) + ((size_t)row * c.kv_heads + h) * HD;
-    __half2 x[G];
+    const int stride = (is_q ? heads : c.kv_heads) * HD;
+    const __half *src = (is_q ? q : is_v ? v : k) + (size_t)h * HD + d;
+    for (int row = blockIdx.x; row < batch_rows; row += gridDim.x) {
+        const int b = row / m, i = row % m;
+        const int p = row_position(pos[b], i);
+        const bool on = real && i < rows_of(rows, b, m) && p >= 0 && p < max_len && p < c.max_pages * PAGE;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (on) x = *reinterpret_cast<const uint4 *>(src + (size_t)row * stride);
+        uint8_t *record = nullptr;
+        if (on && !is_q) record = record_of<HD>(c, b, p, h);
+        const __half2 *xh = reinterpret_cast<const __half2 *>(&x);
+        uint4 y;
+        y.x = __shfl_xor_sync(0xffffffffu, x.x, T / 2), y.y = __shfl_xor_sync(0xffffffffu, x.y, T / 2);
+        y.z = __shfl_xor_sync(0xffffffffu, x.z, T / 2), y.w = __shfl_xor_sync(0xffffffffu, x.w, T / 2);
+        if (on && !is_v) {
+            const float4 *cs = reinterpret_cast<const float4 *>(cos_t + (size_t)p * (HD / 2) + d % (HD / 2));
+            const float4 *sn = reinterpret_cast<const float4 *>(sin_t + (size_t)p * (HD / 2) + d % (HD / 2));
+            const float4 c0 = cs[0], c1 = cs[1], s0 = sn[0], s1 = sn[1];
+            const float cc[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+            const __half2 *yh = reinterpret_cast<const __half2 *>(&y);
+            const float sign = d < HD / 2 ? 1.f : -1.f;      // b * c + a * s = b * c - a * (-s)
+            uint4 z;
+            __half2 *zh = reinterpret_cast<__half2 *>(&z);
 #pragma unroll
-    for (int g = 0; g < G; ++g) x[g] = *reinterpret_cast<const __half2 *>(src + g * GROUP + 2 * lane);
-    if (!is_v) {
-        const float *cs = cos_t + (size_t)p * (HD / 2), *sn = sin_t + (size_t)p * (HD / 2);
-        if constexpr (G == 1) {   // the other number of a pair lies 32 numbers on: in the other half of the warp
-            const __half2 y = __shfl_xor_sync(0xffffffffu, x[0], 16);
-            const int d = 2 * (lane & 15);
-            const float c0 = cs[d], c1 = cs[d + 1], s0 = sn[d], s1 = sn[d + 1];
-            const float2 u = __half22float2(x[0]), w = __half22float2(y);
-            const float sign = lane < 16 ? 1.f : -1.f;      // b * c + a * s = b * c - a * (-s)
-            x[0] = __half2(turned(u.x, c0, w.x, sign * s0), turned(u.y, c1, w.y, sign * s1));
-        } else {
-#pragma unroll
-            for (int g = 0; g < G / 2; ++g) {
-                const int d = g * GROUP + 2 * lane;
-                const float2 cc = *reinterpret_cast<const float2 *>(cs + d), ss = *reinterpret_cast<const float2 *>(sn + d);
-                const float2 u = __half22float2(x[g]), w = __half22float2(x[g + G / 2]);
-                x[g] = __half2(turned(u.x, cc.x, w.x, ss.x), turned(u.y, cc.y, w.y, ss.y));
-                x[g + G / 2] = __half2(turned(w.x, cc.x, u.x, -ss.x), turned(w.y, cc.y, u.y, -ss.y));
+            for (int e = 0; e < 4; ++e) {
+                const float2 u = __half22float2(xh[e]), w = __half22float2(yh[e]);
+                zh[e] = __half2(turned(u.x, cc[2 * e], w.x, sign * ss[2 * e]), turned(u.y, cc[2 * e + 1], w.y, sign * ss[2 * e + 1]));
             }
+            x = z;
+        }
+        if (on && is_q) *reinterpret_cast<uint4 *>(q_out + (size_t)row * stride + (size_t)h * HD + d) = x;
+        if (!__any_sync(0xffffffffu, record != nullptr)) continue;
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 u = __half22float2(xh[e]);
+            f[2 * e] = u.x, f[2 * e + 1] = u.y;
+        }
+        float lo = f[0], hi = f[0];
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) lo = fminf(lo, f[e]), hi = fmaxf(hi, f[e]), odd |= !(fabsf(f[e]) <= 65504.f);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        const bool bad = __ballot_sync(0xffffffffu, odd) >> (threadIdx.x & 24) & 0xffu;
+        const __half scale = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
+        const float s = __half2float(scale);
+        const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+        uint32_t codes = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) codes |= (uint32_t)fminf(rintf(__fmul_rn(__fsub_rn(f[e], lo), inv)), 15.f) << (4 * e);
+        if (record) {
+            const int at = p % PAGE, g = t / 8;
+            *reinterpret_cast<uint32_t *>(record + (is_v ? R::CODES : 0) + at * R::ROW + R::place(g, at) * 32 + 4 * (t % 8)) = bad ? 0u : codes;
+            if (t % 8 == 0)
+                reinterpret_cast<__half2 *>(record + 2 * R::CODES + (is_v ? R::PARAMS : 0))[at * R::G + g] =
+                    bad ? __half2(__ushort_as_half(0x7fff), __ushort_as_half(0x7fff)) : __half2(scale, __float2half_rn(lo));
         }
     }
-    if (is_q) {
-        __half *dst = q_out + ((size_t)row * heads + h) * HD;
-#pragma unroll
-        for (int g = 0; g < G; ++g) *reinterpret_cast<__half2 *>(dst + g * GROUP + 2 * lane) = x[g];
-        return;
-    }
-    uint8_t *record = record_of<HD>(c, b, p, h);
-    if (record) store_row<HD>(x, record, is_v, p % PAGE, lane);
-}
-
-template <typename T>
-__device__ __forceinline__ void store_pair(T *dst, float a, float b);
-template <>
-__device__ __forceinline__ void store_pair<float>(float *dst, float a, float b) { *reinterpret_cast<float2 *>(dst) = make_float2(a, b); }
-template <>
-__device__ __forceinline__ void store_pair<__half>(__half *dst, float a, float b) { *reinterpret_cast<__half2 *>(dst) = __floats2half2_rn(a, b); }
-
-// The two numbers that lane l holds of group g of a row.
-template <int HD>
-__device__ __forceinline__ float2 row_pair(const uint8_t *record, bool value, int p, int g, int lane) {
-    using R = Record<HD>;
-    const uint8_t byte = record[(value ? R::CODES : 0) + p * R::ROW + R::place(g, p) * 32 + lane];
-    const float2 sl = __half22float2(reinterpret_cast<const __half2 *>(record + 2 * R::CODES + (value ? R::PARAMS : 0))[p * R::G + g]);
-    return make_float2(fmaf(sl.x, (float)(byte & 15), sl.y), fmaf(sl.x, (float)(byte >> 4), sl.y));
 }
 
 template <int HD, typename T>
-__global__ void __launch_bounds__(256) read_kv4_kernel(CacheArgs c, const int64_t *pos, T *k_out, T *v_out, int m) {
+__global__ void __launch_bounds__(ROW_THREADS) read_kv4_kernel(CacheArgs c, const int64_t *pos, T *k_out, T *v_out, int batch_rows, int m) {
+    using R = Record<HD>;
+    constexpr int N = HD / 8;
     pdl_prologue();
-    const int lane = threadIdx.x & 31;
-    const int unit = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int row = blockIdx.y, b = row / m, i = row % m;
+    const int unit = blockIdx.y * (ROW_THREADS / N) + threadIdx.x / N, t = threadIdx.x % N;
     if (unit >= 2 * c.kv_heads) return;
     const bool is_v = unit >= c.kv_heads;
-    const int h = is_v ? unit - c.kv_heads : unit;
-    const int p = row_position(pos[b], i);
-    const uint8_t *record = record_of<HD>(c, b, p, h);
-    T *dst = (is_v ? v_out : k_out) + ((size_t)row * c.kv_heads + h) * HD;
+    const int h = is_v ? unit - c.kv_heads : unit, g = t / 8;
+    T *dst = (is_v ? v_out : k_out) + (size_t)h * HD + 8 * t;
+    for (int row = blockIdx.x; row < batch_rows; row += gridDim.x) {
+        const int b = row / m, p = row_position(pos[b], row % m), at = p & (PAGE - 1);
+        const uint8_t *record = record_of<HD>(c, b, p, h);
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (record) {
+            const uint32_t codes = *reinterpret_cast<const uint32_t *>(record + (is_v ? R::CODES : 0) + at * R::ROW + R::place(g, at) * 32 + 4 * (t % 8));
+            const float2 sl = __half22float2(reinterpret_cast<const __half2 *>(record + 2 * R::CODES + (is_v ? R::PARAMS : 0))[at * R::G + g]);
 #pragma unroll
-    for (int g = 0; g < HD / GROUP; ++g) {
-        const float2 v = record ? row_pair<HD>(record, is_v, p % PAGE, g, lane) : make_float2(0.f, 0.f);
-        store_pair(dst + g * GROUP + 2 * lane, v.x, v.y);
+            for (int e = 0; e < 8; ++e) f[e] = fmaf(sl.x, (float)(codes >> (4 * e) & 15u), sl.y);
+        }
+        T *to = dst + (size_t)row * c.kv_heads * HD;
+        if constexpr (sizeof(T) == 4) {
+            reinterpret_cast<float4 *>(to)[0] = make_float4(f[0], f[1], f[2], f[3]);
+            reinterpret_cast<float4 *>(to)[1] = make_float4(f[4], f[5], f[6], f[7]);
+        } else {
+            uint4 o;
+            __half2 *oh = reinterpret_cast<__half2 *>(&o);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) oh[e] = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
+            *reinterpret_cast<uint4 *>(to) = o;
+        }
     }
 }
 
 // ---- attention on the tensor cores -----------------------------------------------------------------------------------------------
 //
 // A score is scale * sum_g (s_g * D_g + low_g * Q_g) with D_g = sum over the group of q * code and Q_g = sum of q; an output is
-// E_g * A_g + sum_t p_t * low_t with A_g = sum over positions of (p * s_g / E_g) * code.  The codes are 16-bit floats without any error, so D_g and A_g are matrix products of 16-bit operands (m16n8k16, 32-bit sums) in which only the
+// E_g * A_g + sum_t p_t * (low_t + 8 s_t) with A_g = sum over positions of (p * s_g / E_g) * (code - 8).  The codes are 16-bit floats without any error, so D_g and A_g are matrix products of 16-bit operands (m16n8k16, 32-bit sums) in which only the
 // weight p * s is rounded; it goes in as the sum of two 16-bit numbers.  E_g, a power of two not below any scale so far, keeps the weights in
 // their range.  Neither keys nor values are ever formed.
 //
@@ -269,6 +270,19 @@ __device__ __forceinline__ uint32_t codes_low(uint32_t x) {
     return h;
 }
 constexpr float UNIT = 1048576.f;
+// The same less 8.  Sums over the positions of a long text are made of these: an output is the mean of many values and small beside each, so the
+// sums should be no larger than it either (with codes from 0 on, 100 thousand positions lost two digits to the tensor core's rounding).
+__device__ __forceinline__ uint32_t codes_mid_8(uint32_t x) {
+    uint32_t h = x & 0x00f000f0u;
+    asm("add.rn.f16x2 %0, %0, %1;" : "+r"(h) : "r"(0x80808080u));      // - 2**-17
+    return h;
+}
+__device__ __forceinline__ uint32_t codes_low_8(uint32_t x) {
+    uint32_t h;
+    asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(h) : "r"(x));
+    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(h) : "r"(0x00100010u), "r"(0x94089408u));   // * 2**-20 - 2**-10 - 2**-17
+    return h;
+}
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -757,7 +771,8 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
                     for (int f = 0; f < 2; ++f) {
 #pragma unroll
                         for (int g = 0; g < G; ++g) {
-                            const float2 f0 = as_float2(v0[f][g]), f1 = as_float2(v1[f][g]);
+                            float2 f0 = as_float2(v0[f][g]), f1 = as_float2(v1[f][g]);
+                            f0.y = fmaf(8.f, f0.x, f0.y), f1.y = fmaf(8.f, f1.x, f1.y);
                             const float u0 = f0.x * to_one[g], u1 = f1.x * to_one[g];
                             uint32_t b[NT][2], b2[NT][2];
 #pragma unroll
@@ -795,7 +810,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
 #pragma unroll
                                 for (int t = 0; t < 2; ++t) {
                                     const uint32_t xa = za >> (8 * t), xb = zb >> (8 * t);
-                                    const uint32_t a0 = codes_low(xa), a1 = codes_mid(xa), a2 = codes_low(xb), a3 = codes_mid(xb);
+                                    const uint32_t a0 = codes_low_8(xa), a1 = codes_mid_8(xa), a2 = codes_low_8(xb), a3 = codes_mid_8(xb);
 #pragma unroll
                                     for (int nt = 0; nt < NT; ++nt) {
                                         mma16816(acc[nt][4 * g + 2 * k + t], a0, a1, a2, a3, b[nt][0], b[nt][1]);
@@ -998,6 +1013,12 @@ bool aligned16(const void *a, const void *b = nullptr, const void *c = nullptr, 
     return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c) | reinterpret_cast<uintptr_t>(d) |
              reinterpret_cast<uintptr_t>(e)) & 15) == 0;
 }
+// Blocks of the row kernels: all heads of a row side by side, as many rows as fill the GPU about twice.
+dim3 row_grid(int rows, int heads, int hd) {
+    const int across = (heads * (hd / 8) + ROW_THREADS - 1) / ROW_THREADS;
+    const int most = 148 * 12 / across > 1 ? 148 * 12 / across : 1;
+    return dim3((unsigned)(rows < most ? rows : most), (unsigned)across);
+}
 int check_cache(int batch, int m, int kv_heads, int hd, int max_pages, int pages) {
     if (hd != 64 && hd != 128 && hd != 256) return SAL_E_UNSUPPORTED;
     if (batch < 1 || m < 1 || kv_heads < 1 || kv_heads > 256 || max_pages < 1 || max_pages > MAX_PAGES || pages < 1) return SAL_E_SHAPE;
@@ -1074,11 +1095,11 @@ int sal_rope_kv4_write_f16(const void *q, const void *k, const void *v, const vo
     if (heads < 1 || heads > 16384 || max_len < 1) return SAL_E_SHAPE;
     if (!aligned16(q, k, v, q_out, pool) || !aligned16(cos, sin)) return SAL_E_ALIGN;
     const CacheArgs c = {reinterpret_cast<uint8_t *>(pool), table, kv_heads, max_pages, pages};
-    const dim3 grid((heads + 2 * kv_heads + 7) / 8, batch * m);
+    const dim3 grid = row_grid(batch * m, heads + 2 * kv_heads, hd);
     auto kernel = hd == 64 ? rope_kv4_write_kernel<64> : hd == 128 ? rope_kv4_write_kernel<128> : rope_kv4_write_kernel<256>;
-    return sal_launch_pdl(kernel, grid, dim3(256), 0, stream, reinterpret_cast<const __half *>(q), reinterpret_cast<const __half *>(k),
+    return sal_launch_pdl(kernel, grid, dim3(ROW_THREADS), 0, stream, reinterpret_cast<const __half *>(q), reinterpret_cast<const __half *>(k),
                           reinterpret_cast<const __half *>(v), reinterpret_cast<const float *>(cos), reinterpret_cast<const float *>(sin), pos, rows, c,
-                          reinterpret_cast<__half *>(q_out), m, heads, max_len);
+                          reinterpret_cast<__half *>(q_out), batch * m, m, heads, max_len);
 }
 
 int sal_read_kv4(const void *pool, const int32_t *table, const int64_t *pos, void *k_out, void *v_out, int out_f32, int batch, int m, int kv_heads,
@@ -1088,13 +1109,13 @@ int sal_read_kv4(const void *pool, const int32_t *table, const int64_t *pos, voi
     if (rc != SAL_OK) return rc;
     if (!aligned16(pool, k_out, v_out)) return SAL_E_ALIGN;
     const CacheArgs c = {reinterpret_cast<uint8_t *>(const_cast<void *>(pool)), table, kv_heads, max_pages, pages};
-    const dim3 grid((2 * kv_heads + 7) / 8, batch * m);
+    const dim3 grid = row_grid(batch * m, 2 * kv_heads, hd);
     if (out_f32) {
         auto kernel = hd == 64 ? read_kv4_kernel<64, float> : hd == 128 ? read_kv4_kernel<128, float> : read_kv4_kernel<256, float>;
-        return sal_launch_pdl(kernel, grid, dim3(256), 0, stream, c, pos, reinterpret_cast<float *>(k_out), reinterpret_cast<float *>(v_out), m);
+        return sal_launch_pdl(kernel, grid, dim3(ROW_THREADS), 0, stream, c, pos, reinterpret_cast<float *>(k_out), reinterpret_cast<float *>(v_out), batch * m, m);
     }
     auto kernel = hd == 64 ? read_kv4_kernel<64, __half> : hd == 128 ? read_kv4_kernel<128, __half> : read_kv4_kernel<256, __half>;
-    return sal_launch_pdl(kernel, grid, dim3(256), 0, stream, c, pos, reinterpret_cast<__half *>(k_out), reinterpret_cast<__half *>(v_out), m);
+    return sal_launch_pdl(kernel, grid, dim3(ROW_THREADS), 0, stream, c, pos, reinterpret_cast<__half *>(k_out), reinterpret_cast<__half *>(v_out), batch * m, m);
 }
 
 size_t sal_attention_kv4_workspace_bytes(int batch, int m, int heads, int kv_heads, int hd) {
