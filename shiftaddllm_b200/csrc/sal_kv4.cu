@@ -41,13 +41,22 @@ struct Record {
 
 // a * c - b * s to the nearest 32-bit number of the exact sum (products split into value and error), then to 16 bits: the same
 // bits as 64-bit arithmetic gives, at a fraction of its price.
-__device__ __forceinline__ __half turned(float a, float c, float b, float s) {
+__device__ __noinline__ __half turned_exactly(float a, float c, float b, float s) {
     const float p = __fmul_rn(a, c), pe = __fmaf_rn(a, c, -p);
     const float q = __fmul_rn(b, s), qe = __fmaf_rn(b, s, -q);
     const float d = __fsub_rn(p, q), bb = __fsub_rn(d, p);
     const float de = __fsub_rn(__fsub_rn(p, __fsub_rn(d, bb)), __fadd_rn(q, bb));
     const float r = __fadd_rn(d, __fadd_rn(de, __fsub_rn(pe, qe)));
     return __float2half_rn(isfinite(r) ? r : d);   // an infinite product has no error term
+}
+// The sum with the second product's error taken off is within two units of the exact one in its last place.  That decides the 16-bit number unless
+// it lies so near to the middle between two of them (`unsure`), is subnormal there, or overflows: one number in a thousand.
+__device__ __forceinline__ float nearly_turned(float a, float c, float b, float s, bool &unsure) {
+    const float q = __fmul_rn(b, s);
+    const float r = __fsub_rn(__fmaf_rn(a, c, -q), __fmaf_rn(b, s, -q));
+    const uint32_t u = __float_as_uint(r) & 0x7fffffffu;
+    unsure = (u & 0x1fffu) - 0x0ffcu <= 8u || u - 0x38800000u >= 0x47700000u - 0x38800000u;
+    return r;
 }
 
 // The position of row i of a sequence, clamped so that the sum cannot overflow; the caller compares it with the positions that exist.
@@ -77,13 +86,13 @@ __device__ __forceinline__ uint8_t *record_of(const CacheArgs &c, int b, int p, 
 
 // Writing and reading: a thread has eight neighbouring numbers of a head, 16 bytes of 16-bit numbers or 4 bytes of codes, HD / 8 threads a head.  The
 // other numbers of its rotary pairs are HD / 16 threads on, a group is eight threads.  Bound by bytes; what counts are wide accesses and many
-// rows in flight.  Blocks go over the rows with a stride, threads of a block over the heads of a row.
+// rows in flight.  Blocks go over a sequence's rows with a stride, threads of a block over the heads of a row.
 constexpr int ROW_THREADS = 256;
 
 template <int HD>
-__global__ void __launch_bounds__(ROW_THREADS) rope_kv4_write_kernel(const __half *q, const __half *k, const __half *v, const float *cos_t, const float *sin_t,
-                                                                     const int64_t *pos, const int32_t *rows, CacheArgs c, __half *q_out, int batch_rows, int m,
-                                                                     int heads, int max_len) {
+__global__ void __launch_bounds__(ROW_THREADS, 4) rope_kv4_write_kernel(const __half *q, const __half *k, const __half *v, const float *cos_t, const float *sin_t,
+                                                                     const int64_t *pos, const int32_t *rows, CacheArgs c, __half *q_out, int m, int heads,
+                                                                     int max_len) {
     using R = Record<HD>;
     constexpr int T = HD / 8;
     pdl_prologue();
@@ -92,35 +101,60 @@ __global__ void __launch_bounds__(ROW_THREADS) rope_kv4_write_kernel(const __hal
     const int h = is_q ? unit : is_v ? unit - heads - c.kv_heads : unit - heads;
     const int stride = (is_q ? heads : c.kv_heads) * HD;
     const __half *src = (is_q ? q : is_v ? v : k) + (size_t)h * HD + d;
-    for (int row = blockIdx.x; row < batch_rows; row += gridDim.x) {
-        const int b = row / m, i = row % m;
-        const int p = row_position(pos[b], i);
-        const bool on = real && i < rows_of(rows, b, m) && p >= 0 && p < max_len && p < c.max_pages * PAGE;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (on) x = *reinterpret_cast<const uint4 *>(src + (size_t)row * stride);
+    const bool any_turned = __any_sync(0xffffffffu, !is_v);      // of the warp
+    // this sequence's rows that are there and have a position: first .. last - 1 of its m
+    const int b = blockIdx.z, start = row_position(pos[b], 0);
+    const int last = real ? min(rows_of(rows, b, m), min(max_len, c.max_pages * PAGE) - start) : 0;      // start may be negative, or far behind
+    const size_t base = (size_t)b * m;
+    // the next row's numbers are asked for in front of this row's work
+    uint4 next = make_uint4(0, 0, 0, 0);
+    auto there = [&](int i) { return i < last && start + i >= 0; };
+    auto ask = [&](int i) {
+        if (there(i)) next = *reinterpret_cast<const uint4 *>(src + (base + i) * stride);
+    };
+    ask(blockIdx.x);
+    for (int i = blockIdx.x; i < m; i += gridDim.x) {
+        const bool on = there(i);
+        const int p = start + i;
+        const size_t row = base + i;
+        uint4 x = next;
+        ask(i + gridDim.x);
         uint8_t *record = nullptr;
         if (on && !is_q) record = record_of<HD>(c, b, p, h);
-        const __half2 *xh = reinterpret_cast<const __half2 *>(&x);
-        uint4 y;
-        y.x = __shfl_xor_sync(0xffffffffu, x.x, T / 2), y.y = __shfl_xor_sync(0xffffffffu, x.y, T / 2);
-        y.z = __shfl_xor_sync(0xffffffffu, x.z, T / 2), y.w = __shfl_xor_sync(0xffffffffu, x.w, T / 2);
-        if (on && !is_v) {
-            const float4 *cs = reinterpret_cast<const float4 *>(cos_t + (size_t)p * (HD / 2) + d % (HD / 2));
-            const float4 *sn = reinterpret_cast<const float4 *>(sin_t + (size_t)p * (HD / 2) + d % (HD / 2));
-            const float4 c0 = cs[0], c1 = cs[1], s0 = sn[0], s1 = sn[1];
-            const float cc[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-            const __half2 *yh = reinterpret_cast<const __half2 *>(&y);
-            const float sign = d < HD / 2 ? 1.f : -1.f;      // b * c + a * s = b * c - a * (-s)
-            uint4 z;
-            __half2 *zh = reinterpret_cast<__half2 *>(&z);
+        __half2 *xh = reinterpret_cast<__half2 *>(&x);
+        if (any_turned) {
+            const uint32_t flip = d < HD / 2 ? 0u : 0x80008000u;      // b * c + a * s = b * c - (-a) * s
+            uint4 y;
+            y.x = __shfl_xor_sync(0xffffffffu, x.x, T / 2) ^ flip, y.y = __shfl_xor_sync(0xffffffffu, x.y, T / 2) ^ flip;
+            y.z = __shfl_xor_sync(0xffffffffu, x.z, T / 2) ^ flip, y.w = __shfl_xor_sync(0xffffffffu, x.w, T / 2) ^ flip;
+            if (on && !is_v) {
+                const float4 *cs = reinterpret_cast<const float4 *>(cos_t + (size_t)p * (HD / 2) + d % (HD / 2));
+                const float4 *sn = reinterpret_cast<const float4 *>(sin_t + (size_t)p * (HD / 2) + d % (HD / 2));
+                const float4 c0 = cs[0], c1 = cs[1], s0 = sn[0], s1 = sn[1];
+                const float cc[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+                const __half2 *yh = reinterpret_cast<const __half2 *>(&y);
+                uint4 z;
+                __half2 *zh = reinterpret_cast<__half2 *>(&z);
+                unsigned unsure = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 u = __half22float2(xh[e]), w = __half22float2(yh[e]);
-                zh[e] = __half2(turned(u.x, cc[2 * e], w.x, sign * ss[2 * e]), turned(u.y, cc[2 * e + 1], w.y, sign * ss[2 * e + 1]));
+                for (int e = 0; e < 4; ++e) {
+                    const float2 u = __half22float2(xh[e]), w = __half22float2(yh[e]);
+                    bool f0, f1;
+                    zh[e] = __floats2half2_rn(nearly_turned(u.x, cc[2 * e], w.x, ss[2 * e], f0), nearly_turned(u.y, cc[2 * e + 1], w.y, ss[2 * e + 1], f1));
+                    unsure |= (f0 ? 1u << (2 * e) : 0u) | (f1 ? 2u << (2 * e) : 0u);
+                }
+                if (unsure) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 u = __half22float2(xh[e]), w = __half22float2(yh[e]);
+                        if (unsure >> (2 * e) & 1u) zh[e] = __half2(turned_exactly(u.x, cc[2 * e], w.x, ss[2 * e]), zh[e].y);
+                        if (unsure >> (2 * e) & 2u) zh[e] = __half2(zh[e].x, turned_exactly(u.y, cc[2 * e + 1], w.y, ss[2 * e + 1]));
+                    }
+                }
+                x = z;
             }
-            x = z;
         }
-        if (on && is_q) *reinterpret_cast<uint4 *>(q_out + (size_t)row * stride + (size_t)h * HD + d) = x;
+        if (on && is_q) *reinterpret_cast<uint4 *>(q_out + row * stride + (size_t)h * HD + d) = x;
         if (!__any_sync(0xffffffffu, record != nullptr)) continue;
         float f[8];
 #pragma unroll
@@ -155,7 +189,7 @@ __global__ void __launch_bounds__(ROW_THREADS) rope_kv4_write_kernel(const __hal
 }
 
 template <int HD, typename T>
-__global__ void __launch_bounds__(ROW_THREADS) read_kv4_kernel(CacheArgs c, const int64_t *pos, T *k_out, T *v_out, int batch_rows, int m) {
+__global__ void __launch_bounds__(ROW_THREADS) read_kv4_kernel(CacheArgs c, const int64_t *pos, T *k_out, T *v_out, int m) {
     using R = Record<HD>;
     constexpr int N = HD / 8;
     pdl_prologue();
@@ -164,8 +198,9 @@ __global__ void __launch_bounds__(ROW_THREADS) read_kv4_kernel(CacheArgs c, cons
     const bool is_v = unit >= c.kv_heads;
     const int h = is_v ? unit - c.kv_heads : unit, g = t / 8;
     T *dst = (is_v ? v_out : k_out) + (size_t)h * HD + 8 * t;
-    for (int row = blockIdx.x; row < batch_rows; row += gridDim.x) {
-        const int b = row / m, p = row_position(pos[b], row % m), at = p & (PAGE - 1);
+    const int b = blockIdx.z, start = row_position(pos[b], 0);
+    for (int i = blockIdx.x; i < m; i += gridDim.x) {
+        const int p = start + i, at = p & (PAGE - 1);
         const uint8_t *record = record_of<HD>(c, b, p, h);
         float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (record) {
@@ -174,7 +209,7 @@ __global__ void __launch_bounds__(ROW_THREADS) read_kv4_kernel(CacheArgs c, cons
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = fmaf(sl.x, (float)(codes >> (4 * e) & 15u), sl.y);
         }
-        T *to = dst + (size_t)row * c.kv_heads * HD;
+        T *to = dst + ((size_t)b * m + i) * c.kv_heads * HD;
         if constexpr (sizeof(T) == 4) {
             reinterpret_cast<float4 *>(to)[0] = make_float4(f[0], f[1], f[2], f[3]);
             reinterpret_cast<float4 *>(to)[1] = make_float4(f[4], f[5], f[6], f[7]);
@@ -1013,11 +1048,10 @@ bool aligned16(const void *a, const void *b = nullptr, const void *c = nullptr, 
     return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c) | reinterpret_cast<uintptr_t>(d) |
              reinterpret_cast<uintptr_t>(e)) & 15) == 0;
 }
-// Blocks of the row kernels: all heads of a row side by side, as many rows as fill the GPU about twice.
-dim3 row_grid(int rows, int heads, int hd) {
-    const int across = (heads * (hd / 8) + ROW_THREADS - 1) / ROW_THREADS;
-    const int most = 148 * 12 / across > 1 ? 148 * 12 / across : 1;
-    return dim3((unsigned)(rows < most ? rows : most), (unsigned)across);
+// Blocks of the row kernels: all heads of a row side by side (y), sequences (z), and as many rows of each as fill the GPU about once.
+dim3 row_grid(int batch, int m, int heads, int hd) {
+    const long long across = ((long long)heads * (hd / 8) + ROW_THREADS - 1) / ROW_THREADS, most = 148 * 6 / (across * batch);
+    return dim3((unsigned)(m < most ? m : most > 1 ? most : 1), (unsigned)across, (unsigned)batch);
 }
 int check_cache(int batch, int m, int kv_heads, int hd, int max_pages, int pages) {
     if (hd != 64 && hd != 128 && hd != 256) return SAL_E_UNSUPPORTED;
@@ -1095,11 +1129,11 @@ int sal_rope_kv4_write_f16(const void *q, const void *k, const void *v, const vo
     if (heads < 1 || heads > 16384 || max_len < 1) return SAL_E_SHAPE;
     if (!aligned16(q, k, v, q_out, pool) || !aligned16(cos, sin)) return SAL_E_ALIGN;
     const CacheArgs c = {reinterpret_cast<uint8_t *>(pool), table, kv_heads, max_pages, pages};
-    const dim3 grid = row_grid(batch * m, heads + 2 * kv_heads, hd);
+    const dim3 grid = row_grid(batch, m, heads + 2 * kv_heads, hd);
     auto kernel = hd == 64 ? rope_kv4_write_kernel<64> : hd == 128 ? rope_kv4_write_kernel<128> : rope_kv4_write_kernel<256>;
     return sal_launch_pdl(kernel, grid, dim3(ROW_THREADS), 0, stream, reinterpret_cast<const __half *>(q), reinterpret_cast<const __half *>(k),
                           reinterpret_cast<const __half *>(v), reinterpret_cast<const float *>(cos), reinterpret_cast<const float *>(sin), pos, rows, c,
-                          reinterpret_cast<__half *>(q_out), batch * m, m, heads, max_len);
+                          reinterpret_cast<__half *>(q_out), m, heads, max_len);
 }
 
 int sal_read_kv4(const void *pool, const int32_t *table, const int64_t *pos, void *k_out, void *v_out, int out_f32, int batch, int m, int kv_heads,
@@ -1109,13 +1143,13 @@ int sal_read_kv4(const void *pool, const int32_t *table, const int64_t *pos, voi
     if (rc != SAL_OK) return rc;
     if (!aligned16(pool, k_out, v_out)) return SAL_E_ALIGN;
     const CacheArgs c = {reinterpret_cast<uint8_t *>(const_cast<void *>(pool)), table, kv_heads, max_pages, pages};
-    const dim3 grid = row_grid(batch * m, 2 * kv_heads, hd);
+    const dim3 grid = row_grid(batch, m, 2 * kv_heads, hd);
     if (out_f32) {
         auto kernel = hd == 64 ? read_kv4_kernel<64, float> : hd == 128 ? read_kv4_kernel<128, float> : read_kv4_kernel<256, float>;
-        return sal_launch_pdl(kernel, grid, dim3(ROW_THREADS), 0, stream, c, pos, reinterpret_cast<float *>(k_out), reinterpret_cast<float *>(v_out), batch * m, m);
+        return sal_launch_pdl(kernel, grid, dim3(ROW_THREADS), 0, stream, c, pos, reinterpret_cast<float *>(k_out), reinterpret_cast<float *>(v_out), m);
     }
     auto kernel = hd == 64 ? read_kv4_kernel<64, __half> : hd == 128 ? read_kv4_kernel<128, __half> : read_kv4_kernel<256, __half>;
-    return sal_launch_pdl(kernel, grid, dim3(ROW_THREADS), 0, stream, c, pos, reinterpret_cast<__half *>(k_out), reinterpret_cast<__half *>(v_out), batch * m, m);
+    return sal_launch_pdl(kernel, grid, dim3(ROW_THREADS), 0, stream, c, pos, reinterpret_cast<__half *>(k_out), reinterpret_cast<__half *>(v_out), m);
 }
 
 size_t sal_attention_kv4_workspace_bytes(int batch, int m, int heads, int kv_heads, int hd) {
