@@ -54,8 +54,8 @@ __device__ __noinline__ __half turned_exactly(float a, float c, float b, float s
 __device__ __forceinline__ float nearly_turned(float a, float c, float b, float s, bool &unsure) {
     const float q = __fmul_rn(b, s);
     const float r = __fsub_rn(__fmaf_rn(a, c, -q), __fmaf_rn(b, s, -q));
-    const uint32_t u = __float_as_uint(r) & 0x7fffffffu;
-    unsure = (u & 0x1fffu) - 0x0ffcu <= 8u || u - 0x38800000u >= 0x47700000u - 0x38800000u;
+    const uint32_t u = __float_as_uint(r);
+    unsure = (u - 0x0ffcu & 0x1fffu) <= 8u || (u & 0x7fffffffu) - 0x38800000u >= 0x47700000u - 0x38800000u;
     return r;
 }
 
@@ -1048,9 +1048,9 @@ bool aligned16(const void *a, const void *b = nullptr, const void *c = nullptr, 
     return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c) | reinterpret_cast<uintptr_t>(d) |
              reinterpret_cast<uintptr_t>(e)) & 15) == 0;
 }
-// Blocks of the row kernels: all heads of a row side by side (y), sequences (z), and as many rows of each as fill the GPU about once.
-dim3 row_grid(int batch, int m, int heads, int hd) {
-    const long long across = ((long long)heads * (hd / 8) + ROW_THREADS - 1) / ROW_THREADS, most = 148 * 6 / (across * batch);
+// Blocks of the row kernels: all heads of a row side by side (y), sequences (z), and as many rows of each as fill the GPU once.
+dim3 row_grid(int batch, int m, int heads, int hd, int per_sm) {
+    const long long across = ((long long)heads * (hd / 8) + ROW_THREADS - 1) / ROW_THREADS, most = 148LL * per_sm / (across * batch);
     return dim3((unsigned)(m < most ? m : most > 1 ? most : 1), (unsigned)across, (unsigned)batch);
 }
 int check_cache(int batch, int m, int kv_heads, int hd, int max_pages, int pages) {
@@ -1129,7 +1129,7 @@ int sal_rope_kv4_write_f16(const void *q, const void *k, const void *v, const vo
     if (heads < 1 || heads > 16384 || max_len < 1) return SAL_E_SHAPE;
     if (!aligned16(q, k, v, q_out, pool) || !aligned16(cos, sin)) return SAL_E_ALIGN;
     const CacheArgs c = {reinterpret_cast<uint8_t *>(pool), table, kv_heads, max_pages, pages};
-    const dim3 grid = row_grid(batch, m, heads + 2 * kv_heads, hd);
+    const dim3 grid = row_grid(batch, m, heads + 2 * kv_heads, hd, 4);
     auto kernel = hd == 64 ? rope_kv4_write_kernel<64> : hd == 128 ? rope_kv4_write_kernel<128> : rope_kv4_write_kernel<256>;
     return sal_launch_pdl(kernel, grid, dim3(ROW_THREADS), 0, stream, reinterpret_cast<const __half *>(q), reinterpret_cast<const __half *>(k),
                           reinterpret_cast<const __half *>(v), reinterpret_cast<const float *>(cos), reinterpret_cast<const float *>(sin), pos, rows, c,
@@ -1143,7 +1143,7 @@ int sal_read_kv4(const void *pool, const int32_t *table, const int64_t *pos, voi
     if (rc != SAL_OK) return rc;
     if (!aligned16(pool, k_out, v_out)) return SAL_E_ALIGN;
     const CacheArgs c = {reinterpret_cast<uint8_t *>(const_cast<void *>(pool)), table, kv_heads, max_pages, pages};
-    const dim3 grid = row_grid(batch, m, 2 * kv_heads, hd);
+    const dim3 grid = row_grid(batch, m, 2 * kv_heads, hd, 8);
     if (out_f32) {
         auto kernel = hd == 64 ? read_kv4_kernel<64, float> : hd == 128 ? read_kv4_kernel<128, float> : read_kv4_kernel<256, float>;
         return sal_launch_pdl(kernel, grid, dim3(ROW_THREADS), 0, stream, c, pos, reinterpret_cast<float *>(k_out), reinterpret_cast<float *>(v_out), m);
