@@ -29,6 +29,7 @@ import torch
 import torch.nn.functional as F
 
 from . import decode_ops, lutgemm
+from .kv4 import Kv4Cache
 from .quant import LutLinear
 
 
@@ -377,35 +378,72 @@ class BcqLlamaBatchDecoder:
     per group (M = batch: the weights are streamed once for all sequences); the steps between them are the
     M-row forms of the fused helpers (residual + RMSNorm per row, rotary step + cache write + split attention
     per sequence in one launch) or, with `fused=False`, plain torch ops.  Weights are those of a
-    `BcqLlamaDecoder` (pass it as `like` to share them instead of drawing new ones)."""
+    `BcqLlamaDecoder` (pass it as `like` to share them instead of drawing new ones).
+
+    `cache_bits=4` keeps keys and values in 4 bits, in pages that the sequences share (`self.cache`, a :class:`kv4.Kv4Cache` of `pages` pages; None:
+    enough for all).  Each sequence then has a position of its own: `prefill` takes prompts of different lengths, `fork` makes one sequence
+    the copy of another.  With `set_sampling` the next tokens are drawn from the logits instead of taken greedily (either cache)."""
 
     def __init__(self, shape: LlamaShape, wbits: int = 3, group_size: int = 128, max_len: int = 640, batch: int = 16,
-                 device="cuda", seed: int = 0, like: "BcqLlamaDecoder | None" = None, fused: bool = True):
+                 device="cuda", seed: int = 0, like: "BcqLlamaDecoder | None" = None, fused: bool = True, cache_bits: int = 16,
+                 pages: int | None = None):
         if not 1 <= batch <= 64:
             raise ValueError("batch must be 1..64 (rows of one small-batch LUT product)")
+        if cache_bits not in (4, 16) or (cache_bits == 4 and not fused):
+            raise ValueError("cache_bits must be 16, or 4 with the fused helpers")
         self.shape, self.max_len, self.batch = shape, max_len, batch
         self.device = torch.device(device)
         if like is None:
             like = BcqLlamaDecoder(shape, wbits, group_size, max_len=8, device=device, seed=seed, fused=False)
         self.embed, self.lm_head, self.final_norm, self.blocks = like.embed, like.lm_head, like.final_norm, like.blocks
         hd, kvh, h, b = shape.head_dim, shape.kv_heads, shape.hidden, batch
-        self.k_cache = torch.zeros(shape.layers, b, max_len, kvh, hd, dtype=torch.float16, device=self.device)
-        self.v_cache = torch.zeros_like(self.k_cache)
+        self.cache_bits, self.cache, self.lengths = cache_bits, None, [0] * batch      # lengths: of the 4-bit cache's sequences
+        if cache_bits == 4:
+            self.cache = Kv4Cache(shape.layers, kvh, hd, batch, max_len, pages, self.device)
+        else:
+            self.k_cache = torch.zeros(shape.layers, b, max_len, kvh, hd, dtype=torch.float16, device=self.device)
+            self.v_cache = torch.zeros_like(self.k_cache)
         inv = 1.0 / (shape.rope_theta ** (torch.arange(0, hd, 2, device=self.device).float() / hd))
         ang = torch.arange(max_len, device=self.device).float()[:, None] * inv[None, :]
         self.cos, self.sin = ang.cos(), ang.sin()
         self.positions = torch.arange(max_len, device=self.device)
         self.token = torch.zeros(b, dtype=torch.long, device=self.device)
-        self.pos = torch.zeros(1, dtype=torch.long, device=self.device)
+        self.pos = torch.zeros(b if cache_bits == 4 else 1, dtype=torch.long, device=self.device)
         self.logits = torch.zeros(b, shape.vocab, dtype=torch.float32, device=self.device)
+        self.sampling = None      # (temperature, top_k, top_p, min_p), each [batch]; None: greedy
+        self.u = torch.zeros(b, dtype=torch.float32, device=self.device)      # the random numbers of a step
         f16 = dict(dtype=torch.float16, device=self.device)
         self._q, self._k, self._v = torch.empty(b, h, **f16), torch.empty(b, kvh * hd, **f16), torch.empty(b, kvh * hd, **f16)
         self._o, self._down = torch.empty(b, h, **f16), torch.empty(b, h, **f16)
         self._gate, self._up = torch.empty(b, shape.ffn, **f16), torch.empty(b, shape.ffn, **f16)
         self._x, self._hn, self._attn = torch.empty(b, h, **f16), torch.empty(b, h, **f16), torch.empty(b, h, **f16)
         self.fused = fused
-        self._attn_ws = decode_ops.attention_workspace_batch(b, shape.heads, hd, self.device) if fused else None
+        if cache_bits == 4:
+            self._attn_ws = decode_ops.attention_kv4_workspace(b, 1, shape.heads, kvh, hd, self.device)
+        else:
+            self._attn_ws = decode_ops.attention_workspace_batch(b, shape.heads, hd, self.device) if fused else None
         self.graph = None
+
+    def set_sampling(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """From the next step on tokens are drawn (:func:`decode_ops.sample_token`); each argument is one number or one per sequence.  A captured
+        graph is dropped unless it already samples: settings and random numbers are then read anew by every replay.  temperature=None: greedy
+        again."""
+        if temperature is None:
+            self.graph, self.sampling = None if self.sampling is not None else self.graph, None
+            return
+        if self.sampling is None:
+            self.graph = None
+            self.sampling = tuple(torch.zeros(self.batch, dtype=t, device=self.device) for t in (torch.float32, torch.int32, torch.float32, torch.float32))
+        for own, v in zip(self.sampling, (temperature, top_k, top_p, min_p)):
+            own.copy_(torch.as_tensor(v, dtype=own.dtype).expand(self.batch))
+
+    def _next_tokens(self, lg):
+        """Tokens of the fp16 logits; the fp32 copy stays in `logits`."""
+        self.logits.copy_(lg.float())
+        if self.sampling is None:
+            self.token.copy_(self.logits.argmax(dim=-1))
+        else:
+            decode_ops.sample_token(lg, self.u, self.token, *self.sampling)
 
     def _rope(self, t, heads):
         hd, b = self.shape.head_dim, self.batch
@@ -426,8 +464,12 @@ class BcqLlamaBatchDecoder:
         for li, blk in enumerate(self.blocks):
             decode_ops.residual_rmsnorm_rows(x, delta, blk.input_norm, hn, x, s.eps)
             _group((blk.q_proj, blk.k_proj, blk.v_proj), hn, (self._q, self._k, self._v))
-            if not decode_ops.rope_attention_decode_batch(self._q, self._k, self._v, self.cos, self.sin, self.pos, self.k_cache[li],
-                                                          self.v_cache[li], self._attn, s.heads, kvh, hd, scale, self._attn_ws):
+            if self.cache_bits == 4:
+                cache = self.cache
+                decode_ops.rope_kv4_write(self._q, self._k, self._v, self.cos, self.sin, self.pos, cache.table, cache.pool[li], self._q, s.heads, kvh, hd)
+                decode_ops.attention_kv4(self._q, cache.pool[li], cache.table, self.pos, self._attn, s.heads, kvh, hd, scale, self._attn_ws)
+            elif not decode_ops.rope_attention_decode_batch(self._q, self._k, self._v, self.cos, self.sin, self.pos, self.k_cache[li],
+                                                            self.v_cache[li], self._attn, s.heads, kvh, hd, scale, self._attn_ws):
                 raise RuntimeError("this head shape is not taken by the fused attention helper: use fused=False")
             _group((blk.o_proj,), self._attn, (self._o,))
             decode_ops.residual_rmsnorm_rows(x, self._o, blk.post_norm, hn, x, s.eps)
@@ -435,8 +477,7 @@ class BcqLlamaBatchDecoder:
             _group((blk.down_proj,), self._gate, (self._down,), x_mul=self._up)   # with SiLU(gate)*up as its activation
             delta = self._down
         decode_ops.residual_rmsnorm_rows(x, delta, self.final_norm, hn, x, s.eps)
-        self.logits.copy_(torch.matmul(hn, self.lm_head.t()).float())
-        self.token.copy_(self.logits.argmax(dim=-1))
+        self._next_tokens(torch.matmul(hn, self.lm_head.t()))
         self.pos.add_(1)
 
     def step(self):
@@ -464,33 +505,135 @@ class BcqLlamaBatchDecoder:
             _group((blk.down_proj,), self._gate, (self._down,), x_mul=self._up)   # with SiLU(gate)*up as its activation
             x = x + self._down
         hn = F.rms_norm(x, (s.hidden,), self.final_norm, s.eps)
-        self.logits.copy_(torch.matmul(hn, self.lm_head.t()).float())
-        self.token.copy_(self.logits.argmax(dim=-1))
+        self._next_tokens(torch.matmul(hn, self.lm_head.t()))
         self.pos.add_(1)
 
-    capture = BcqLlamaDecoder.capture
+    def capture(self):
+        """As :meth:`BcqLlamaDecoder.capture`; the warm-up step of a 4-bit cache writes one position of every sequence."""
+        if self.cache_bits == 4:
+            self._make_room(1)
+        return BcqLlamaDecoder.capture(self)
+
     generate_step = step
 
     def reset(self):
         self.token.zero_()
         self.pos.zero_()
+        if self.cache_bits == 4:
+            for b in range(self.batch):
+                self.cache.free(b)
+            self.lengths = [0] * self.batch
+            return
         self.k_cache.zero_()
         self.v_cache.zero_()
 
+    def _make_room(self, n: int) -> None:
+        """Pages for the next n positions of every sequence (4-bit cache)."""
+        for b, length in enumerate(self.lengths):
+            if length + n > self.max_len:
+                raise ValueError("the sequence does not fit the KV cache")
+            self.cache.reserve(b, length, length + n)
+
+    def _run(self, u=None):
+        """One step (graph replay) with its random numbers."""
+        if self.sampling is not None and u is not None:
+            self.u.copy_(u)
+        (self.graph.replay if self.graph is not None else self.step)()
+        if self.cache_bits == 4:
+            self.lengths = [n + 1 for n in self.lengths]
+
     def feed(self, token_rows):
         """Teacher-forced pass over prompts of equal length: `token_rows` [length][batch] token ids."""
-        run = self.graph.replay if self.graph is not None else self.step
+        if self.cache_bits == 4:
+            self._make_room(len(token_rows))
         for row in token_rows:
             self.token.copy_(torch.as_tensor(row, dtype=torch.long, device=self.device))
-            run()
+            self._run()
 
-    def generate(self, n):
-        run = self.graph.replay if self.graph is not None else self.step
+    def generate(self, n, u=None):
+        """n steps; the tokens [n, batch].  Where tokens are sampled, `u` [n, batch] are the random numbers, in [0, 1)."""
+        if self.sampling is not None and (u is None or tuple(u.shape) != (n, self.batch)):
+            raise ValueError("sampling needs random numbers u [n, batch]")
+        if self.cache_bits == 4:
+            self._make_room(n)
         out = []
-        for _ in range(n):
-            run()
+        for i in range(n):
+            self._run(None if u is None else u[i])
             out.append(self.token.clone())
         return torch.stack(out)                                          # [n, batch]
+
+    def fork(self, src: int, dst: int) -> None:
+        """Sequence `dst` goes on from where `src` is (4-bit cache): its pages are shared until one of the two writes into them."""
+        if self.cache_bits != 4:
+            raise RuntimeError("only a 4-bit cache's sequences can be forked")
+        self.cache.fork(src, dst)
+        self.lengths[dst] = self.lengths[src]
+        self.token[dst], self.pos[dst], self.logits[dst] = self.token[src], self.pos[src], self.logits[src]
+
+    def prefill(self, prompts, u=None):
+        """Prompts of different lengths, a list of token ids (maybe none) for every sequence, in passes of many rows (4-bit cache).  Leaves what a
+        token-by-token feed of each sequence would: its positions in the cache, `pos`, the logits of its last token and the next one (drawn with
+        `u` [batch] where tokens are sampled).  Sequences without tokens keep what they have."""
+        s = self.shape
+        if self.cache_bits != 4:
+            raise RuntimeError("prompts of different lengths need cache_bits=4")
+        if len(prompts) != self.batch:
+            raise ValueError(f"{self.batch} prompts are needed, got {len(prompts)}")
+        if self.sampling is not None and u is None:
+            raise ValueError("sampling needs random numbers u [batch]")
+        counts = [len(p) for p in prompts]
+        if any(n + c > self.max_len for n, c in zip(self.lengths, counts)):
+            raise ValueError("prompt does not fit the KV cache")
+        if not any(counts):
+            return
+        for b, c in enumerate(counts):
+            self.cache.reserve(b, self.lengths[b], self.lengths[b] + c)
+        hd, kvh, h, dev = s.head_dim, s.kv_heads, s.hidden, self.device
+        limit = lutgemm._lib.SAL_MAX_M if any(l.wbit > 4 for blk in self.blocks for l in blk.linears().values()) else BcqLlamaDecoder.PREFILL_ROWS
+        m = min(max(counts), max(1, limit // self.batch))
+        scale, f16 = 1.0 / math.sqrt(hd), dict(dtype=torch.float16, device=dev)
+        ws = decode_ops.attention_kv4_workspace(self.batch, m, s.heads, kvh, hd, dev)
+        ids = torch.zeros(self.batch, -(-max(counts) // m) * m, dtype=torch.long)
+        for b, p in enumerate(prompts):
+            ids[b, :counts[b]] = torch.as_tensor(p, dtype=torch.long)
+        ids, pos = ids.to(dev), self.pos.clone()
+        last = torch.zeros(self.batch, h, **f16)
+        for c0 in range(0, max(counts), m):
+            left = torch.tensor([min(max(c - c0, 0), m) for c in counts], dtype=torch.int32)
+            rows, n = left.to(dev), self.batch * m
+            many = n > lutgemm._lib.SAL_MAX_M
+            x = self.embed.index_select(0, ids[:, c0:c0 + m].reshape(-1))
+            q, k, v = torch.zeros(n, h, **f16), torch.zeros(n, kvh * hd, **f16), torch.zeros(n, kvh * hd, **f16)
+            hn, attn, delta = torch.empty(n, h, **f16), torch.zeros(n, h, **f16), None      # rows that are not there stay zero
+            o_out, down = torch.empty(n, h, **f16), torch.empty(n, h, **f16)
+            gate, up = torch.empty(n, s.ffn, **f16), torch.empty(n, s.ffn, **f16)
+            for li, blk in enumerate(self.blocks):
+                decode_ops.residual_rmsnorm_rows(x, delta, blk.input_norm, hn, x, s.eps)
+                _group((blk.q_proj, blk.k_proj, blk.v_proj), hn, (q, k, v), many_rows=many)
+                decode_ops.rope_kv4_write(q, k, v, self.cos, self.sin, pos, self.cache.table, self.cache.pool[li], q, s.heads, kvh, hd, rows=rows)
+                decode_ops.attention_kv4(q, self.cache.pool[li], self.cache.table, pos, attn, s.heads, kvh, hd, scale, ws, rows=rows)
+                _group((blk.o_proj,), attn, (o_out,), many_rows=many)
+                decode_ops.residual_rmsnorm_rows(x, o_out, blk.post_norm, hn, x, s.eps)
+                _group((blk.gate_proj, blk.up_proj), hn, (gate, up), many_rows=many)
+                _group((blk.down_proj,), gate, (down,), x_mul=up, many_rows=many)   # with SiLU(gate)*up as its activation
+                delta = down
+            if delta is not None:
+                x = x + delta
+            ends = [b for b, c in enumerate(counts) if c0 < c <= c0 + m]      # sequences whose prompt ends in this pass
+            if ends:
+                at = torch.tensor(ends, device=dev)
+                last[at] = x.view(self.batch, m, h)[at, torch.tensor([counts[b] - c0 - 1 for b in ends], device=dev)]
+            pos += rows
+        hn = F.rms_norm(last, (h,), self.final_norm, s.eps)
+        some = torch.tensor([c > 0 for c in counts], device=dev)
+        token, logits = self.token.clone(), self.logits.clone()
+        if self.sampling is not None:
+            self.u.copy_(u)
+        self._next_tokens(torch.matmul(hn, self.lm_head.t()))
+        self.token.copy_(torch.where(some, self.token, token))
+        self.logits.copy_(torch.where(some[:, None], self.logits, logits))
+        self.pos.copy_(pos)
+        self.lengths = [n + c for n, c in zip(self.lengths, counts)]
 
 
 def benchmark_batch(model: BcqLlamaBatchDecoder, prompt_len: int, new_tokens: int, warmup: int = 5, seed: int = 0):
@@ -502,7 +645,11 @@ def benchmark_batch(model: BcqLlamaBatchDecoder, prompt_len: int, new_tokens: in
     if model.graph is None:
         model.capture()
     model.reset()
-    model.feed(prompts)
+    if model.cache_bits == 4:
+        model.prefill(prompts.t().tolist(), u=model.u)
+        model._make_room(max(warmup, new_tokens))
+    else:
+        model.feed(prompts)
     torch.cuda.synchronize(dev)
     state = (model.token.clone(), model.pos.clone())
     for _ in range(warmup):
@@ -512,6 +659,8 @@ def benchmark_batch(model: BcqLlamaBatchDecoder, prompt_len: int, new_tokens: in
     torch.cuda.synchronize(dev)
     t0 = time.perf_counter()
     for _ in range(new_tokens):
+        if model.sampling is not None:
+            model.u.uniform_()
         model.graph.replay()
     torch.cuda.synchronize(dev)
     wall = time.perf_counter() - t0
@@ -564,12 +713,21 @@ def main():
     ap.add_argument("--no-fused", action="store_true", help="plain torch ops between the GEMVs")
     ap.add_argument("--atomic", action="store_true", help="GEMVs accumulate into fixed-point buffers with integer atomics (no split-K tail, still deterministic)")
     ap.add_argument("--batch", type=int, default=1, help="sequences decoded in lock step (small-batch LUT products)")
+    ap.add_argument("--cache-bits", type=int, default=16, choices=(4, 16), help="bits of keys and values in the cache (4: with --batch)")
+    ap.add_argument("--temperature", type=float, help="draw the tokens instead of taking the likeliest (with --batch)")
+    ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--top-p", type=float, default=1.0)
+    ap.add_argument("--min-p", type=float, default=0.0)
     args = ap.parse_args()
+    if args.batch == 1 and (args.cache_bits == 4 or args.temperature is not None):
+        ap.error("--cache-bits 4 and --temperature need --batch 2 or more")
     shape = SHAPES[args.model]
     if args.batch > 1:
-        model = BcqLlamaBatchDecoder(shape, args.wbits, args.groupsize, max_len=args.prompt + 2 * args.new + 16, batch=args.batch)
+        model = BcqLlamaBatchDecoder(shape, args.wbits, args.groupsize, max_len=args.prompt + 2 * args.new + 16, batch=args.batch, cache_bits=args.cache_bits)
+        if args.temperature is not None:
+            model.set_sampling(args.temperature, args.top_k, args.top_p, args.min_p)
         res = benchmark_batch(model, args.prompt, args.new)
-        res.update({"model": args.model, "wbits": args.wbits, "groupsize": args.groupsize, "data": "synthetic weights and prompts"})
+        res.update({"cache_bits": args.cache_bits, "sampled": args.temperature is not None, "model": args.model, "wbits": args.wbits, "groupsize": args.groupsize, "data": "synthetic weights and prompts"})
         print(json.dumps(res))
         return
     model = BcqLlamaDecoder(shape, args.wbits, args.groupsize, max_len=args.prompt + 2 * args.new + 16, fused=not args.no_fused,

@@ -1,0 +1,128 @@
+"""Pages of a 4-bit cache: which sequence has which, on the host.
+
+The pool (:func:`decode_ops.kv4_pool`) holds pages of 64 positions of all layers; a sequence (`slot`) has a list of them, in the device table
+that the kernels read.  Pages are counted: a forked sequence shares its parent's, and whoever first writes into a shared page gets a copy of its
+own.  All calls act in the order of torch's current stream, so pages that earlier launches read may be given away at once; with several
+streams the caller orders them.
+"""
+from __future__ import annotations
+
+import heapq
+
+import torch
+
+from . import decode_ops
+
+PAGE = decode_ops.KV4_PAGE
+
+
+class Kv4Cache:
+    """Keys and values of up to `slots` sequences of up to `max_len` positions, in `pages` pages shared by all.
+
+    ``pool[layer]`` and ``table`` are what :func:`decode_ops.rope_kv4_write`, :func:`decode_ops.attention_kv4` and :func:`decode_ops.read_kv4`
+    take; both stay where they are for as long as the cache lives, so captured launches go on seeing it."""
+
+    def __init__(self, layers: int, kv_heads: int, hd: int, slots: int, max_len: int, pages: int | None = None, device="cuda"):
+        if min(layers, kv_heads, slots, max_len) < 1 or (pages is not None and pages < 1):
+            raise ValueError("layers, kv_heads, slots, max_len and pages must be at least 1")
+        self.kv_heads, self.hd, self.max_len = kv_heads, hd, max_len
+        width = -(-max_len // PAGE)
+        self.pages = slots * width if pages is None else pages
+        self.pool = decode_ops.kv4_pool(layers, self.pages, kv_heads, hd, device)
+        self.table = torch.full((slots, width), -1, dtype=torch.int32, device=device)      # -1: a page that does not exist
+        self._of = [[] for _ in range(slots)]            # pages of each slot, in order
+        self._users = [0] * self.pages
+        self._free = list(range(self.pages))             # a heap: the lowest page first
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def pages_of(self, slot: int) -> list[int]:
+        return list(self._of[slot])
+
+    def _take(self, n: int) -> list[int]:
+        if n > len(self._free):
+            raise RuntimeError(f"the cache has {len(self._free)} free pages, {n} are needed")
+        got = [heapq.heappop(self._free) for _ in range(n)]
+        for p in got:
+            self._users[p] = 1
+        return got
+
+    def _drop(self, page: int) -> None:
+        self._users[page] -= 1
+        if self._users[page] == 0:
+            heapq.heappush(self._free, page)
+
+    def _publish(self, *slots: int) -> None:
+        width = self.table.shape[1]
+        for s in slots:
+            self.table[s].copy_(torch.tensor(self._of[s] + [-1] * (width - len(self._of[s])), dtype=torch.int32))
+
+    def reserve(self, slot: int, first: int, last: int) -> None:
+        """Makes positions first .. last - 1 of a sequence writable: pages it lacks are added, pages it shares with others in that range are
+        replaced by copies.  RuntimeError, and nothing changed, where there are not enough free pages."""
+        if not 0 <= first <= last <= self.max_len:
+            raise ValueError(f"positions {first} .. {last} of {self.max_len}")
+        mine = self._of[slot]
+        if first > len(mine) * PAGE:
+            raise ValueError(f"position {first} lies behind the sequence's {len(mine)} pages")
+        need = -(-last // PAGE)
+        shared = [i for i in range(first // PAGE, min(need, len(mine))) if self._users[mine[i]] > 1] if last > first else []
+        more = max(0, need - len(mine))
+        if not shared and not more:
+            return
+        got = self._take(len(shared) + more)
+        decode_ops.copy_kv4_pages(self.pool, [mine[i] for i in shared], got[:len(shared)])
+        for i, p in zip(shared, got):
+            self._drop(mine[i])
+            mine[i] = p
+        mine += got[len(shared):]
+        self._publish(slot)
+
+    def fork(self, src: int, dst: int) -> None:
+        """Sequence `dst` (whose own pages are given up) becomes one with `src`'s positions; the pages are shared until one of them writes."""
+        if src == dst:
+            return
+        for p in self._of[src]:
+            self._users[p] += 1
+        self._give_up(dst, 0)
+        self._of[dst] = list(self._of[src])
+        self._publish(dst)
+
+    def truncate(self, slot: int, length: int) -> None:
+        """Gives up the pages behind position length - 1."""
+        if length < 0:
+            raise ValueError("length must not be negative")
+        self._give_up(slot, -(-length // PAGE))
+        self._publish(slot)
+
+    def free(self, slot: int) -> None:
+        self.truncate(slot, 0)
+
+    def _give_up(self, slot: int, keep: int) -> None:
+        for p in self._of[slot][keep:]:
+            self._drop(p)
+        del self._of[slot][keep:]
+
+    def compact(self) -> int:
+        """Moves the used pages to the front of the pool; returns their number.  What lies behind them is free."""
+        used = self.pages - len(self._free)
+        moves = {}
+        holes = sorted(p for p in self._free if p < used)
+        for p in range(used, self.pages):
+            if self._users[p]:
+                moves[p] = holes[len(moves)]
+        if moves:
+            decode_ops.copy_kv4_pages(self.pool, list(moves), list(moves.values()))
+            for a, b in moves.items():
+                self._users[b], self._users[a] = self._users[a], 0
+            touched = []
+            for s, mine in enumerate(self._of):
+                if any(p in moves for p in mine):
+                    self._of[s] = [moves.get(p, p) for p in mine]
+                    touched.append(s)
+            self._free = list(range(used, self.pages))
+            heapq.heapify(self._free)
+            self._publish(*touched)
+        return used
