@@ -120,6 +120,8 @@ int sal_causal_softmax_f16(void *scores, int heads, int m, int T, int first, flo
  * 2j (low half) and 2j + 1; group g of position p lies in block g ^ f(p) of its row, f(p) = s(p) for hd 256, s(p) >> 1 for 128, 0 for 64,
  * s(p) = (p & 3) ^ ((p >> 1) & 2).  A page costs kv_heads * 64 * (hd + hd / 8) bytes: 72 bytes for 128 numbers.
  *
+ * heads <= 16384, kv_heads <= 256, max_pages <= 2**20.
+ *
  * Rows: `m` new rows of each of `batch` sequences, batch * m <= SAL_KV4_MAX_ROWS.  Row i of sequence b stands at position pos[b] + i
  * (pos int64, on the device); rows int32 [batch] (may be NULL: all) says how many of the m rows there are, what the others have is neither
  * read nor written.
@@ -131,7 +133,8 @@ int sal_causal_softmax_f16(void *scores, int heads, int m, int T, int first, flo
  * positions without a page.
  * sal_attention_kv4_f16: q [batch][m][heads][hd] (rotated), out likewise; row i of sequence b sees positions 0..pos[b] + i as far as their
  * pages exist (a row that sees none gets zeros).  Scores and sums in fp32.  workspace: sal_attention_kv4_workspace_bytes of scratch, zero-filled
- * once, 16-byte aligned, not shared between streams.
+ * once, 16-byte aligned, for calls of up to that many sequences and rows, not shared between streams (nor between graphs that may run at
+ * once).  Its first word reports a device-side wait that ran out (SAL_E_TIMEOUT; sal_workspace_status reads and clears it).
  * sal_copy_kv4_pages: page dst[i] becomes a copy of page src[i], in all of `layers` layers (pool [layers][pages][page_bytes]).  src and dst
  * are HOST arrays, which the call has done with when it returns; no page may be written twice, or written and read (SAL_E_SHAPE). */
 #define SAL_KV4_PAGE 64

@@ -337,10 +337,14 @@ __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast
 __device__ __forceinline__ __half2 as_half2(uint32_t h) { return *reinterpret_cast<__half2 *>(&h); }
 __device__ __forceinline__ float2 as_float2(uint32_t h) { return __half22float2(*reinterpret_cast<__half2 *>(&h)); }
 
-// Scratch: status word, counter of arrivals per item, then two parts per thread block.
+// Scratch: status word, a counter of arrivals per item that can be shared, then two parts per thread block.  The counters have a place of their own
+// whatever the call's size: they have to be zero between calls, and the parts of a call of another size must not lie there.
 constexpr int WS_HEADER = 256;
+constexpr int MAX_KV_HEADS = 256;
 constexpr int CHUNK = 128;             // units of a block's run that are looked up at once
-constexpr int MAX_LIST = 256;         // (sequence, column tile) pairs whose work is dealt out; with more, a block takes an item
+constexpr int MAX_LIST = 256;                // (sequence, column tile) pairs whose work is dealt out; with more, a block takes an item
+constexpr int SET_ASIDE = 16;         // pages of a warp
+constexpr size_t WS_COUNTERS = (size_t)MAX_LIST * MAX_KV_HEADS * 4;
 constexpr int MIN_UNITS = 3;
 constexpr float MOVE_AT = 256.f;      // weights stay below 2**8 ..
 constexpr float W_ONE = 64.f;         // .. and, times this, inside 16 bits; the second parts' last bit is then 2**-30 of a weight of 1
@@ -370,7 +374,9 @@ struct AttnShape {
     static constexpr int PARTS = WK * PG;                              // warps that share a column
     static constexpr int REC = Record<HD>::BYTES;
     static constexpr int PART = COLS * (HD + 2);                       // floats of a part: outputs, maxima, sums
-    static constexpr int MERGE = PARTS > 1 ? PARTS * PART * 4 : 0;     // bytes of the warps' parts
+    static constexpr int SUMS = NT * (HD / 16) * 4;                    // a lane's running sums
+    static constexpr int SLOT = PARTS > 1 && PART > SUMS * 32 ? PART : SUMS * 32;      // floats of a warp's own memory: its sums, at last its part
+    static constexpr int MERGE = WARPS * SLOT * 4;
     static constexpr bool QUERIES = WC == 1;                           // an item's queries travel with its first page
     static constexpr int STAGE = REC + (QUERIES ? COLS * HD * 2 : 0);
     static constexpr int STAGES = HD == 64 ? 8 : 4;                    // a power of two
@@ -413,7 +419,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
     constexpr int G = R::G, COLS = S::COLS;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring = smem;
-    float *merge = reinterpret_cast<float *>(smem + S::STAGES * S::STAGE);
+    float *merge = reinterpret_cast<float *>(smem + S::STAGES * S::STAGE);      // a slot for every warp
     int2 *sched = reinterpret_cast<int2 *>(smem + S::STAGES * S::STAGE + S::MERGE);      // of two chunks of units: (record or none, item if its first page)
     int *list = reinterpret_cast<int *>(sched + 2 * CHUNK);                              // units in front of a pair, per kv head
     __shared__ uint64_t bars[S::STAGES];
@@ -633,6 +639,11 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
 #pragma unroll
         for (int i = 0; i < (G + 1) / 2; ++i) big_h[i] = 0x04000400u;
         bool first = true;                                      // nothing was added up yet
+        // The tensor core rounds its sums towards zero with every product added: 5e-4 of the output after 2500 of them.  Every so many pages a
+        // warp adds them to sums of its own in shared memory and begins anew.
+        float *own_sums = merge + warp * S::SLOT + lane;
+        bool set_aside = false;
+        int since = 0;
         // the queries are read (a stage is filled again once its page is done with), s_out is written
         asm volatile("bar.sync 1, %0;" ::"n"(S::THREADS) : "memory");
 
@@ -649,6 +660,16 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
             const int st = (seq + p) & (S::STAGES - 1);
             if (alive) alive = mbar_wait(full + 8 * st, (seq + p) / S::STAGES & 1);
             const uint8_t *rec = ring + st * S::STAGE;
+            if (++since > SET_ASIDE) {
+                since = 1;
+#pragma unroll
+                for (int i = 0; i < S::SUMS; ++i) {
+                    float &sum_i = acc[i / (HD / 4)][i / 4 % (HD / 16)][i % 4];
+                    own_sums[32 * i] = set_aside ? own_sums[32 * i] + sum_i : sum_i;
+                    sum_i = 0.f;
+                }
+                set_aside = true;
+            }
             if (alive && sched[(unit0 + pg) & (2 * CHUNK - 1)].x >= 0) {
 #pragma unroll 1
                 for (int i = 0; i < 2 / WK; ++i) {
@@ -795,6 +816,10 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
                                     accm[nt][e][g] *= by;
 #pragma unroll
                                     for (int k = 0; k < 4; ++k) acc[nt][4 * g + k][e] *= by * fg[g], acc[nt][4 * g + k][e + 2] *= by * fg[g];
+                                    if (set_aside) {
+#pragma unroll
+                                        for (int k = 0; k < 8; ++k) own_sums[32 * (nt * (HD / 4) + (4 * g + k / 2) * 4 + e + 2 * (k & 1))] *= by * fg[g];
+                                    }
                                 }
                             }
                         first = false;
@@ -874,7 +899,12 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
         const bool all = n == it.pages;
         // The blocks of an item are neighbours; a part lies in the block's first place if the item began in front of the block, else in its second.
         float *part = a.parts + ((size_t)blockIdx.x * 2 + (at == 0 ? 1 : 0)) * S::PART;
-        float *mine = merge + (wk + WK * pg) * S::PART;
+        if (set_aside) {
+#pragma unroll
+            for (int i = 0; i < S::SUMS; ++i) acc[i / (HD / 4)][i / 4 % (HD / 16)][i % 4] += own_sums[32 * i];
+            __syncwarp();      // the part goes where the sums were
+        }
+        float *mine = merge + warp * S::SLOT;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -935,13 +965,13 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
                 const int col = x / HD;
                 float t[S::PARTS], l[S::PARTS], top = -INFINITY, total = 0.f;
 #pragma unroll
-                for (int w = 0; w < S::PARTS; ++w) t[w] = merge[w * S::PART + COLS * HD + col], l[w] = merge[w * S::PART + COLS * (HD + 1) + col], top = fmaxf(top, t[w]);
+                for (int w = 0; w < S::PARTS; ++w) t[w] = merge[w * S::SLOT + COLS * HD + col], l[w] = merge[w * S::SLOT + COLS * (HD + 1) + col], top = fmaxf(top, t[w]);
                 float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int w = 0; w < S::PARTS; ++w) {
                     if (l[w] == 0.f) continue;
                     const float f = exp2_approx(t[w] - top);
-                    const float4 v = *reinterpret_cast<const float4 *>(merge + w * S::PART + x);
+                    const float4 v = *reinterpret_cast<const float4 *>(merge + w * S::SLOT + x);
                     total += f * l[w];
                     o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
                 }
@@ -1055,7 +1085,7 @@ dim3 row_grid(int batch, int m, int heads, int hd, int per_sm) {
 }
 int check_cache(int batch, int m, int kv_heads, int hd, int max_pages, int pages) {
     if (hd != 64 && hd != 128 && hd != 256) return SAL_E_UNSUPPORTED;
-    if (batch < 1 || m < 1 || kv_heads < 1 || kv_heads > 256 || max_pages < 1 || max_pages > MAX_PAGES || pages < 1) return SAL_E_SHAPE;
+    if (batch < 1 || m < 1 || kv_heads < 1 || kv_heads > MAX_KV_HEADS || max_pages < 1 || max_pages > MAX_PAGES || pages < 1) return SAL_E_SHAPE;
     if ((long long)batch * m > SAL_KV4_MAX_ROWS || (long long)pages * kv_heads > 0x7fffffff) return SAL_E_SHAPE;
     return SAL_OK;
 }
@@ -1079,12 +1109,6 @@ AttnPlan attention_plan(int batch, int m, int rep, int hd) {
     return p;
 }
 
-// Counters of the items that can be shared.  Fewer rows a sequence need no more: up to four narrow tiles stand where a wide one does.
-size_t counter_bytes(const AttnPlan &p, int batch, int kv_heads) {
-    const long long pairs = p.pairs > 4LL * batch ? p.pairs : 4LL * batch;
-    return ((size_t)(pairs < MAX_LIST ? pairs : MAX_LIST) * kv_heads * 4 + 255) / 256 * 256;
-}
-
 template <int HD, int NT, bool DUP, int WK, int PG, int WC>
 int launch_tiles(const AttnArgs &a, const AttnPlan &p, void *stream) {
     using S = AttnShape<HD, NT, DUP, WK, PG, WC>;
@@ -1099,7 +1123,7 @@ int launch_tiles(const AttnArgs &a, const AttnPlan &p, void *stream) {
         int per_sm = 0, sms = 0;
         if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, S::THREADS, S::SMEM) != cudaSuccess || per_sm < 1) return SAL_E_LAUNCH;
         if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return SAL_E_LAUNCH;
-        blocks = per_sm * sms;
+        blocks = (per_sm * sms <= p.max_blocks ? per_sm : p.max_blocks / sms > 0 ? p.max_blocks / sms : 1) * sms;      // the same number on every SM
         resident[dev].store(blocks, std::memory_order_relaxed);
     }
     const unsigned grid = a.whole ? (unsigned)p.pairs * a.c.kv_heads : (unsigned)(blocks < p.max_blocks ? blocks : p.max_blocks);
@@ -1155,7 +1179,7 @@ int sal_read_kv4(const void *pool, const int32_t *table, const int64_t *pos, voi
 size_t sal_attention_kv4_workspace_bytes(int batch, int m, int heads, int kv_heads, int hd) {
     if (check_cache(batch, m, kv_heads, hd, 1, 1) != SAL_OK || heads < 1 || heads > 16384 || heads % kv_heads) return 0;
     const AttnPlan p = attention_plan(batch, m, heads / kv_heads, hd);
-    return WS_HEADER + counter_bytes(p, batch, kv_heads) + (size_t)p.max_blocks * 2 * p.cols * (hd + 2) * 4;
+    return WS_HEADER + WS_COUNTERS + (size_t)p.max_blocks * 2 * p.cols * (hd + 2) * 4;
 }
 
 int sal_attention_kv4_f16(const void *q, const void *pool, const int32_t *table, const int64_t *pos, const int32_t *rows, void *out, int batch, int m,
@@ -1176,7 +1200,7 @@ int sal_attention_kv4_f16(const void *q, const void *pool, const int32_t *table,
     a.out = reinterpret_cast<__half *>(out);
     a.status = reinterpret_cast<int *>(ws);
     a.counters = reinterpret_cast<unsigned *>(ws + WS_HEADER);
-    a.parts = reinterpret_cast<float *>(ws + WS_HEADER + counter_bytes(p, batch, kv_heads));
+    a.parts = reinterpret_cast<float *>(ws + WS_HEADER + WS_COUNTERS);
     a.batch = batch, a.m = m, a.heads = heads, a.rep = heads / kv_heads;
     a.col_tiles = p.col_tiles;
     a.whole = p.pairs > MAX_LIST;

@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
             __syncthreads();
             for (int i = tid; i < BINS; i += THREADS) s.hist[i] = 0;
             __syncthreads();
-            const mass_t ahead_of = survey(by_mass);
+            const mass_t ahead_of = survey(has_p);
             look(by_mass, k - in_front, (goal - (double)ahead_of) / (double)(1ull << UNIT_BITS));
             window[0].y += in_front;      // tokens in front of it in all
         };
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
             if (top_k > 0) {
                 narrow(false, top_k, 0.);
                 const int in_front = window[0].y;
-                gather(window[0].x, window[1].x, false);
+                gather(window[0].x, window[1].x, has_p);      // the prefix's weights are what top_p is of
                 total = listed <= LIST ? settle(false, top_k - in_front, 0.) : by_bits(false, top_k, 0.);
             }
             if (has_p) {
@@ -520,8 +520,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
                 const int k_ties = ties;
                 const double goal = (double)top_p * (double)total;
                 if (top_k > 0) {
-                    if (fine != 1.f) {      // the whole range again
-                        from = 0, upto = BINS - 1, fine = 1.f, front_known = false;
+                    const bool narrowed = fine != 1.f;
+                    from = 0, upto = BINS - 1, fine = 1.f, front_known = false;      // the whole range again
+                    if (narrowed) {
                         __syncthreads();
                         for (int i = tid; i < BINS; i += THREADS) s.hist[i] = 0;
                         __syncthreads();

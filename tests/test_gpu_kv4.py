@@ -522,3 +522,100 @@ def test_the_mean_of_many_values_keeps_its_digits(heads, kvh, m):
     s.masked_fill_(torch.arange(n, device="cuda") > (n - m + torch.arange(m, device="cuda"))[:, None], float("-inf"))
     want = (torch.softmax(s, -1) @ v).transpose(0, 1).reshape(1, m, -1)
     assert (out.double() - want).norm() <= 2.0 ** -11 * want.norm()
+
+
+def test_one_workspace_for_calls_of_every_size():
+    """Scratch of the largest call serves the smaller ones in any order: what one leaves there does not disturb the next."""
+    rng = np.random.default_rng(12)
+    heads, kvh, hd, width = 8, 2, 128, 40
+    pool, table = filled(rng, 4, width, kvh, hd)
+    g_pool, g_table = cuda(pool), cuda(table)
+    ws = decode_ops.attention_kv4_workspace(4, 300, heads, kvh, hd, "cuda")
+    calls = []
+    for batch, m, pos in ((1, 1, [2500]), (4, 300, [2200, 0, 77, 1500]), (2, 5, [2000, 900]), (3, 1, [1, 2, 2555]), (4, 16, [2000] * 4), (1, 200, [2300])):
+        q = cuda(rng.standard_normal((batch, m, heads * hd)).astype(np.float16))
+        args = (q, g_pool, g_table[:batch].contiguous(), torch.tensor(pos, device="cuda"))
+        alone = torch.empty_like(q)
+        decode_ops.attention_kv4(*args, alone, heads, kvh, hd, 0.09, decode_ops.attention_kv4_workspace(batch, m, heads, kvh, hd, "cuda"))
+        calls.append((args, alone))
+    for i in rng.permutation(np.repeat(np.arange(len(calls)), 6)):
+        args, alone = calls[i]
+        out = torch.empty_like(alone)
+        decode_ops.attention_kv4(*args, out, heads, kvh, hd, 0.09, ws)
+        assert torch.equal(out, alone)
+
+
+def written(kvh, hd, lengths, width):
+    """A pool with random rows, its table, and a function that reads a sequence back as K, V [kvh, n, hd] in 64 bits."""
+    batch = len(lengths)
+    pages = sum(-(-n // PAGE) for n in lengths)
+    pool = decode_ops.kv4_pool(1, pages, kvh, hd, "cuda")[0]
+    table = torch.full((batch, width), -1, dtype=torch.int32, device="cuda")
+    order, at = torch.randperm(pages, device="cuda").int(), 0
+    cos, sin = torch.ones(width * PAGE, hd // 2, device="cuda"), torch.zeros(width * PAGE, hd // 2, device="cuda")
+    for b, n in enumerate(lengths):
+        k = -(-n // PAGE)
+        table[b, :k] = order[at:at + k]
+        at += k
+        for c0 in range(0, n, 50000):
+            x, y = (torch.randn(1, min(50000, n - c0), kvh * hd, device="cuda").half() for _ in range(2))
+            decode_ops.rope_kv4_write(x, x, y, cos, sin, torch.tensor([c0], device="cuda"), table[b:b + 1].contiguous(), pool, torch.empty_like(x), kvh, kvh, hd)
+
+    def back(b, heads):
+        got = []
+        for c0 in range(0, lengths[b], 50000):
+            k, v = (torch.empty(1, min(50000, lengths[b] - c0), kvh, hd, device="cuda") for _ in range(2))
+            decode_ops.read_kv4(pool, table[b:b + 1].contiguous(), torch.tensor([c0], device="cuda"), k, v, kvh, hd)
+            got.append((k[0, :, heads].double(), v[0, :, heads].double()))
+        return (torch.cat(x).transpose(0, 1) for x in zip(*got))
+
+    return pool, table, back
+
+
+def against_64_bits(q, out, back, b, pos, kv_head, heads, kvh, hd, scale):
+    """Rows of the query heads of one kv head; the bound as in test_the_mean_of_many_values_keeps_its_digits."""
+    rep, m = heads // kvh, q.shape[1]
+    k, v = back(b, [kv_head])
+    x = q[b].view(m, heads, hd)[:, kv_head * rep:(kv_head + 1) * rep].transpose(0, 1).double()      # [rep, m, hd]
+    s = x @ k[0].T * scale
+    s.masked_fill_(torch.arange(s.shape[-1], device="cuda") > pos + torch.arange(m, device="cuda")[:, None], float("-inf"))
+    want = torch.softmax(s, -1) @ v[0]
+    got = out[b].view(m, heads, hd)[:, kv_head * rep:(kv_head + 1) * rep].transpose(0, 1).double()
+    assert (got - want).norm() <= 2.0 ** -11 * want.norm(), (b, kv_head)
+
+
+def test_runs_of_many_pages():
+    """So much work that a thread block's run has several hundred pages."""
+    torch.manual_seed(6)
+    heads, kvh, hd, lengths = 32, 32, 64, [150001, 70, 90017]
+    pool, table, back = written(kvh, hd, lengths, -(-150001 // PAGE))
+    q = torch.randn(3, 1, heads * hd, device="cuda").half()
+    out, pos = torch.empty_like(q), torch.tensor([n - 1 for n in lengths], device="cuda")
+    decode_ops.attention_kv4(q, pool, table, pos, out, heads, kvh, hd, 0.125, decode_ops.attention_kv4_workspace(3, 1, heads, kvh, hd, "cuda"))
+    for b, h in ((0, 0), (0, 31), (1, 7), (2, 0), (2, 30)):
+        against_64_bits(q, out, back, b, lengths[b] - 1, h, heads, kvh, hd, 0.125)
+
+
+@pytest.mark.parametrize("batch,m,heads,kvh,hd", [(300, 1, 4, 2, 64), (40, 70, 8, 1, 128), (300, 3, 2, 2, 256)])
+def test_more_sequences_than_the_list_takes(batch, m, heads, kvh, hd):
+    """A thread block takes an item then, long texts among them."""
+    torch.manual_seed(7)
+    lengths = [1 + (b * 37) % 200 + m for b in range(batch)]
+    lengths[3], lengths[-1] = 20011, 9000
+    pool, table, back = written(kvh, hd, lengths, -(-20011 // PAGE))
+    q = torch.randn(batch, m, heads * hd, device="cuda").half()
+    out, pos = torch.empty_like(q), torch.tensor([n - m for n in lengths], device="cuda")
+    decode_ops.attention_kv4(q, pool, table, pos, out, heads, kvh, hd, 0.1, decode_ops.attention_kv4_workspace(batch, m, heads, kvh, hd, "cuda"))
+    for b in (0, 3, 17, batch - 2, batch - 1):
+        against_64_bits(q, out, back, b, lengths[b] - m, kvh - 1, heads, kvh, hd, 0.1)
+
+
+def test_queries_may_be_overwritten_by_the_outputs():
+    rng = np.random.default_rng(13)
+    pool, table = filled(rng, 2, 60, 2, 128)
+    q = cuda(rng.standard_normal((2, 3, 8 * 128)).astype(np.float16))
+    args = (cuda(pool), cuda(table), torch.tensor([3700, 40], device="cuda"))
+    out, ws = torch.empty_like(q), decode_ops.attention_kv4_workspace(2, 3, 8, 2, 128, "cuda")
+    decode_ops.attention_kv4(q, *args, out, 8, 2, 128, 0.1, ws)
+    decode_ops.attention_kv4(q, *args, q, 8, 2, 128, 0.1, ws)
+    assert torch.equal(q, out)

@@ -161,3 +161,28 @@ def test_refusals():
             decode_ops.sample_token(**{**dict(logits=x, u=u, token=token), **kw})
     torch.cuda.synchronize()
     assert token.tolist() == [-7] * 3
+
+
+@pytest.mark.parametrize("dtype,off", [(torch.float16, 1), (torch.float16, 7), (torch.float32, 3)])
+def test_rows_that_begin_anywhere(dtype, off):
+    """Rows and slices at any alignment, and nothing read in front of them or behind."""
+    torch.manual_seed(off)
+    for rows, vocab in ((3, 4097), (2, 33001), (1, 130003)):
+        whole = torch.full((off + rows * vocab + 9,), 60000.0, dtype=dtype, device="cuda")      # larger than any logit
+        x = whole[off:off + rows * vocab].view(rows, vocab)
+        x.copy_(2.5 * torch.randn(rows, vocab, device="cuda"))
+        for f in (dict(), dict(top_k=30, top_p=0.8), dict(top_p=0.95), dict(temperature=0.0)):
+            check(x, torch.rand(rows, device="cuda"), **f)
+
+
+@pytest.mark.parametrize("rows,vocab", [(300, 2048), (40, 60000), (1, 8192)])
+def test_few_values_many_times(rows, vocab):
+    """Logits on a coarse grid: windows full of equal logits, in one bin and in many."""
+    torch.manual_seed(rows)
+    for levels in (2, 5, 60):
+        x = (torch.randint(0, levels, (rows, vocab), device="cuda").float() / levels * 4).half()
+        for f in (dict(top_k=vocab // 3), dict(top_p=0.6), dict(top_k=vocab // 2, top_p=0.5, min_p=0.2)):
+            check(x[:4].contiguous(), torch.rand(min(rows, 4), device="cuda"), **f)
+        token = torch.empty(rows, dtype=torch.int64, device="cuda")
+        decode_ops.sample_token(x, torch.rand(rows, device="cuda"), token, top_p=0.6)
+        assert ((token >= 0) & (token < vocab)).all()
