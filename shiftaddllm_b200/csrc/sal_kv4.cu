@@ -345,7 +345,6 @@ constexpr int CHUNK = 128;             // units of a block's run that are looked
 constexpr int MAX_LIST = 256;                // (sequence, column tile) pairs whose work is dealt out; with more, a block takes an item
 constexpr int SET_ASIDE = 16;         // pages of a warp
 constexpr size_t WS_COUNTERS = (size_t)MAX_LIST * MAX_KV_HEADS * 4;
-constexpr int MIN_UNITS = 3;
 constexpr float MOVE_AT = 256.f;      // weights stay below 2**8 ..
 constexpr float W_ONE = 64.f;         // .. and, times this, inside 16 bits; the second parts' last bit is then 2**-30 of a weight of 1
 
@@ -379,7 +378,12 @@ struct AttnShape {
     static constexpr int MERGE = WARPS * SLOT * 4;
     static constexpr bool QUERIES = WC == 1;                           // an item's queries travel with its first page
     static constexpr int STAGE = REC + (QUERIES ? COLS * HD * 2 : 0);
-    static constexpr int STAGES = HD == 64 ? 8 : 4;                    // a power of two
+    // What an item costs by itself (its first page's wait, the sum over the warps, the output or the part) in pages: 2.8 us against 1.2 us a page
+    // with one column and heads of 128.  Counted as 1, 2, 3, 4 pages: 63, 55, 54, 54 us for 16 sequences of 300 to 4000 positions with 32 heads;
+    // with 64 columns (512 rows behind 1536 positions, 32 heads) 134, 135, 137, 139.
+    static constexpr int ITEM_UNITS = WC == 1 ? 3 : 1;
+    static constexpr int MIN_UNITS = ITEM_UNITS + 2;
+    static constexpr int STAGES = 4;      // a power of two; so many pages on lie within 32 units, ITEM_UNITS at most being in front of each
     static constexpr int SMEM = STAGES * STAGE + MERGE + 2 * CHUNK * 8 + MAX_LIST * 4 + 16;
     static constexpr int MIN_BLOCKS = HD < 256 && NT == 1 ? 3 : 2;
 };
@@ -416,7 +420,7 @@ template <int HD, int NT, bool DUP, int WK, int PG, int WC>
 __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, AttnShape<HD, NT, DUP, WK, PG, WC>::MIN_BLOCKS) attention_tiles_kernel(AttnArgs a) {
     using S = AttnShape<HD, NT, DUP, WK, PG, WC>;
     using R = Record<HD>;
-    constexpr int G = R::G, COLS = S::COLS;
+    constexpr int G = R::G, COLS = S::COLS, ITEM_UNITS = S::ITEM_UNITS;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring = smem;
     float *merge = reinterpret_cast<float *>(smem + S::STAGES * S::STAGE);      // a slot for every warp
@@ -436,21 +440,20 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
     pdl_prologue();
     const int kvh = a.c.kv_heads, pairs = a.batch * a.col_tiles;
     Item it = {};
-    // The list counts an item as its pages and one unit more, which stands for what an item costs by itself (first page's wait, sum over
-    // the warps, output).  This block's run: `left` units from unit `at` of the item on.
+    // The list counts an item as ITEM_UNITS and its pages.  This block's run: `left` units from unit `at` of the item on.
     int at, pair;
     long long left, per = 0;
     if (a.whole) {
         pair = blockIdx.x / kvh;
         it.h = blockIdx.x % kvh;
         if (!item_of<COLS>(a, pair / a.col_tiles, pair % a.col_tiles, it)) return;
-        at = 0, left = it.pages + 1;
+        at = 0, left = it.pages + ITEM_UNITS;
     } else {
         int total = 0;         // units of all pairs, and in front of each
         for (int i0 = 0; i0 < pairs; i0 += S::THREADS) {
             const int i = i0 + tid;
             Item x = {};
-            const int n = i < pairs && item_of<COLS>(a, i / a.col_tiles, i % a.col_tiles, x) ? x.pages + 1 : 0;
+            const int n = i < pairs && item_of<COLS>(a, i / a.col_tiles, i % a.col_tiles, x) ? x.pages + ITEM_UNITS : 0;
             int run = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -471,7 +474,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
         __syncthreads();
         const long long all = (long long)total * kvh;
         per = (all + gridDim.x - 1) / gridDim.x;
-        if (per < MIN_UNITS) per = MIN_UNITS;
+        if (per < S::MIN_UNITS) per = S::MIN_UNITS;
         const long long begin = per * blockIdx.x;
         if (begin >= all) return;
         left = begin + per < all ? per : all - begin;
@@ -485,14 +488,14 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
         pair = lo;
         const int in_pair = (int)(begin - (long long)list[pair] * kvh);
         item_of<COLS>(a, pair / a.col_tiles, pair % a.col_tiles, it);
-        it.h = in_pair / (it.pages + 1);
-        at = in_pair % (it.pages + 1);
+        it.h = in_pair / (it.pages + ITEM_UNITS);
+        at = in_pair % (it.pages + ITEM_UNITS);
     }
     const int cols = a.m * a.rep;
 
     // ---- what the run fetches: unit by unit, a chunk at a time, one unit per thread ----------------------------------------------------
     const long long units = left, begin = per * blockIdx.x;
-    constexpr int NOTHING = -2, NO_PAGE = -1;       // an item's own unit, or behind the run; a page that does not exist
+    constexpr int NOTHING = -2, NO_PAGE = -1;       // an item's own units, or behind the run; a page that does not exist
     const int pair0 = pair, h0 = it.h, at0 = at;
     auto look_up = [&](int chunk) {
         static_assert(CHUNK == S::THREADS, "a thread looks up one unit");
@@ -511,10 +514,10 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
                 const int in_pair = (int)(begin + u - (long long)list[p] * kvh), n = list[p + 1] - list[p];
                 h = in_pair / n, t = in_pair % n;
             }
-            if (t > 0) {
-                const int page = a.c.table[(size_t)(p / a.col_tiles) * a.c.max_pages + t - 1];
+            if (t >= ITEM_UNITS) {
+                const int page = a.c.table[(size_t)(p / a.col_tiles) * a.c.max_pages + t - ITEM_UNITS];
                 e.x = page >= 0 && page < a.c.pages ? page * kvh + h : NO_PAGE;
-                if (t == 1 || u == 0) e.y = p * kvh + h;
+                if (t == ITEM_UNITS || u == 0) e.y = p * kvh + h;
             }
         }
         sched[(chunk & 1) * CHUNK + tid] = e;
@@ -548,7 +551,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
     }
     // moves on to the next item: the next kv head, or the next pair that has rows
     auto next_item = [&] {
-        left -= it.pages + 1 - at;
+        left -= it.pages + ITEM_UNITS - at;
         at = 0;
         if (left <= 0 || ++it.h < kvh) return;
         do ++pair;
@@ -566,8 +569,8 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
     int seq = 0, next_chunk = CHUNK;               // pages of the run in front of the item
     bool alive = true;
     for (; left > 0; next_item()) {
-        const int base = max(at - 1, 0), n = (int)min((long long)at + left, (long long)it.pages + 1) - 1 - base;
-        if (n <= 0) continue;       // the item's first unit only
+        const int base = max(at - ITEM_UNITS, 0), n = (int)min((long long)at + left, (long long)it.pages + ITEM_UNITS) - ITEM_UNITS - base;
+        if (n <= 0) continue;       // units of the item itself only
         const int there = min(min(COLS, cols - it.ct * COLS), it.rows * a.rep - it.ct * COLS);      // columns of the item
         if (tid < there) {
             const int j = it.ct * COLS + tid;
@@ -648,7 +651,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
         asm volatile("bar.sync 1, %0;" ::"n"(S::THREADS) : "memory");
 
         for (int p0 = 0; p0 < n; p0 += PG) {
-            const int unit0 = (int)(units - left) + base + p0 + 1 - at;
+            const int unit0 = (int)(units - left) + base + p0 + ITEM_UNITS - at;
             if (unit0 >= next_chunk) {      // two chunks are at hand: the one behind is looked up once nobody needs the one in front
                 asm volatile("bar.sync 1, %0;" ::"n"(S::THREADS) : "memory");
                 look_up(next_chunk / CHUNK + 1);
@@ -985,8 +988,8 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
         }
         if (!all) {
             // first and last block that has pages of this item
-            const long long start = (long long)list[pair] * kvh + (long long)it.h * (it.pages + 1);
-            const int block0 = (int)((start + 1) / per), block1 = (int)((start + it.pages) / per);
+            const long long start = (long long)list[pair] * kvh + (long long)it.h * (it.pages + ITEM_UNITS);
+            const int block0 = (int)((start + ITEM_UNITS) / per), block1 = (int)((start + ITEM_UNITS + it.pages - 1) / per);
             unsigned *counter = a.counters + (size_t)pair * kvh + it.h;
             asm volatile("bar.sync 1, %0;" ::"n"(S::WARPS * 32) : "memory");
             if (tid == 0) {
