@@ -360,6 +360,7 @@ struct AttnArgs {
     int batch, m, heads, rep;
     int col_tiles;      // column tiles of a sequence
     int whole;          // a block takes an item
+    int splits;         // of an item's pages, at most (many columns)
     float scale_log2;   // scale * log2(e) * UNIT
 };
 
@@ -1064,6 +1065,514 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
     }
 }
 
+// ---- many columns: the fifth generation's tensor cores --------------------------------------------------------------------------------
+//
+// The same sums with the queries as rows of the products: 128 columns of an item against a page.  Codes less 8 are expanded once for all 128 into
+// shared memory as 16-bit floats (exact; 64 positions x 64 numbers in rows of 128 bytes, swizzled), which serves the keys as an operand that
+// runs along the dimensions and the values as one that runs along the positions.  D_g stands in tensor memory, one row a lane; two threads share a
+// row, each with 32 of the page's positions.  They leave the weights p * s_g / E_g as two 16-bit parts where D_g was, from where they are the second
+// product's first operand.  A page's outputs start from zero and are added to 32-bit sums in registers, so the maximum may move with every page
+// and nothing is added up in the tensor core beyond a page.  E_g is the page's own.
+//
+// A block takes one item, or one of `splits` equal runs of its pages; the last one to arrive adds the parts up in order.  Items with the most pages are
+// launched first.  While the tensor core works for one of the two blocks of an SM the other one expands, and within a block the next page's keys are expanded
+// behind the second product's back.
+template <int HD>
+struct WideShape {
+    static constexpr int G = HD / GROUP, COLS = 128, THREADS = 256, STAGES = 3;
+    static constexpr int REC = Record<HD>::BYTES;
+    static constexpr int Q_BYTES = G * COLS * 128, TILE = PAGE * 128, T_BYTES = G * TILE;      // a group of the queries, of a page
+    static constexpr int SMEM = 1024 + Q_BYTES + 2 * T_BYTES + STAGES * REC + 2 * G * PAGE * 8 + 2 * (1 + G) * COLS * 4;
+    static constexpr int TMEM = 2 * HD;                                // columns: D_g or weights, then outputs
+    static constexpr int PART = COLS * (HD + 2);
+};
+constexpr int WIDE_BLOCKS = 2 * 148;      // resident at once
+constexpr int WIDE_SPLITS = 32;
+
+__device__ __forceinline__ void tmem_load8(float *v, uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "r"(addr)
+                 : "memory");
+}
+// two 32-bit sums or products at once
+struct Two {
+    unsigned long long x;
+    __device__ __forceinline__ Two() {}
+    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ float2 get() const {
+        float2 v;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(x));
+        return v;
+    }
+};
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+    Two d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.x) : "l"(a.x), "l"(b.x), "l"(c.x));
+    return d;
+}
+__device__ __forceinline__ Two mul(Two a, Two b) {
+    Two d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.x) : "l"(a.x), "l"(b.x));
+    return d;
+}
+__device__ __forceinline__ Two add(Two a, Two b) {
+    Two d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.x) : "l"(a.x), "l"(b.x));
+    return d;
+}
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t *v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }      // own writes, for the tensor core
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// d[128][64] = or += a * b, a in shared memory
+__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t more) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                 "r"(more)
+                 : "memory");
+}
+// a in tensor memory
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t more) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+                 "r"(more)
+                 : "memory");
+}
+// Rows of 128 bytes, eight of them an atom of 1024, 128-byte swizzle; both strides are an atom's (an operand of 64 numbers across has one of them only).
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {
+    return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(1024 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// eight codes less 8 as 16-bit floats, in the order 0 4 1 5 2 6 3 7
+__device__ __forceinline__ uint4 eight_codes(uint32_t x) {
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t y = x >> (8 * i);
+        asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(o[2 * i]) : "r"(y));
+        asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(o[2 * i + 1]) : "r"(y));
+        asm("add.rn.f16x2 %0, %0, %1;" : "+r"(o[2 * i]) : "r"(0xe408e408u));                                // 1024 + c - 1032
+        asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(o[2 * i + 1]) : "r"(0x2c002c00u), "r"(0xd480d480u));      // (1024 + 16 c) / 16 - 72
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(WideShape<HD>::THREADS, 2) attention_wide_kernel(AttnArgs a) {
+    using S = WideShape<HD>;
+    using R = Record<HD>;
+    constexpr int G = S::G, COLS = S::COLS, N = HD / 2;      // outputs of a thread
+    extern __shared__ __align__(1024) uint8_t wide_smem[];
+    __shared__ uint64_t bars[S::STAGES + 2];
+    __shared__ uint32_t s_tmem;
+    __shared__ float s_back[G];
+    __shared__ int s_flag;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, half = tid / COLS, row = tid % COLS;
+    uint8_t *smem = wide_smem + ((1024u - (smem_u32(wide_smem) & 1023u)) & 1023u);
+    const uint32_t q_tile = smem_u32(smem), k_tile = q_tile + S::Q_BYTES, v_tile = k_tile + S::T_BYTES;
+    uint8_t *ring = smem + S::Q_BYTES + 2 * S::T_BYTES;
+    float *kp = reinterpret_cast<float *>(ring + S::STAGES * S::REC), *vp = kp + 2 * G * PAGE;      // of [group][pair of positions]: two scales, two lowest + 8 scales
+    float *swap = reinterpret_cast<float *>(vp + 2 * G * PAGE);      // [half][1 + G][row]
+    const uint32_t full = smem_u32(bars), bar_s = full + 8 * S::STAGES, bar_o = bar_s + 8;
+
+    // The tensor memory is taken behind the wait for the launch in front and before the next one may start: neither then holds what the other waits for.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int kvh = a.c.kv_heads, split = blockIdx.x % a.splits, item = blockIdx.x / a.splits;
+    Item it = {};
+    it.h = item % kvh;
+    if (!item_of<COLS>(a, item / kvh % a.batch, a.col_tiles - 1 - item / kvh / a.batch, it)) return;
+    const int pair = it.b * a.col_tiles + it.ct;
+    const int splits = min(a.splits, (it.pages + 3) / 4);      // a run has four pages at least, or the item one run
+    if (split >= splits) return;
+    const int page1 = (int)((long long)it.pages * (split + 1) / splits);
+    const int32_t *table = a.c.table + (size_t)it.b * a.c.max_pages;
+    auto next_page = [&](int p) {      // the next one that exists
+        for (; p < page1; ++p) {
+            const int x = table[p];
+            if (x >= 0 && x < a.c.pages) break;
+        }
+        return p;
+    };
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(S::TMEM) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        fence_before();
+    } else if (tid == 32) {
+        for (int i = 0; i < S::STAGES + 2; ++i) mbar_init(full + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    fence_after();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem = s_tmem, mine = tmem + ((uint32_t)(warp & 3) << 21);      // lanes of this warp: 32 of them
+
+    int p = next_page((int)((long long)it.pages * split / splits));
+    int to_fetch = p;      // of one thread
+    auto fetch = [&](int st) {
+        if (to_fetch >= page1) return;
+        mbar_expect_tx(full + 8 * st, S::REC);
+        bulk_copy(smem_u32(ring + st * S::REC), a.c.pool + ((size_t)table[to_fetch] * kvh + it.h) * S::REC, S::REC, full + 8 * st);
+        to_fetch = next_page(to_fetch + 1);
+    };
+    if (tid == 32)
+        for (int st = 0; st < S::STAGES; ++st) fetch(st);
+    __syncwarp();
+
+    // ---- queries: rows of the first operand, zero where there is no column ---------------------------------------------------------------
+    const int col = it.ct * COLS + row, i_row = col / a.rep;
+    const bool real = col < a.m * a.rep && i_row < it.rows;
+    const size_t at = (((size_t)it.b * a.m + i_row) * a.heads + it.h * a.rep + col % a.rep) * HD + half * N;
+    float qsum[G];
+    {
+        const int g = half * N / GROUP, chunk0 = half * N % GROUP / 8;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < N / 8; ++i) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (real) x = *reinterpret_cast<const uint4 *>(a.q + at + 8 * i);
+            const float2 f0 = as_float2(x.x), f1 = as_float2(x.y), f2 = as_float2(x.z), f3 = as_float2(x.w);
+            sum += f0.x + f0.y + f1.x + f1.y + f2.x + f2.y + f3.x + f3.y;
+            *reinterpret_cast<uint4 *>(smem + g * COLS * 128 + row * 128 + (((chunk0 + i) ^ (row & 7)) << 4)) =
+                make_uint4(prmt(x.x, x.z, 0x5410), prmt(x.x, x.z, 0x7632), prmt(x.y, x.w, 0x5410), prmt(x.y, x.w, 0x7632));      // in the codes' order
+        }
+        swap[half * (1 + G) * COLS + row] = sum;
+    }
+    const int lim = real ? min(it.first + i_row, a.c.max_pages * PAGE - 1) : -2;
+    const int low_lim = __reduce_min_sync(0xffffffffu, real ? lim : 0x7fffffff), top_lim = __reduce_max_sync(0xffffffffu, lim);      // of 32 rows
+
+    // ---- a page's codes and parameters ------------------------------------------------------------------------------------------------
+    const int hb = tid & 1, xg = G == 2 ? tid >> 3 & 1 : 0, xk = G == 2 ? tid >> 4 << 2 | (tid >> 1 & 3) : tid >> 1;      // 16 bytes: both sides without bank conflicts
+    const int x_from = xk * R::ROW + R::place(xg, xk) * 32 + 16 * hb;
+    auto expand = [&](const uint8_t *codes, uint32_t tile) {
+        if (tid >= 2 * G * PAGE) return;
+        const uint4 x = *reinterpret_cast<const uint4 *>(codes + x_from);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        uint8_t *to = smem + (tile - q_tile) + xg * S::TILE + xk * 128;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4 *>(to + ((4 * hb + i) ^ (xk & 7)) * 16) = eight_codes(w[i]);
+    };
+    const float scale_log2 = a.scale_log2 * (1.f / UNIT);
+    auto parameters = [&](const uint8_t *rec, int page) {      // positions behind the last one that is seen: nothing
+        const __half2 *from = reinterpret_cast<const __half2 *>(rec + 2 * R::CODES);
+        if (tid < G * PAGE) {
+            const int k = tid % PAGE, g = tid / PAGE;
+            const float2 x = page * PAGE + k <= it.last ? __half22float2(from[k * G + g]) : make_float2(0.f, 0.f);
+            float *to = kp + (tid >> 1) * 4 + (tid & 1);
+            to[0] = x.x * scale_log2, to[2] = fmaf(8.f, x.x, x.y) * scale_log2;
+        }
+        if (warp >= 4 && warp < 4 + G) {
+            const int g = warp - 4;
+            float2 x[2];
+            float top = 6.1035156e-5f;      // 2**-14
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int k = lane + 32 * e;
+                x[e] = page * PAGE + k <= it.last ? __half22float2(from[R::PARAMS / 4 + k * G + g]) : make_float2(0.f, 0.f);
+                top = fmaxf(top, x[e].x);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float big = __uint_as_float((__float_as_uint(top) + 0x007fffffu) & 0x7f800000u);      // the power of two from there on
+            const float to_one = W_ONE / big;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float *to = vp + ((g * PAGE + lane + 32 * e) >> 1) * 4 + (lane & 1);
+                to[0] = x[e].x * to_one, to[2] = fmaf(8.f, x[e].x, x[e].y);
+            }
+            if (lane == 0) s_back[g] = big / W_ONE;
+        }
+    };
+    constexpr uint32_t IDESC = 1u << 4 | (uint32_t)(PAGE >> 3) << 17 | (uint32_t)(COLS >> 4) << 24;      // 32-bit sums, 16-bit operands, 128 x 64
+    constexpr uint32_t IDESC_V = IDESC | 1u << 16;                                                     // the second operand runs along the positions
+    auto scores = [&] {
+        if (warp == 0) {
+            if (elect_one()) {
+                fence_after();
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma_smem(tmem + 64 * g, tile_desc(q_tile + g * COLS * 128) + 2 * k, tile_desc(k_tile + g * S::TILE) + 2 * k, IDESC, k);
+                mma_commit(bar_s);
+            }
+            __syncwarp();
+        }
+    };
+    auto outputs = [&] {
+        if (warp == 0) {
+            if (elect_one()) {
+                fence_after();
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {      // 16 positions, first or second parts of their weights
+                        const int k = x >> 1;
+                        mma_tmem(tmem + HD + 64 * g, tmem + 64 * g + 8 * x, tile_desc(v_tile + g * S::TILE + 16 * k * 128), IDESC_V, x);
+                    }
+                mma_commit(bar_o);
+            }
+            __syncwarp();
+        }
+    };
+
+    bool alive = true;
+    Two acc[N / 2], sums(0.f, 0.f);      // outputs
+    float accm[G], ref = -INFINITY, back = 0.f, f = 1.f;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) acc[i] = Two(0.f, 0.f);
+#pragma unroll
+    for (int g = 0; g < G; ++g) accm[g] = 0.f;
+    bool taken = false;      // this warp's rows see something of the page
+    int seq = 0;
+    auto take = [&] {      // the outputs of page seq - 1
+        if (alive) alive = mbar_wait(bar_o, (seq - 1) & 1);
+        __syncwarp();
+        fence_after();
+        if (!taken) return;
+        if (__any_sync(0xffffffffu, f != 1.f)) {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) acc[i] = mul(acc[i], Two(f, f));
+        }
+#pragma unroll
+        for (int i = 0; i < N; i += 16) {
+            float v[16];
+            tmem_load8(v, mine + HD + half * N + i);
+            tmem_load8(v + 8, mine + HD + half * N + i + 8);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) acc[(i + e) / 2] = fma(Two(v[e], v[e + 1]), Two(back, back), acc[(i + e) / 2]);
+        }
+    };
+    if (p < page1) {
+        if (alive) alive = mbar_wait(full, 0);
+        __syncwarp();
+        expand(ring, k_tile);
+        parameters(ring, p);
+    }
+    fence_smem();
+    __syncthreads();
+#pragma unroll
+    for (int g = 0; g < G; ++g) qsum[g] = G == 2 ? swap[g * (1 + G) * COLS + row] : swap[row] + swap[(1 + G) * COLS + row];
+    if (p < page1) scores();
+    __syncthreads();      // `swap` is free
+
+    for (; p < page1; ++seq) {
+        const int st = seq % S::STAGES, after = next_page(p + 1);
+        if (seq) take();
+        expand(ring + st * S::REC + R::CODES, v_tile);
+        if (alive) alive = mbar_wait(bar_s, seq & 1);
+        __syncwarp();
+        fence_after();
+        taken = p * PAGE <= top_lim;
+        if (taken) {
+            const int t0 = p * PAGE + 32 * half;
+            const uint32_t own = mine + 32 * half;      // this thread's columns of group 0
+            const bool masked = p * PAGE + PAGE - 1 > low_lim;      // for some of the rows
+            float top = -INFINITY;
+            // scores into the last group's place, the registers being the outputs'
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+                float d[G][8];
+#pragma unroll
+                for (int g = 0; g < G; ++g) tmem_load8(d[g], own + 64 * g + k);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                float u[8];
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    Two t(0.f, 0.f);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const float4 x = *reinterpret_cast<const float4 *>(kp + 2 * (g * PAGE + 32 * half + k + e));
+                        const Two low = g ? fma(Two(x.z, x.w), Two(qsum[g], qsum[g]), t) : mul(Two(x.z, x.w), Two(qsum[g], qsum[g]));
+                        t = fma(Two(x.x, x.y), Two(d[g][e], d[g][e + 1]), low);
+                    }
+                    const float2 v = t.get();
+                    u[e] = v.x, u[e + 1] = v.y;
+                }
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) u[e] = t0 + k + e <= lim ? u[e] : -INFINITY;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, u[e]);
+                tmem_store8(own + 64 * (G - 1) + k, reinterpret_cast<const uint32_t *>(u));
+            }
+            swap[half * (1 + G) * COLS + row] = top;
+            switch (warp & 3) {      // the two warps of these rows
+                case 0: asm volatile("bar.sync 1, 64;" ::: "memory"); break;
+                case 1: asm volatile("bar.sync 2, 64;" ::: "memory"); break;
+                case 2: asm volatile("bar.sync 3, 64;" ::: "memory"); break;
+                default: asm volatile("bar.sync 4, 64;" ::: "memory"); break;
+            }
+            top = fmaxf(ref, fmaxf(top, swap[(1 - half) * (1 + G) * COLS + row]));
+            const float from = top == -INFINITY ? 0.f : top;
+            f = ref == -INFINITY ? 1.f : exp2_approx(ref - from);
+            ref = top;
+            back = s_back[half * N / GROUP];
+            sums = mul(sums, Two(f, f));
+            Two low[G];
+#pragma unroll
+            for (int g = 0; g < G; ++g) low[g] = Two(0.f, 0.f);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            auto weights = [&](auto some) {      // where a position is not seen its parameters are not looked at either
+#pragma unroll
+                for (int k = 0; k < 32; k += 16) {
+                    float s[16];
+                    tmem_load8(s, own + 64 * (G - 1) + k), tmem_load8(s + 8, own + 64 * (G - 1) + k + 8);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    Two w[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float2 v = add(Two(s[2 * e], s[2 * e + 1]), Two(-from, -from)).get();
+                        w[e] = Two(exp2_approx(v.x), exp2_approx(v.y));
+                        sums = add(sums, w[e]);
+                    }
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        uint32_t hi[8], lo[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            float4 x = *reinterpret_cast<const float4 *>(vp + 2 * (g * PAGE + 32 * half + k + 2 * e));
+                            if (decltype(some)::value) {
+                                if (t0 + k + 2 * e > lim) x.x = 0.f, x.z = 0.f;
+                                if (t0 + k + 2 * e + 1 > lim) x.y = 0.f, x.w = 0.f;
+                            }
+                            const Two z = mul(w[e], Two(x.x, x.y));
+                            low[g] = fma(w[e], Two(x.z, x.w), low[g]);
+                            const float2 v = z.get();
+                            const __half2 h = __floats2half2_rn(v.x, v.y);
+                            const float2 r = __half22float2(h);
+                            const float2 rest = add(z, Two(-r.x, -r.y)).get();
+                            hi[e] = as_u32(h), lo[e] = as_u32(__floats2half2_rn(rest.x, rest.y));
+                        }
+                        tmem_store8(own + 64 * g + k, hi);      // where the scores of these positions were
+                        tmem_store8(own + 64 * g + k + 8, lo);
+                    }
+                }
+            };
+            if (masked) weights(std::true_type{});
+            else weights(std::false_type{});
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const float2 v = low[g].get();
+                accm[g] = fmaf(accm[g], f, v.x + v.y);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+        fence_before();
+        fence_smem();
+        __syncthreads();
+        outputs();
+        if (tid == 32) fetch(st);
+        __syncwarp();
+        if (after < page1) {
+            const int next = (seq + 1) % S::STAGES;
+            if (alive) alive = mbar_wait(full + 8 * next, (seq + 1) / S::STAGES & 1);
+            __syncwarp();
+            expand(ring + next * S::REC, k_tile);
+            parameters(ring + next * S::REC, after);
+            fence_smem();
+            __syncthreads();
+            scores();
+        }
+        p = after;
+    }
+    if (seq) take();
+
+    // ---- the outputs, or a part of them --------------------------------------------------------------------------------------------------
+    fence_before();
+    __syncthreads();
+    const float2 both = sums.get();
+    float sum = both.x + both.y, out[N];
+    swap[half * (1 + G) * COLS + row] = sum;
+#pragma unroll
+    for (int g = 0; g < G; ++g) swap[(half * (1 + G) + 1 + g) * COLS + row] = accm[g];
+    __syncthreads();
+    {
+        const int g = half * N / GROUP;
+        sum = swap[row] + swap[(1 + G) * COLS + row];
+        const float low = swap[(1 + g) * COLS + row] + swap[(2 + G + g) * COLS + row];
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 v = acc[i / 2].get();
+            out[i] = v.x + low, out[i + 1] = v.y + low;
+        }
+    }
+    auto store = [&](auto get, float total) {      // get(i): output i, in order
+        if (!real) return;
+        const float inv = 1.f / total;
+#pragma unroll
+        for (int i = 0; i < N; i += 8) {
+            uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = total == 0.f ? 0u : as_u32(__floats2half2_rn(get(i + 2 * e) * inv, get(i + 2 * e + 1) * inv));      // no position: zeros
+            *reinterpret_cast<uint4 *>(a.out + at + i) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+    };
+    auto in_order = [&](int i) { return out[(i & ~7) + 2 * (i & 3) + (i >> 2 & 1)]; };
+    if (splits == 1) {
+        store(in_order, sum);
+    } else {
+        const size_t first = ((size_t)pair * kvh + it.h) * a.splits;
+        float *part = a.parts + (first + split) * S::PART;      // [output / 4][row][4], maxima, sums
+        float4 *part4 = reinterpret_cast<float4 *>(part) + half * (N / 4) * COLS + row;
+#pragma unroll
+        for (int i = 0; i < N; i += 4) __stcg(part4 + i / 4 * COLS, make_float4(in_order(i), in_order(i + 1), in_order(i + 2), in_order(i + 3)));
+        if (half == 0) __stcg(part + COLS * HD + row, sum == 0.f ? -INFINITY : ref), __stcg(part + COLS * (HD + 1) + row, sum);
+        unsigned *counter = a.counters + (size_t)pair * kvh + it.h;
+        __syncthreads();
+        if (tid == 0) {
+            unsigned old;
+            asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+            s_flag = old == (unsigned)(splits - 1);
+        }
+        __syncthreads();
+        if (s_flag) {
+            const float *parts = a.parts + first * S::PART;
+            float top = -INFINITY, total = 0.f;
+            for (int k = 0; k < splits; ++k) top = fmaxf(top, __ldcg(parts + (size_t)k * S::PART + COLS * HD + row));
+#pragma unroll
+            for (int i = 0; i < N; ++i) out[i] = 0.f;
+            for (int k = 0; k < splits; ++k) {
+                const float *other = parts + (size_t)k * S::PART;
+                const float l = __ldcg(other + COLS * (HD + 1) + row), t = __ldcg(other + COLS * HD + row);
+                const float4 *other4 = reinterpret_cast<const float4 *>(other) + half * (N / 4) * COLS + row;
+                float4 v[N / 4];
+#pragma unroll
+                for (int i = 0; i < N / 4; ++i) v[i] = __ldcg(other4 + i * COLS);
+                if (l == 0.f) continue;
+                const float w = exp2_approx(t - top);
+                total = fmaf(w, l, total);
+#pragma unroll
+                for (int i = 0; i < N / 4; ++i) {
+                    out[4 * i] = fmaf(w, v[i].x, out[4 * i]), out[4 * i + 1] = fmaf(w, v[i].y, out[4 * i + 1]);
+                    out[4 * i + 2] = fmaf(w, v[i].z, out[4 * i + 2]), out[4 * i + 3] = fmaf(w, v[i].w, out[4 * i + 3]);
+                }
+            }
+            store([&](int i) { return out[i]; }, total);
+            if (tid == 0) *counter = 0;      // ready for the next launch
+        }
+    }
+    if (!alive) {      // a wait ran out: what is on its way lands before the block ends
+        if (lane == 0) atomicExch(a.status, SAL_E_TIMEOUT);
+        for (int i = 0; i < S::STAGES + 2; ++i) (void)mbar_wait(full + 8 * i, 0), (void)mbar_wait(full + 8 * i, 1);
+    }
+    __syncthreads();
+    if (warp == 0) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM));
+    }
+}
+
 // Page copies travel as kernel arguments: a captured launch needs no list in memory that somebody would have to keep.
 constexpr int MAX_PAIRS = 256;
 struct PagePairs {
@@ -1105,10 +1614,10 @@ AttnPlan attention_plan(int batch, int m, int rep, int hd) {
     const int cols = m * rep;
     AttnPlan p = {};
     p.kind = cols <= 4 ? FOUR_COLUMNS : cols <= (hd < 256 ? 8 : 32) ? EIGHT_COLUMNS : cols <= 64 && hd < 256 ? SIXTEEN_COLUMNS : MANY_COLUMNS;
-    p.cols = p.kind == FOUR_COLUMNS ? 4 : p.kind == EIGHT_COLUMNS ? 8 : p.kind == SIXTEEN_COLUMNS ? 16 : hd < 256 ? 64 : 32;
+    p.cols = p.kind == FOUR_COLUMNS ? 4 : p.kind == EIGHT_COLUMNS ? 8 : p.kind == SIXTEEN_COLUMNS ? 16 : hd < 256 ? 128 : 32;
     p.col_tiles = (cols + p.cols - 1) / p.cols;
     p.pairs = batch * p.col_tiles;
-    p.max_blocks = p.kind == MANY_COLUMNS ? 320 : 448;
+    p.max_blocks = p.kind != MANY_COLUMNS ? 448 : hd < 256 ? WIDE_BLOCKS / 2 : 320;
     return p;
 }
 
@@ -1133,13 +1642,21 @@ int launch_tiles(const AttnArgs &a, const AttnPlan &p, void *stream) {
     return sal_launch_pdl(kernel, dim3(grid), dim3(S::THREADS), S::SMEM, stream, a);
 }
 template <int HD>
+int launch_wide(const AttnArgs &a, const AttnPlan &p, void *stream) {
+    static std::atomic<bool> configured[64];
+    if (sal_allow_shared_memory(attention_wide_kernel<HD>, configured) != cudaSuccess) return SAL_E_LAUNCH;
+    return sal_launch_pdl(attention_wide_kernel<HD>, dim3((unsigned)(p.pairs * a.c.kv_heads * a.splits)), dim3(WideShape<HD>::THREADS), WideShape<HD>::SMEM, stream, a);
+}
+template <int HD>
 int launch_attention(const AttnArgs &a, const AttnPlan &p, void *stream) {
     switch (p.kind) {
         case FOUR_COLUMNS: return launch_tiles<HD, 1, true, 2, 2, 1>(a, p, stream);
         case EIGHT_COLUMNS: return launch_tiles<HD, 1, false, 2, 2, 1>(a, p, stream);
         case SIXTEEN_COLUMNS:
             if constexpr (HD < 256) return launch_tiles<HD, 2, false, 2, 2, 1>(a, p, stream);
-        default: return launch_tiles<HD, (HD < 256 ? 2 : 1), false, 1, 1, 4>(a, p, stream);
+        default:
+            if constexpr (HD < 256) return launch_wide<HD>(a, p, stream);
+            else return launch_tiles<HD, 1, false, 1, 1, 4>(a, p, stream);
     }
 }
 
@@ -1207,6 +1724,8 @@ int sal_attention_kv4_f16(const void *q, const void *pool, const int32_t *table,
     a.batch = batch, a.m = m, a.heads = heads, a.rep = heads / kv_heads;
     a.col_tiles = p.col_tiles;
     a.whole = p.pairs > MAX_LIST;
+    const int items = p.pairs * kv_heads, splits = WIDE_BLOCKS / items;
+    a.splits = splits < 1 ? 1 : splits > WIDE_SPLITS ? WIDE_SPLITS : splits;
     a.scale_log2 = scale * (1.4426950408889634f * UNIT);
     return hd == 64 ? launch_attention<64>(a, p, stream) : hd == 128 ? launch_attention<128>(a, p, stream) : launch_attention<256>(a, p, stream);
 }
