@@ -1088,6 +1088,7 @@ struct WideShape {
 };
 constexpr int WIDE_BLOCKS = 2 * 148;      // resident at once
 constexpr int WIDE_SPLITS = 32;
+constexpr float MOVE_BY = 8.f;            // 2**8 = MOVE_AT
 
 __device__ __forceinline__ void tmem_load8(float *v, uint32_t addr) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -1338,7 +1339,7 @@ __global__ void __launch_bounds__(WideShape<HD>::THREADS, 2) attention_wide_kern
         __syncwarp();
         fence_after();
         if (!taken) return;
-        if (__any_sync(0xffffffffu, f != 1.f)) {
+        if (__any_sync(0xffffffffu, f != 1.f)) {      // seldom
 #pragma unroll
             for (int i = 0; i < N / 2; ++i) acc[i] = mul(acc[i], Two(f, f));
         }
@@ -1414,11 +1415,15 @@ __global__ void __launch_bounds__(WideShape<HD>::THREADS, 2) attention_wide_kern
                 default: asm volatile("bar.sync 4, 64;" ::: "memory"); break;
             }
             top = fmaxf(ref, fmaxf(top, swap[(1 - half) * (1 + G) * COLS + row]));
-            const float from = top == -INFINITY ? 0.f : top;
-            f = ref == -INFINITY ? 1.f : exp2_approx(ref - from);
-            ref = top;
+            f = 1.f;
+            if (top > ref + MOVE_BY) {      // weights stay below MOVE_AT
+                if (ref != -INFINITY) f = exp2_approx(ref - top);
+                ref = top;
+            }
+            const float from = ref == -INFINITY ? 0.f : ref;
             back = s_back[half * N / GROUP];
-            sums = mul(sums, Two(f, f));
+            const bool moved = __any_sync(0xffffffffu, f != 1.f);
+            if (moved) sums = mul(sums, Two(f, f));
             Two low[G];
 #pragma unroll
             for (int g = 0; g < G; ++g) low[g] = Two(0.f, 0.f);
@@ -1451,7 +1456,7 @@ __global__ void __launch_bounds__(WideShape<HD>::THREADS, 2) attention_wide_kern
                             const float2 v = z.get();
                             const __half2 h = __floats2half2_rn(v.x, v.y);
                             const float2 r = __half22float2(h);
-                            const float2 rest = add(z, Two(-r.x, -r.y)).get();
+                            const float2 rest = fma(Two(r.x, r.y), Two(-1.f, -1.f), z).get();
                             hi[e] = as_u32(h), lo[e] = as_u32(__floats2half2_rn(rest.x, rest.y));
                         }
                         tmem_store8(own + 64 * g + k, hi);      // where the scores of these positions were
