@@ -1279,7 +1279,7 @@ __global__ void __launch_bounds__(WideShape<HD>::THREADS, 2) attention_wide_kern
             for (int e = 0; e < 2; ++e) {
                 const int k = lane + 32 * e;
                 x[e] = page * PAGE + k <= it.last ? __half22float2(from[R::PARAMS / 4 + k * G + g]) : make_float2(0.f, 0.f);
-                top = fmaxf(top, x[e].x);
+                if (x[e].x <= 65504.f) top = fmaxf(top, x[e].x);      // one that is not finite is for the rows that see it
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));

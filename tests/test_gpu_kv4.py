@@ -619,3 +619,66 @@ def test_queries_may_be_overwritten_by_the_outputs():
     decode_ops.attention_kv4(q, *args, out, 8, 2, 128, 0.1, ws)
     decode_ops.attention_kv4(q, *args, q, 8, 2, 128, 0.1, ws)
     assert torch.equal(q, out)
+
+
+@pytest.mark.parametrize("heads,kvh,hd,m", [(1, 1, 128, 65), (1, 1, 64, 128), (3, 1, 128, 43), (5, 1, 64, 77), (8, 2, 128, 17), (64, 1, 64, 2), (2, 2, 128, 257)])
+@pytest.mark.parametrize("far", [0, 1500])
+def test_tiles_of_many_columns(heads, kvh, hd, m, far):
+    """Up to, at and behind the end of a tile of 128 columns; with `far` an item's pages are split."""
+    rng = np.random.default_rng(m + far)
+    pos, rows = [far, 63, -2, far + 65], [m, max(1, m // 3), m, 0]
+    width = (far + 65 + m) // PAGE + 1
+    pool, table = filled(rng, 4, width, kvh, hd)
+    for b, p in enumerate(pos):
+        poison(pool, table, b, max(0, p + rows[b]), hd)
+    check_attention(rng.standard_normal((4, m, heads * hd)).astype(np.float16), pool, table, pos, rows, heads, kvh, hd)
+
+
+@pytest.mark.parametrize("spread", [1e-4, 1.0, 300.0])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_columns_of_small_and_large_numbers(hd, spread):
+    rng = np.random.default_rng(17)
+    pool, table = filled(rng, 1, 5, 2, hd, spread=spread)
+    q = (rng.standard_normal((1, 70, 2 * hd)) * 3).astype(np.float16)
+    check_attention(q, pool, table, [240], None, 2, 2, hd, scale=0.5 if spread < 1 else None)
+
+
+def test_a_later_rows_nan_in_a_tile_of_many_columns():
+    rng = np.random.default_rng(18)
+    heads, kvh, hd, m = 4, 1, 128, 40
+    pool, table = filled(rng, 1, 2, kvh, hd)
+    q = rng.standard_normal((1, m, heads * hd)).astype(np.float16)
+    clean = check_attention(q, pool, table, [50], None, heads, kvh, hd)
+    poison(pool, table, 0, 60, hd)                          # rows from 10 on see it
+    out = torch.empty(1, m, heads * hd, dtype=torch.float16, device="cuda")
+    ws = decode_ops.attention_kv4_workspace(1, m, heads, kvh, hd, "cuda")
+    decode_ops.attention_kv4(cuda(q), cuda(pool), cuda(table), torch.tensor([50]).cuda(), out, heads, kvh, hd, 1 / math.sqrt(hd), ws)
+    got = out.view(1, m, heads, hd).double().cpu().numpy()
+    assert np.isnan(got[:, 10:]).all()
+    want, bound = attention(q, filled(np.random.default_rng(18), 1, 2, kvh, hd)[0], table, [50], None, heads, kvh, hd, 1 / math.sqrt(hd))
+    assert (np.abs(got - want)[:, :10] <= bound[:, :10]).all() and np.isfinite(clean).all()
+
+
+def test_many_columns_without_some_pages():
+    rng = np.random.default_rng(19)
+    heads, kvh, hd, m = 4, 2, 128, 70
+    pool, table = filled(rng, 4, 9, kvh, hd)
+    table[0, 0], table[0, 4:6], table[1, 8], table[2] = -1, -7, 2 ** 31 - 1, pool.shape[0]
+    pos = [430, 9 * PAGE - 71, 300, 10 ** 12]                # the third sees nothing at all, the fourth all there is
+    check_attention(rng.standard_normal((4, m, heads * hd)).astype(np.float16), pool, table, pos, None, heads, kvh, hd)
+
+
+@pytest.mark.parametrize("heads,kvh,m", [(2, 1, 70), (1, 1, 65)])
+def test_the_mean_of_many_values_in_a_tile_of_many_columns(heads, kvh, m):
+    test_the_mean_of_many_values_keeps_its_digits(heads, kvh, m)
+
+
+def test_many_queries_may_be_overwritten_by_the_outputs():
+    rng = np.random.default_rng(20)
+    pool, table = filled(rng, 2, 60, 2, 128)
+    q = cuda(rng.standard_normal((2, 40, 8 * 128)).astype(np.float16))
+    args = (cuda(pool), cuda(table), torch.tensor([3700, 40], device="cuda"))
+    out, ws = torch.empty_like(q), decode_ops.attention_kv4_workspace(2, 40, 8, 2, 128, "cuda")
+    decode_ops.attention_kv4(q, *args, out, 8, 2, 128, 0.1, ws)
+    decode_ops.attention_kv4(q, *args, q, 8, 2, 128, 0.1, ws)
+    assert torch.equal(q, out)
