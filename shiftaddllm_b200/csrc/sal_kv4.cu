@@ -85,8 +85,9 @@ __device__ __forceinline__ uint8_t *record_of(const CacheArgs &c, int b, int p, 
 }
 
 // Writing and reading: a thread has eight neighbouring numbers of a head, 16 bytes of 16-bit numbers or 4 bytes of codes, HD / 8 threads a head.  The
-// other numbers of its rotary pairs are HD / 16 threads on, a group is eight threads.  Bound by bytes; what counts are wide accesses and many
-// rows in flight.  Blocks go over a sequence's rows with a stride, threads of a block over the heads of a row.
+// other numbers of its rotary pairs are HD / 16 threads on, a group is eight threads.  Writing is bound by instruction issue (conversions, the checks of
+// the rounding, shuffles; about 280 a warp and row): 27 us for 1537 rows of 64 + 8 heads of 128, 57 MB; reading them back 5.7 us; one row of 16
+// sequences 3.1 and 1.9 us, a launch's latency.  Blocks go over a sequence's rows with a stride, threads of a block over the heads of a row.
 constexpr int ROW_THREADS = 256;
 
 template <int HD>
@@ -238,6 +239,9 @@ __global__ void __launch_bounds__(ROW_THREADS) read_kv4_kernel(CacheArgs c, cons
 // themselves, from the positions on the device: texts of any lengths keep all SMs equally busy, and a captured launch follows the texts.  A
 // page of a head is one contiguous record, so its fetch is one bulk copy into a ring of shared memory.  Blocks that share an item leave
 // their part (maximum, sum, unnormalised output) in scratch; the last one to arrive adds them up in the order of the positions.
+//
+// Bound by instruction issue (about 390 a warp for 16 positions; 52 % of the issue slots, 35 % of HBM), not by bytes: 54 us for 159 MB of records
+// (16 sequences of 300 to 4000 positions, 32 heads of 128; 2.9 TB/s), 97 us for 294 MB (three of 70 to 100 thousand, 64 query and 8 kv heads).
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
@@ -380,9 +384,9 @@ struct AttnShape {
     static constexpr bool QUERIES = WC == 1;                           // an item's queries travel with its first page
     static constexpr int STAGE = REC + (QUERIES ? COLS * HD * 2 : 0);
     // What an item costs by itself (its first page's wait, the sum over the warps, the output or the part) in pages: 2.8 us against 1.2 us a page
-    // with one column and heads of 128.  Counted as 1, 2, 3, 4 pages: 63, 55, 54, 54 us for 16 sequences of 300 to 4000 positions with 32 heads;
-    // with 64 columns (512 rows behind 1536 positions, 32 heads) 134, 135, 137, 139.
-    static constexpr int ITEM_UNITS = WC == 1 ? 3 : 1;
+    // with one column and heads of 128.  Counted as 1, 2, 3, 4 pages: 63, 55, 54, 54 us for 16 sequences of 300 to 4000 positions with 32 heads; as
+    // 1 and 3 with 32 columns and heads of 256: 109 and 92 (four sequences, 33 rows behind 1000 to 5000 positions), 152 and 156 (512 rows of one).
+    static constexpr int ITEM_UNITS = 3;
     static constexpr int MIN_UNITS = ITEM_UNITS + 2;
     static constexpr int STAGES = 4;      // a power of two; so many pages on lie within 32 units, ITEM_UNITS at most being in front of each
     static constexpr int SMEM = STAGES * STAGE + MERGE + 2 * CHUNK * 8 + MAX_LIST * 4 + 16;
@@ -1075,7 +1079,9 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
 // and nothing is added up in the tensor core beyond a page.  E_g is the page's own.
 //
 // A block takes one item, or one of `splits` equal runs of its pages; the last one to arrive adds the parts up in order.  Items with the most pages are
-// launched first.  While the tensor core works for one of the two blocks of an SM the other one expands, and within a block the next page's keys are expanded
+// launched first.  Equal runs that may end inside an item, as above, cost more in parts of 128 columns and new starts than they even out: 98 us where this
+// takes 79 (512 rows behind 1536 positions, 32 heads of 128: 15 GFLOP, and half as much again for the second parts).  Bound by instruction issue and latency at
+// 16 warps an SM: 46 % of the issue slots, 1140 instructions a warp and page.  While the tensor core works for one of the two blocks of an SM the other one expands, and within a block the next page's keys are expanded
 // behind the second product's back.
 template <int HD>
 struct WideShape {
@@ -1086,8 +1092,8 @@ struct WideShape {
     static constexpr int TMEM = 2 * HD;                                // columns: D_g or weights, then outputs
     static constexpr int PART = COLS * (HD + 2);
 };
-constexpr int WIDE_BLOCKS = 2 * 148;      // resident at once
-constexpr int WIDE_SPLITS = 32;
+constexpr int WIDE_BLOCKS = 2 * 148;      // resident at once: two of 100 KB and 128 registers a thread on an SM
+constexpr int WIDE_SPLITS = 32;           // one block adds the parts up
 constexpr float MOVE_BY = 8.f;            // 2**8 = MOVE_AT
 
 __device__ __forceinline__ void tmem_load8(float *v, uint32_t addr) {
@@ -1578,7 +1584,7 @@ __global__ void __launch_bounds__(WideShape<HD>::THREADS, 2) attention_wide_kern
     }
 }
 
-// Page copies travel as kernel arguments: a captured launch needs no list in memory that somebody would have to keep.
+// Bound by HBM: 44.1 us for 15 pages of 32 layers, 283 MB read and written, 98 % of the copy rate.  Page copies travel as kernel arguments: a captured launch needs no list in memory that somebody would have to keep.
 constexpr int MAX_PAIRS = 256;
 struct PagePairs {
     int src[MAX_PAIRS], dst[MAX_PAIRS];
@@ -1615,6 +1621,11 @@ struct AttnPlan {
     int pairs;         // (sequence, column tile) pairs
     int max_blocks;    // thread blocks that share the list
 };
+// Columns of a sequence that share a kv head decide.  The tile's width is what a page's codes are expanded for, so it follows the columns up to what the registers
+// hold (16 for heads below 256, 8 for those).  Behind 64 columns the fifth generation's tensor cores take over, in tiles of 128: 79 us against
+// 134 in tiles of 64 on the older path (512 rows behind 1536 positions, 32 heads of 128), 64 against 115 (4 sequences, 128 columns, 1000 to 6000 positions),
+// 26 against 65 (66 columns behind 2000); for 64 columns and fewer tiles of 16 are the faster ones: 206 against 225 (64 rows, 8 sequences), 40 against 72 (up to
+// 40 columns, 6 sequences).  Heads of 256 would need all of the tensor memory and stay on the older path, in tiles of 32.
 AttnPlan attention_plan(int batch, int m, int rep, int hd) {
     const int cols = m * rep;
     AttnPlan p = {};
