@@ -252,6 +252,7 @@ class BcqLlamaDecoder:
         """Captures `step` in a CUDA graph (one eager warm-up step first: it sizes the workspace and
         runs the library's one-off probes, which must not happen under capture)."""
         stream = torch.cuda.Stream(self.device)
+        stream.wait_stream(torch.cuda.current_stream(self.device))      # which may still be at the weights, the token or its position
         with torch.cuda.stream(stream):
             saved = (self.token.clone(), self.pos.clone())
             self.step()

@@ -237,6 +237,7 @@ class ColumnParallelDecoder:
         """Captures `step` in a CUDA graph (after one eager warm-up step, which sizes the scratch buffers and
         runs the library's one-off probes; all ranks must call this together)."""
         stream = torch.cuda.Stream(self.device)
+        stream.wait_stream(torch.cuda.current_stream(self.device))      # which may still be at the weights, the token or its position
         with torch.cuda.stream(stream):
             saved = (self.token.clone(), self.pos.clone(), self._slot)
             self.step()

@@ -1,0 +1,52 @@
+"""A step is captured on a stream of its own, which has to wait for what the caller's stream still does to the state."""
+import contextlib
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from shiftaddllm_b200 import decoder, shard_decoder
+
+
+@pytest.fixture()
+def log(monkeypatch):
+    """The calls of a capture, in order, on a host without a GPU."""
+    seen, current = [], object()
+
+    class Stream:
+        def __init__(self, device=None):
+            self.cuda_stream = 1
+
+        def wait_stream(self, other):
+            seen.append("wait" if other is current else "wait for another stream")
+
+    @contextlib.contextmanager
+    def on(name):
+        seen.append(name)
+        yield
+
+    monkeypatch.setattr(torch.cuda, "Stream", Stream)
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: on("side stream"))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: current)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: seen.append("synchronize"))
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", object)
+    monkeypatch.setattr(torch.cuda, "graph", lambda g, stream=None: on("capture"))
+    return seen
+
+
+def state(log, **more):
+    return SimpleNamespace(device=torch.device("cpu"), token=torch.zeros(1), pos=torch.zeros(1), step=lambda: log.append("step"), **more)
+
+
+def in_order(log):
+    assert log[:3] == ["wait", "side stream", "step"] and log[-1] == "synchronize" and log.count("step") == 2
+
+
+def test_decoder(log):
+    decoder.BcqLlamaDecoder.capture(state(log))
+    in_order(log)
+
+
+def test_column_parallel_decoder(log):
+    shard_decoder.ColumnParallelDecoder.capture(state(log, _slot=0, blocks=[None] * shard_decoder.NSLOTS))
+    in_order(log)

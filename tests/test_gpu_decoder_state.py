@@ -1,0 +1,43 @@
+"""The state of the batch decoder's sequences between its calls: tokens, positions, pages and lengths stay in step, whatever is called next."""
+import pytest
+import torch
+
+from shiftaddllm_b200.decoder import SHAPES, BcqLlamaBatchDecoder, BcqLlamaDecoder
+
+pytestmark = pytest.mark.gpu
+BATCH = 3
+
+
+@pytest.fixture(scope="module")
+def like():
+    return BcqLlamaDecoder(SHAPES["tiny"], max_len=8, seed=3, fused=False)
+
+
+def make(like, bits=4, **kw):
+    return BcqLlamaBatchDecoder(SHAPES["tiny"], max_len=300, batch=BATCH, like=like, cache_bits=bits, **kw)
+
+
+def prompts(lengths, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, 1000, (n,), generator=g).tolist() for n in lengths]
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_capture_behind_work_that_is_still_in_flight(like, bits):
+    """The caller's stream is a tenth of a second behind when the step is captured."""
+    rows = torch.tensor(prompts([9] * BATCH, seed=1)).t()
+    forced = torch.tensor([11, 500, 999], device="cuda")
+    eager, captured = make(like, bits), make(like, bits)
+    for m in (eager, captured):
+        if bits == 4:
+            m.prefill(prompts([5, 130, 70]))
+        m.token.zero_()
+        torch.cuda.synchronize()
+        if m is captured:
+            torch.cuda._sleep(200_000_000)
+        m.feed(rows)
+        m.token.copy_(forced)
+        if m is captured:
+            m.capture()
+    assert torch.equal(captured.generate(8), eager.generate(8)) and torch.equal(captured.logits, eager.logits)
+    assert torch.equal(captured.pos, eager.pos)
