@@ -321,6 +321,7 @@ class Timer:
         torch.cuda.synchronize(self.device)
 
     def capture(self, one_step):
+        self.stream.wait_stream(torch.cuda.current_stream(self.device))      # which made what the step reads
         with torch.cuda.stream(self.stream):
             one_step()                       # also sizes the workspace and runs the one-off probes
             torch.cuda.synchronize(self.device)

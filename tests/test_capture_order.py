@@ -5,6 +5,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
+import bench
 from shiftaddllm_b200 import decoder, shard_decoder
 
 
@@ -29,7 +30,7 @@ def log(monkeypatch):
     monkeypatch.setattr(torch.cuda, "stream", lambda s: on("side stream"))
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: current)
     monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: seen.append("synchronize"))
-    monkeypatch.setattr(torch.cuda, "CUDAGraph", object)
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", lambda: SimpleNamespace(replay=None))
     monkeypatch.setattr(torch.cuda, "graph", lambda g, stream=None: on("capture"))
     return seen
 
@@ -50,3 +51,10 @@ def test_decoder(log):
 def test_column_parallel_decoder(log):
     shard_decoder.ColumnParallelDecoder.capture(state(log, _slot=0, blocks=[None] * shard_decoder.NSLOTS))
     in_order(log)
+
+
+def test_the_benchmark_s_steps(log):
+    args = SimpleNamespace(warmup=3)
+    timer = bench.Timer(args, torch.device("cpu"), 1, torch.cuda.Stream())
+    timer.capture(lambda: log.append("step"))
+    assert log[:3] == ["wait", "side stream", "step"] and log.count("step") == 2
