@@ -299,6 +299,14 @@ def attention_kv4(q, pool, table, pos, out, heads, kv_heads, hd, scale: float, w
                                              pages, float(scale), workspace.data_ptr(), workspace.numel(), _stream(q)), "sal_attention_kv4_f16")
 
 
+def attention_kv4_check(workspace):
+    """Waits for the current stream; RuntimeError if a wait of an attention_kv4 call with this workspace ran out since the last look.  That call went
+    on without the pages that it waited for, so its outputs, and all that was made of them, are wrong."""
+    lib = _lib.load()
+    with _on(workspace.device):
+        _lib.check(lib.sal_workspace_status(workspace.data_ptr(), _stream(workspace)), "attention_kv4 on the device")
+
+
 def copy_kv4_pages(pool, src, dst):
     """Page dst[i] of `pool` (uint8 [layers, pages, ..]) becomes a copy of page src[i], in every layer.  src and dst are sequences of whole
     numbers on the host; no page may be written twice, or written and read in the same call."""

@@ -543,6 +543,11 @@ class BcqLlamaBatchDecoder:
         if self.cache_bits == 4:
             self.lengths = [n + 1 for n in self.lengths]
 
+    def _check_attention(self):
+        """RuntimeError if the steps so far met a device-side wait that ran out (4-bit cache; once per call, since it waits for the device)."""
+        if self.cache_bits == 4:
+            decode_ops.attention_kv4_check(self._attn_ws)
+
     def feed(self, token_rows):
         """Teacher-forced pass over prompts of equal length: `token_rows` [length][batch] token ids."""
         if self.cache_bits == 4:
@@ -550,6 +555,7 @@ class BcqLlamaBatchDecoder:
         for row in token_rows:
             self.token.copy_(torch.as_tensor(row, dtype=torch.long, device=self.device))
             self._run()
+        self._check_attention()
 
     def generate(self, n, u=None):
         """n steps; the tokens [n, batch].  Where tokens are sampled, `u` [n, batch] are the random numbers, in [0, 1)."""
@@ -561,6 +567,7 @@ class BcqLlamaBatchDecoder:
         for i in range(n):
             self._run(None if u is None else u[i])
             out.append(self.token.clone())
+        self._check_attention()
         return torch.stack(out)                                          # [n, batch]
 
     def fork(self, src: int, dst: int) -> None:
@@ -625,6 +632,7 @@ class BcqLlamaBatchDecoder:
                 at = torch.tensor(ends, device=dev)
                 last[at] = x.view(self.batch, m, h)[at, torch.tensor([counts[b] - c0 - 1 for b in ends], device=dev)]
             pos += rows
+        decode_ops.attention_kv4_check(ws)      # nothing of the sequences' state has changed yet
         hn = F.rms_norm(last, (h,), self.final_norm, s.eps)
         some = torch.tensor([c > 0 for c in counts], device=dev)
         token, logits = self.token.clone(), self.logits.clone()

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from shiftaddllm_b200 import _lib, decode_ops
 from shiftaddllm_b200.decoder import SHAPES, BcqLlamaBatchDecoder, BcqLlamaDecoder
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +42,15 @@ def test_capture_behind_work_that_is_still_in_flight(like, bits):
             m.capture()
     assert torch.equal(captured.generate(8), eager.generate(8)) and torch.equal(captured.logits, eager.logits)
     assert torch.equal(captured.pos, eager.pos)
+
+
+def test_a_wait_that_ran_out_is_reported_once(like):
+    """The device's word, written here as a kernel writes it."""
+    model = make(like)
+    model.prefill(prompts([5, 130, 70]))
+    for call in (lambda: model.generate(2), lambda: model.feed([[1, 2, 3]])):
+        model._attn_ws[:4].view(torch.int32).fill_(_lib.SAL_E_TIMEOUT)
+        with pytest.raises(RuntimeError, match="wait"):
+            call()
+        call()
+    decode_ops.attention_kv4_check(model._attn_ws)
