@@ -529,11 +529,10 @@ class BcqLlamaBatchDecoder:
         self.v_cache.zero_()
 
     def _make_room(self, n: int) -> None:
-        """Pages for the next n positions of every sequence (4-bit cache)."""
-        for b, length in enumerate(self.lengths):
-            if length + n > self.max_len:
-                raise ValueError("the sequence does not fit the KV cache")
-            self.cache.reserve(b, length, length + n)
+        """Pages for the next n positions of every sequence (4-bit cache), or an error and nothing changed."""
+        if any(length + n > self.max_len for length in self.lengths):
+            raise ValueError("the sequence does not fit the KV cache")
+        self.cache.reserve_all([(b, length, length + n) for b, length in enumerate(self.lengths)])
 
     def _run(self, u=None):
         """One step (graph replay) with its random numbers."""
@@ -594,8 +593,7 @@ class BcqLlamaBatchDecoder:
             raise ValueError("prompt does not fit the KV cache")
         if not any(counts):
             return
-        for b, c in enumerate(counts):
-            self.cache.reserve(b, self.lengths[b], self.lengths[b] + c)
+        self.cache.reserve_all([(b, n, n + c) for b, (n, c) in enumerate(zip(self.lengths, counts))])
         hd, kvh, h, dev = s.head_dim, s.kv_heads, s.hidden, self.device
         limit = lutgemm._lib.SAL_MAX_M if any(l.wbit > 4 for blk in self.blocks for l in blk.linears().values()) else BcqLlamaDecoder.PREFILL_ROWS
         m = min(max(counts), max(1, limit // self.batch))

@@ -62,23 +62,54 @@ class Kv4Cache:
     def reserve(self, slot: int, first: int, last: int) -> None:
         """Makes positions first .. last - 1 of a sequence writable: pages it lacks are added, pages it shares with others in that range are
         replaced by copies.  RuntimeError, and nothing changed, where there are not enough free pages."""
-        if not 0 <= first <= last <= self.max_len:
-            raise ValueError(f"positions {first} .. {last} of {self.max_len}")
-        mine = self._of[slot]
-        if first > len(mine) * PAGE:
-            raise ValueError(f"position {first} lies behind the sequence's {len(mine)} pages")
-        need = -(-last // PAGE)
-        shared = [i for i in range(first // PAGE, min(need, len(mine))) if self._users[mine[i]] > 1] if last > first else []
-        more = max(0, need - len(mine))
-        if not shared and not more:
+        self.reserve_all([(slot, first, last)])
+
+    def reserve_all(self, ranges) -> None:
+        """:meth:`reserve` for several sequences, `ranges` of (slot, first, last): all of them, or none."""
+        plan, users, need, slots = [], {}, 0, set()
+        for slot, first, last in ranges:
+            if not 0 <= first <= last <= self.max_len:
+                raise ValueError(f"positions {first} .. {last} of {self.max_len}")
+            mine = self._of[slot]
+            if first > len(mine) * PAGE:
+                raise ValueError(f"position {first} lies behind the sequence's {len(mine)} pages")
+            if slot in slots:
+                raise ValueError(f"sequence {slot} stands in the list twice")
+            slots.add(slot)
+            width = -(-last // PAGE)
+            shared = []
+            for i in range(first // PAGE, min(width, len(mine))) if last > first else ():
+                left = users.get(mine[i], self._users[mine[i]])      # the last of its users keeps the page
+                if left > 1:
+                    shared.append(i)
+                    users[mine[i]] = left - 1
+            more = max(0, width - len(mine))
+            plan.append((slot, shared, more))
+            need += len(shared) + more
+        if need == 0:
             return
-        got = self._take(len(shared) + more)
-        decode_ops.copy_kv4_pages(self.pool, [mine[i] for i in shared], got[:len(shared)])
-        for i, p in zip(shared, got):
-            self._drop(mine[i])
-            mine[i] = p
-        mine += got[len(shared):]
-        self._publish(slot)
+        got = self._take(need)
+        into, src, dst = iter(got), [], []
+        new = {}
+        for slot, shared, more in plan:
+            pages = new[slot] = list(self._of[slot])
+            for i in shared:
+                src.append(pages[i])
+                pages[i] = next(into)
+                dst.append(pages[i])
+            pages += [next(into) for _ in range(more)]
+        try:
+            decode_ops.copy_kv4_pages(self.pool, src, dst)
+        except BaseException:
+            for p in got:
+                self._drop(p)
+            raise
+        for p in src:
+            self._drop(p)
+        changed = [slot for slot, shared, more in plan if shared or more]
+        for slot in changed:
+            self._of[slot] = new[slot]
+        self._publish(*changed)
 
     def fork(self, src: int, dst: int) -> None:
         """Sequence `dst` (whose own pages are given up) becomes one with `src`'s positions; the pages are shared until one of them writes."""

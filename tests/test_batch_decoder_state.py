@@ -72,3 +72,61 @@ def test_the_check_reads_the_workspace_s_status(lib, monkeypatch):
     with pytest.raises(RuntimeError, match="status"):
         decode_ops.attention_kv4_check(ws)
     decode_ops.attention_kv4_check(ws)
+
+
+def test_a_refused_prompt_takes_no_pages(make):
+    model = make(pages=4)
+    before = state(model)
+    with pytest.raises(RuntimeError):
+        model.prefill([[1] * 200, [2] * 100, []])      # six pages
+    assert state(model) == before
+    model.prefill([[], [2] * 100, []])
+    assert model.lengths == [0, 100, 0] and model.cache.free_pages == 2
+    model.prefill([[1] * 64, [], []])
+    for call in (lambda: model.generate(1), lambda: model.feed([[1, 2, 3]]), model.capture):      # two sequences need a page, one is left
+        before = state(model)
+        with pytest.raises(RuntimeError):
+            call()
+        assert state(model) == before
+
+
+def test_a_full_sequence_takes_no_pages_of_the_others(make):
+    model = make(max_len=130)
+    model.prefill([[1] * 10, [2] * 64, [3] * 130])
+    before = state(model)
+    for call in (lambda: model.generate(1), lambda: model.prefill([[], [1], [1]])):
+        with pytest.raises(ValueError):
+            call()
+        assert state(model) == before
+
+
+def test_pages_for_several_sequences_or_for_none(make):
+    cache = make(pages=6).cache
+    cache.reserve(0, 0, 130)
+    cache.fork(0, 1), cache.fork(0, 2)
+    used = lambda: (cache.free_pages, [cache.pages_of(b) for b in range(BATCH)], list(cache._users))
+    before = used()
+    for bad in ([(0, 130, 140), (1, 130, 140), (2, 100, 193)],      # three copies and a page
+                [(0, 130, 131), (0, 131, 132)], [(0, 130, 131), (1, 193, 194)], [(0, 130, 131), (1, 5, 301)]):
+        with pytest.raises((RuntimeError, ValueError)):
+            cache.reserve_all(bad)
+        assert used() == before
+    cache.pool[0, :, 0, 0] = torch.arange(6, dtype=torch.uint8)
+    cache.reserve_all([(0, 130, 140), (1, 100, 140), (2, 130, 140)])      # the last of them keeps the third page; 1 has a second one of its own
+    assert cache.pages_of(2) == before[1][2] and cache.free_pages == 0 and [cache._users[p] for p in before[1][0]] == [3, 2, 1]
+    for b in range(BATCH):
+        assert [int(cache.pool[0, p, 0, 0]) for p in cache.pages_of(b)] == [0, 1, 2]
+        assert cache.table[b].tolist() == cache.pages_of(b) + [-1, -1]
+
+
+def test_pages_are_given_back_if_they_cannot_be_copied(make, monkeypatch):
+    def fails(pool, src, dst):
+        raise RuntimeError("no copy")
+
+    cache = make(pages=5).cache
+    cache.reserve(0, 0, 130)
+    cache.fork(0, 1)
+    monkeypatch.setattr(decode_ops, "copy_kv4_pages", fails)
+    with pytest.raises(RuntimeError, match="no copy"):
+        cache.reserve(1, 130, 131)
+    assert cache.free_pages == 2 and cache.pages_of(1) == cache.pages_of(0) and [cache._users[p] for p in cache.pages_of(0)] == [2, 2, 2]
