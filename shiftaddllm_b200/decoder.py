@@ -542,24 +542,32 @@ class BcqLlamaBatchDecoder:
         if self.cache_bits == 4:
             self.lengths = [n + 1 for n in self.lengths]
 
+    @staticmethod
+    def _check_numbers(u, shape):
+        if u is None or tuple(u.shape) != shape:
+            raise ValueError(f"sampling needs random numbers u {list(shape)}")
+
     def _check_attention(self):
         """RuntimeError if the steps so far met a device-side wait that ran out (4-bit cache; once per call, since it waits for the device)."""
         if self.cache_bits == 4:
             decode_ops.attention_kv4_check(self._attn_ws)
 
-    def feed(self, token_rows):
-        """Teacher-forced pass over prompts of equal length: `token_rows` [length][batch] token ids."""
+    def feed(self, token_rows, u=None):
+        """Teacher-forced pass over prompts of equal length: `token_rows` [length][batch] token ids.  Where tokens are sampled, the ones behind the
+        last row are drawn with `u` [batch]."""
+        if len(token_rows) and self.sampling is not None:
+            self._check_numbers(u, (self.batch,))
         if self.cache_bits == 4:
             self._make_room(len(token_rows))
-        for row in token_rows:
+        for i, row in enumerate(token_rows):
             self.token.copy_(torch.as_tensor(row, dtype=torch.long, device=self.device))
-            self._run()
+            self._run(u if i + 1 == len(token_rows) else None)
         self._check_attention()
 
     def generate(self, n, u=None):
         """n steps; the tokens [n, batch].  Where tokens are sampled, `u` [n, batch] are the random numbers, in [0, 1)."""
-        if self.sampling is not None and (u is None or tuple(u.shape) != (n, self.batch)):
-            raise ValueError("sampling needs random numbers u [n, batch]")
+        if self.sampling is not None:
+            self._check_numbers(u, (n, self.batch))
         if self.cache_bits == 4:
             self._make_room(n)
         out = []
@@ -586,8 +594,8 @@ class BcqLlamaBatchDecoder:
             raise RuntimeError("prompts of different lengths need cache_bits=4")
         if len(prompts) != self.batch:
             raise ValueError(f"{self.batch} prompts are needed, got {len(prompts)}")
-        if self.sampling is not None and u is None:
-            raise ValueError("sampling needs random numbers u [batch]")
+        if self.sampling is not None:
+            self._check_numbers(u, (self.batch,))
         counts = [len(p) for p in prompts]
         if any(n + c > self.max_len for n, c in zip(self.lengths, counts)):
             raise ValueError("prompt does not fit the KV cache")
@@ -656,7 +664,7 @@ def benchmark_batch(model: BcqLlamaBatchDecoder, prompt_len: int, new_tokens: in
         model.prefill(prompts.t().tolist(), u=model.u)
         model._make_room(max(warmup, new_tokens))
     else:
-        model.feed(prompts)
+        model.feed(prompts, u=model.u)
     torch.cuda.synchronize(dev)
     state = (model.token.clone(), model.pos.clone())
     for _ in range(warmup):

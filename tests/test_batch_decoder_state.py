@@ -130,3 +130,38 @@ def test_pages_are_given_back_if_they_cannot_be_copied(make, monkeypatch):
     with pytest.raises(RuntimeError, match="no copy"):
         cache.reserve(1, 130, 131)
     assert cache.free_pages == 2 and cache.pages_of(1) == cache.pages_of(0) and [cache._users[p] for p in cache.pages_of(0)] == [2, 2, 2]
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_fed_prompts_draw_with_their_own_numbers(make, bits):
+    rows, u = [[1, 2, 3], [4, 5, 6]], torch.rand(6, BATCH, generator=torch.Generator().manual_seed(1))
+
+    def drawn(before):
+        model = make(cache_bits=bits)
+        model.set_sampling(0.9)
+        if before:
+            model.feed([[7, 8, 9]], u=u[4])
+            model.generate(1, u=u[5:])
+        model.feed(rows, u=u[0])
+        return torch.cat((model.token[None].clone(), model.generate(3, u=u[1:4])))
+
+    first = drawn(False)
+    assert torch.equal(first, drawn(True)) and torch.equal(first[0], (u[0] * VOCAB).long())
+    model = make(cache_bits=bits)
+    model.set_sampling(0.9)
+    for bad in (None, u, u[0, :2]):
+        with pytest.raises(ValueError):
+            model.feed(rows, u=bad)
+    model.feed([])
+    model.set_sampling(None)
+    model.feed(rows)
+
+
+def test_numbers_are_looked_at_before_a_prompt_takes_pages(make):
+    model = make()
+    model.set_sampling(0.9)
+    before = state(model)
+    for bad in (None, torch.rand(2), torch.rand(1, BATCH)):
+        with pytest.raises(ValueError):
+            model.prefill([[1], [2], [3]], u=bad)
+    assert state(model) == before
