@@ -87,6 +87,26 @@ def _group(lins, x, outs, pdl=True, x_mul=None, atomic=False, swiglu_fixed=False
     lutgemm.lutgemv_grouped(probs, pdl=pdl, atomic_fixed=atomic, swiglu_fixed=swiglu_fixed, many_rows=many_rows)
 
 
+def _capture(model, step):
+    """`step` as a CUDA graph, behind one eager call of it; the model's token and position are put back."""
+    stream = torch.cuda.Stream(model.device)
+    stream.wait_stream(torch.cuda.current_stream(model.device))      # which may still be at the weights, the token or its position
+    with torch.cuda.stream(stream):
+        saved = (model.token.clone(), model.pos.clone())
+        step()
+        torch.cuda.synchronize(model.device)
+        model.token.copy_(saved[0])
+        model.pos.copy_(saved[1])
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            step()
+        model.token.copy_(saved[0])
+        model.pos.copy_(saved[1])
+    torch.cuda.synchronize(model.device)
+    model.graph, model._stream = g, stream
+    return g
+
+
 class BcqLlamaDecoder:
     """Greedy batch-1 decoder with a static KV cache of `max_len` positions."""
 
@@ -251,22 +271,7 @@ class BcqLlamaDecoder:
     def capture(self):
         """Captures `step` in a CUDA graph (one eager warm-up step first: it sizes the workspace and
         runs the library's one-off probes, which must not happen under capture)."""
-        stream = torch.cuda.Stream(self.device)
-        stream.wait_stream(torch.cuda.current_stream(self.device))      # which may still be at the weights, the token or its position
-        with torch.cuda.stream(stream):
-            saved = (self.token.clone(), self.pos.clone())
-            self.step()
-            torch.cuda.synchronize(self.device)
-            self.token.copy_(saved[0])
-            self.pos.copy_(saved[1])
-            g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g, stream=stream):
-                self.step()
-            self.token.copy_(saved[0])
-            self.pos.copy_(saved[1])
-        torch.cuda.synchronize(self.device)
-        self.graph, self._stream = g, stream
-        return g
+        return _capture(self, self.step)
 
     def reset(self, first_token: int = 0):
         self.token.fill_(first_token)
@@ -482,6 +487,14 @@ class BcqLlamaBatchDecoder:
         self.pos.add_(1)
 
     def step(self):
+        """One step of every sequence, without the graph.  On a 4-bit cache it makes room for its position first (ValueError or RuntimeError, and nothing
+        done, where there is none)."""
+        if self.cache_bits == 4:
+            self._make_room(1)
+        self._step()
+        self._count()
+
+    def _step(self):
         if self.fused:
             return self._step_fused()
         s, b = self.shape, self.batch
@@ -510,10 +523,11 @@ class BcqLlamaBatchDecoder:
         self.pos.add_(1)
 
     def capture(self):
-        """As :meth:`BcqLlamaDecoder.capture`; the warm-up step of a 4-bit cache writes one position of every sequence."""
+        """As :meth:`BcqLlamaDecoder.capture`; the warm-up step of a 4-bit cache writes one position of every sequence.  `generate` and `feed` replay the
+        graph and see to the pages; whoever replays it by other ways reserves them and counts `lengths`."""
         if self.cache_bits == 4:
             self._make_room(1)
-        return BcqLlamaDecoder.capture(self)
+        return _capture(self, self._step)
 
     generate_step = step
 
@@ -538,7 +552,10 @@ class BcqLlamaBatchDecoder:
         """One step (graph replay) with its random numbers."""
         if self.sampling is not None and u is not None:
             self.u.copy_(u)
-        (self.graph.replay if self.graph is not None else self.step)()
+        (self.graph.replay if self.graph is not None else self._step)()
+        self._count()
+
+    def _count(self):
         if self.cache_bits == 4:
             self.lengths = [n + 1 for n in self.lengths]
 
@@ -666,19 +683,21 @@ def benchmark_batch(model: BcqLlamaBatchDecoder, prompt_len: int, new_tokens: in
     else:
         model.feed(prompts, u=model.u)
     torch.cuda.synchronize(dev)
-    state = (model.token.clone(), model.pos.clone())
+    state, lengths = (model.token.clone(), model.pos.clone()), model.lengths
     for _ in range(warmup):
-        model.graph.replay()
+        model._run()
     model.token.copy_(state[0])
     model.pos.copy_(state[1])
+    model.lengths = lengths
     torch.cuda.synchronize(dev)
     t0 = time.perf_counter()
     for _ in range(new_tokens):
         if model.sampling is not None:
             model.u.uniform_()
-        model.graph.replay()
+        model._run()
     torch.cuda.synchronize(dev)
     wall = time.perf_counter() - t0
+    model._check_attention()
     return {"tokens_per_s": model.batch * new_tokens / wall, "ms_per_step": 1e3 * wall / new_tokens, "batch": model.batch,
             "prompt_len": prompt_len, "new_tokens": new_tokens}
 

@@ -165,3 +165,30 @@ def test_numbers_are_looked_at_before_a_prompt_takes_pages(make):
         with pytest.raises(ValueError):
             model.prefill([[1], [2], [3]], u=bad)
     assert state(model) == before
+
+
+@pytest.mark.parametrize("name", ["step", "generate_step"])
+def test_single_steps_make_room_and_count(make, name):
+    model = make(pages=7)
+    model.prefill([[1] * 63, [2] * 130, [3] * 20])      # 1 + 3 + 1 pages
+    model.fork(0, 2)
+    for i in range(2):
+        getattr(model, name)()
+        assert model.lengths == model.pos.tolist() == [64 + i, 131 + i, 64 + i]
+        pages = [model.cache.pages_of(b) for b in range(BATCH)]
+        assert not set(pages[0]) & set(pages[2]) and [len(p) for p in pages] == [1 + i, 3, 1 + i]      # position 63, then 64
+    assert model.cache.free_pages == 0
+    model.lengths = [64, 192, 64]      # the fourth page of the second one
+    model.pos.copy_(torch.tensor(model.lengths))
+    before = state(model)
+    with pytest.raises(RuntimeError):
+        getattr(model, name)()
+    assert state(model) == before
+
+
+def test_a_graph_s_replays_count_too(make, monkeypatch):
+    model = make()
+    model.prefill([[1], [2, 3], []])
+    model.graph = SimpleNamespace(replay=model._step)
+    model.generate(2), model.feed([[1, 2, 3]])
+    assert model.lengths == model.pos.tolist() == [4, 5, 3]

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from shiftaddllm_b200 import _lib, decode_ops
-from shiftaddllm_b200.decoder import SHAPES, BcqLlamaBatchDecoder, BcqLlamaDecoder
+from shiftaddllm_b200.decoder import SHAPES, BcqLlamaBatchDecoder, BcqLlamaDecoder, benchmark_batch
 
 pytestmark = pytest.mark.gpu
 BATCH = 3
@@ -54,3 +54,28 @@ def test_a_wait_that_ran_out_is_reported_once(like):
             call()
         call()
     decode_ops.attention_kv4_check(model._attn_ws)
+
+
+def test_single_steps_are_what_generate_does(like):
+    """Over a page's end and on forked sequences, whose common page neither may write to."""
+    stepped, at_once = make(like), make(like)
+    for m in (stepped, at_once):
+        m.prefill(prompts([60, 125, 3]))
+        m.fork(0, 2)
+        m.token[2] = 77
+    want = at_once.generate(12)
+    got = []
+    for _ in range(12):
+        stepped.step()
+        got.append(stepped.token.clone())
+    assert torch.equal(torch.stack(got), want) and torch.equal(stepped.logits, at_once.logits) and stepped.lengths == stepped.pos.tolist()
+
+
+def test_generating_behind_the_benchmark(like):
+    model, fresh = make(like), make(like)
+    benchmark_batch(model, 60, 8)
+    assert model.lengths == model.pos.tolist() == [68] * BATCH
+    ids = torch.randint(0, 1000, (60, BATCH), generator=torch.Generator().manual_seed(0))      # its prompts
+    fresh.prefill(ids.t().tolist())
+    fresh.generate(8)
+    assert torch.equal(model.generate(6), fresh.generate(6)) and torch.equal(model.logits, fresh.logits)
