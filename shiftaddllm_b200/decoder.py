@@ -564,6 +564,12 @@ class BcqLlamaBatchDecoder:
         if u is None or tuple(u.shape) != shape:
             raise ValueError(f"sampling needs random numbers u {list(shape)}")
 
+    def _check_ids(self, rows):
+        """An id outside the vocabulary would be a fault of the device, which ends the process's use of it."""
+        for row in rows:
+            if row.numel() and not 0 <= int(row.min()) <= int(row.max()) < self.shape.vocab:
+                raise ValueError(f"token ids must be 0 .. {self.shape.vocab - 1}")
+
     def _check_attention(self):
         """RuntimeError if the steps so far met a device-side wait that ran out (4-bit cache; once per call, since it waits for the device)."""
         if self.cache_bits == 4:
@@ -572,12 +578,14 @@ class BcqLlamaBatchDecoder:
     def feed(self, token_rows, u=None):
         """Teacher-forced pass over prompts of equal length: `token_rows` [length][batch] token ids.  Where tokens are sampled, the ones behind the
         last row are drawn with `u` [batch]."""
-        if len(token_rows) and self.sampling is not None:
+        token_rows = [torch.as_tensor(row, dtype=torch.long) for row in token_rows]
+        self._check_ids(token_rows)
+        if token_rows and self.sampling is not None:
             self._check_numbers(u, (self.batch,))
         if self.cache_bits == 4:
             self._make_room(len(token_rows))
         for i, row in enumerate(token_rows):
-            self.token.copy_(torch.as_tensor(row, dtype=torch.long, device=self.device))
+            self.token.copy_(row)
             self._run(u if i + 1 == len(token_rows) else None)
         self._check_attention()
 
@@ -613,9 +621,11 @@ class BcqLlamaBatchDecoder:
             raise ValueError(f"{self.batch} prompts are needed, got {len(prompts)}")
         if self.sampling is not None:
             self._check_numbers(u, (self.batch,))
+        prompts = [torch.as_tensor(p, dtype=torch.long, device="cpu") for p in prompts]
         counts = [len(p) for p in prompts]
         if any(n + c > self.max_len for n, c in zip(self.lengths, counts)):
             raise ValueError("prompt does not fit the KV cache")
+        self._check_ids(prompts)
         if not any(counts):
             return
         self.cache.reserve_all([(b, n, n + c) for b, (n, c) in enumerate(zip(self.lengths, counts))])
@@ -626,7 +636,7 @@ class BcqLlamaBatchDecoder:
         ws = decode_ops.attention_kv4_workspace(self.batch, m, s.heads, kvh, hd, dev)
         ids = torch.zeros(self.batch, -(-max(counts) // m) * m, dtype=torch.long)
         for b, p in enumerate(prompts):
-            ids[b, :counts[b]] = torch.as_tensor(p, dtype=torch.long)
+            ids[b, :counts[b]] = p
         ids, pos = ids.to(dev), self.pos.clone()
         last = torch.zeros(self.batch, h, **f16)
         for c0 in range(0, max(counts), m):

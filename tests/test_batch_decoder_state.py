@@ -192,3 +192,16 @@ def test_a_graph_s_replays_count_too(make, monkeypatch):
     model.graph = SimpleNamespace(replay=model._step)
     model.generate(2), model.feed([[1, 2, 3]])
     assert model.lengths == model.pos.tolist() == [4, 5, 3]
+
+
+def test_ids_outside_the_vocabulary_are_refused(make):
+    model = make()
+    before = state(model)
+    for bad in (-1, VOCAB, 1 << 40):
+        for call in (lambda: model.prefill([[1], [2, bad], [3]]), lambda: model.feed([[1, 2, 3], [1, 2, bad]]), lambda: model.feed(torch.tensor([[1, bad, 3]]))):
+            with pytest.raises(ValueError, match="49"):
+                call()
+            assert state(model) == before
+    model.prefill([[0], torch.tensor([VOCAB - 1]), torch.tensor([], dtype=torch.int64)])
+    model.feed(torch.tensor([[1, 2, 3]]))
+    assert model.lengths == [2, 2, 1]
