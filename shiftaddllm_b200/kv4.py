@@ -39,7 +39,12 @@ class Kv4Cache:
         return len(self._free)
 
     def pages_of(self, slot: int) -> list[int]:
-        return list(self._of[slot])
+        return list(self._pages(slot))
+
+    def _pages(self, slot: int) -> list[int]:
+        if not 0 <= slot < len(self._of):      # a list would count negative ones from its end: two names for one sequence
+            raise ValueError(f"there is no sequence {slot} of {len(self._of)}")
+        return self._of[slot]
 
     def _take(self, n: int) -> list[int]:
         if n > len(self._free):
@@ -70,7 +75,7 @@ class Kv4Cache:
         for slot, first, last in ranges:
             if not 0 <= first <= last <= self.max_len:
                 raise ValueError(f"positions {first} .. {last} of {self.max_len}")
-            mine = self._of[slot]
+            mine = self._pages(slot)
             if first > len(mine) * PAGE:
                 raise ValueError(f"position {first} lies behind the sequence's {len(mine)} pages")
             if slot in slots:
@@ -113,18 +118,21 @@ class Kv4Cache:
 
     def fork(self, src: int, dst: int) -> None:
         """Sequence `dst` (whose own pages are given up) becomes one with `src`'s positions; the pages are shared until one of them writes."""
+        pages = list(self._pages(src))
+        self._pages(dst)
         if src == dst:
             return
-        for p in self._of[src]:
+        for p in pages:
             self._users[p] += 1
         self._give_up(dst, 0)
-        self._of[dst] = list(self._of[src])
+        self._of[dst] = pages
         self._publish(dst)
 
     def truncate(self, slot: int, length: int) -> None:
         """Gives up the pages behind position length - 1."""
         if length < 0:
             raise ValueError("length must not be negative")
+        self._pages(slot)
         self._give_up(slot, -(-length // PAGE))
         self._publish(slot)
 

@@ -205,3 +205,18 @@ def test_ids_outside_the_vocabulary_are_refused(make):
     model.prefill([[0], torch.tensor([VOCAB - 1]), torch.tensor([], dtype=torch.int64)])
     model.feed(torch.tensor([[1, 2, 3]]))
     assert model.lengths == [2, 2, 1]
+
+
+@pytest.mark.parametrize("slot", [-1, -BATCH, BATCH, 1 << 20])
+def test_there_is_one_name_for_a_sequence(make, slot):
+    model = make(pages=6)
+    model.prefill([[1] * 100, [2], [3] * 70])
+    before = state(model), list(model.cache._users)
+    c = model.cache
+    for call in (lambda: c.fork(0, slot), lambda: c.fork(slot, 0), lambda: c.fork(slot, slot), lambda: c.free(slot), lambda: c.truncate(slot, 1), lambda: c.pages_of(slot),
+                 lambda: c.reserve(slot, 0, 1), lambda: c.reserve_all([(0, 100, 101), (slot, 0, 1)]), lambda: model.fork(0, slot), lambda: model.fork(slot, 0)):
+        with pytest.raises(ValueError):
+            call()
+        assert (state(model), list(c._users)) == before
+    model.fork(1, 1)
+    assert (state(model), list(c._users)) == before
