@@ -437,11 +437,13 @@ class BcqLlamaBatchDecoder:
         if temperature is None:
             self.graph, self.sampling = None if self.sampling is not None else self.graph, None
             return
+        settings = [torch.as_tensor(v, dtype=t).expand(self.batch) for v, t in
+                    ((temperature, torch.float32), (top_k, torch.int32), (top_p, torch.float32), (min_p, torch.float32))]
         if self.sampling is None:
             self.graph = None
-            self.sampling = tuple(torch.zeros(self.batch, dtype=t, device=self.device) for t in (torch.float32, torch.int32, torch.float32, torch.float32))
-        for own, v in zip(self.sampling, (temperature, top_k, top_p, min_p)):
-            own.copy_(torch.as_tensor(v, dtype=own.dtype).expand(self.batch))
+            self.sampling = tuple(torch.zeros(self.batch, dtype=v.dtype, device=self.device) for v in settings)
+        for own, v in zip(self.sampling, settings):
+            own.copy_(v)
 
     def _next_tokens(self, lg):
         """Tokens of the fp16 logits; the fp32 copy stays in `logits`."""

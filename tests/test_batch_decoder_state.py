@@ -220,3 +220,18 @@ def test_there_is_one_name_for_a_sequence(make, slot):
         assert (state(model), list(c._users)) == before
     model.fork(1, 1)
     assert (state(model), list(c._users)) == before
+
+
+def test_settings_of_another_size_change_nothing(make):
+    model = make()
+    model.graph = graph = object()
+    for bad in (dict(temperature=[1.0, 2.0]), dict(temperature=0.5, top_k=[1] * 4), dict(temperature=0.5, min_p="x")):
+        with pytest.raises((RuntimeError, TypeError, ValueError)):
+            model.set_sampling(**bad)
+        assert model.sampling is None and model.graph is graph
+    model.set_sampling(0.7, top_k=[3, 4, 5], top_p=0.9, min_p=torch.tensor([0.1, 0.0, 0.2]))
+    assert model.graph is None
+    model.graph, before = graph, [t.clone() for t in model.sampling]
+    with pytest.raises(RuntimeError):
+        model.set_sampling(0.1, top_k=2, top_p=[0.5, 0.5])
+    assert all(map(torch.equal, model.sampling, before)) and model.graph is graph and model.sampling[1].tolist() == [3, 4, 5]
