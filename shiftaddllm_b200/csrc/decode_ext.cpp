@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <string>
 #include <vector>
 
@@ -136,6 +137,7 @@ struct Setting {
             ptr = t.data_ptr();
         } else {
             all = v.cast<double>();
+            TORCH_CHECK(dtype != torch::kInt32 || std::fabs(all) <= 0x7fffffff, "sample_token: ", name, " must be a 32-bit number, got ", all);
         }
     }
 };
@@ -155,7 +157,7 @@ void sample_token(const Tensor &logits, const Tensor &u, const Tensor &token, co
     py::gil_scoped_release release;
     c10::cuda::CUDAGuard guard(device);
     check_status(sal_sample_token(logits.data_ptr(), dtype == torch::kFloat32, whole(what, rows), whole(what, vocab), u.data_ptr(), t.ptr,
-                                  static_cast<const int32_t *>(k.ptr), p.ptr, least.ptr, (float)t.all, whole(what, (int64_t)k.all), (float)p.all, (float)least.all,
+                                  static_cast<const int32_t *>(k.ptr), p.ptr, least.ptr, (float)t.all, (int)k.all, (float)p.all, (float)least.all,
                                   token.data_ptr<int64_t>(), stream_of(device)),
                  "sal_sample_token");
 }

@@ -320,6 +320,8 @@ def copy_kv4_pages(pool, src, dst):
         raise RuntimeError(f"copy_kv4_pages: {n} pages to copy, {len(dst)} places")
     if n == 0:
         return
+    if not all(0 <= p < pool.shape[1] for p in (*src, *dst)):      # a 32-bit number of them would wrap around
+        raise RuntimeError(f"copy_kv4_pages: pages must be 0 .. {pool.shape[1] - 1}")
     lib = _lib.load()
     pages = (ctypes.c_int32 * (2 * n))(*src, *dst)
     with _on(pool.device):
@@ -352,6 +354,8 @@ def sample_token(logits, u, token, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
             ptr.append(v.data_ptr())
             one.append(0)
         else:
+            if name == "top_k" and not abs(v) <= 0x7fffffff:
+                raise RuntimeError(f"sample_token: top_k must be a 32-bit number, got {v}")
             ptr.append(None)
             one.append(v)
     lib = _lib.load()
