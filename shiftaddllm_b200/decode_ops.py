@@ -216,7 +216,7 @@ def _kv4_pool_check(what, pool, table, pos, rows, kv_heads, hd):
 
 def _rows_per_sequence(what, name, t, batch, width):
     """m of a tensor [batch, m, width] (or [batch * m, width])."""
-    if not isinstance(t, torch.Tensor) or batch < 1 or t.numel() == 0 or t.numel() % (batch * width):
+    if not isinstance(t, torch.Tensor) or batch < 1 or width < 1 or t.numel() == 0 or t.numel() % (batch * width):
         raise RuntimeError(f"{what}: {name} must hold the same number of rows of {width} numbers for each of {batch} sequences")
     return t.numel() // (batch * width)
 
@@ -245,13 +245,14 @@ def rope_kv4_write(q, k, v, cos, sin, pos, table, pool, q_out, heads, kv_heads, 
     m = _rows_per_sequence("rope_kv4_write", "q", q, batch, heads * hd)
     for name, t, width in (("q", q, heads), ("q_out", q_out, heads), ("k", k, kv_heads), ("v", v, kv_heads)):
         _want("rope_kv4_write", name, t, torch.float16, (batch, m, width * hd), device)
-    _want("rope_kv4_write", "cos", cos, torch.float32, (cos.numel() // (hd // 2), hd // 2), device)
-    _want("rope_kv4_write", "sin", sin, torch.float32, (cos.shape[0], hd // 2), device)
+    angles = cos.numel() // (hd // 2)
+    for name, t in (("cos", cos), ("sin", sin)):
+        _want("rope_kv4_write", name, t, torch.float32, (angles, hd // 2), device)
     lib = _lib.load()
     with _on(device):
         _lib.check(lib.sal_rope_kv4_write_f16(q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos.data_ptr(),
                                               None if rows is None else rows.data_ptr(), table.data_ptr(), pool.data_ptr(), q_out.data_ptr(),
-                                              batch, m, heads, kv_heads, hd, cos.shape[0], max_pages, pages, _stream(q)), "sal_rope_kv4_write_f16")
+                                              batch, m, heads, kv_heads, hd, angles, max_pages, pages, _stream(q)), "sal_rope_kv4_write_f16")
 
 
 def read_kv4(pool, table, pos, k_out, v_out, kv_heads, hd):

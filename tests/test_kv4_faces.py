@@ -41,3 +41,20 @@ def test_top_k(reached):
     for k in (0, 5, -1, (1 << 31) - 1):
         decode_ops.sample_token(logits, u, token, top_k=k)
         assert reached.pop()[10] == k
+
+
+def test_angles_of_any_shape(reached, monkeypatch):
+    """As in the compiled module: rows of hd / 2 numbers, whatever the dimensions in front of them are."""
+    monkeypatch.setattr(_lib, "load", lambda: SimpleNamespace(sal_rope_kv4_write_f16=lambda *a: reached.append(a) or 0))
+    half, pos, table = torch.zeros(1, 1, 128, dtype=torch.float16), torch.zeros(1, dtype=torch.int64), torch.zeros(1, 1, dtype=torch.int32)
+    pool = torch.zeros(2, 2, 64 * 72, dtype=torch.uint8).as_subclass(OnGpu)
+    for shape in ((10, 32), (1, 10, 32), (2, 5, 32)):
+        decode_ops.rope_kv4_write(half, half, half, torch.zeros(shape), torch.zeros(shape), pos, table, pool, half, 2, 2, 64)
+        assert reached.pop()[15] == 10
+    for cos, sin in (((10, 32), (9, 32)), ((10, 64), (10, 64)), ((0, 32), (10, 32))):
+        with pytest.raises(RuntimeError):
+            decode_ops.rope_kv4_write(half, half, half, torch.zeros(cos), torch.zeros(sin), pos, table, pool, half, 2, 2, 64)
+    for heads in (0, -1):
+        with pytest.raises(RuntimeError):
+            decode_ops.rope_kv4_write(half, half, half, torch.zeros(10, 32), torch.zeros(10, 32), pos, table, pool, half, heads, 2, 64)
+    assert not reached
