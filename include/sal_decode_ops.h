@@ -132,7 +132,9 @@ int sal_causal_softmax_f16(void *scores, int heads, int m, int T, int first, flo
  * sal_read_kv4: the values of m positions from pos[b] on, k_out and v_out [batch][m][kv_heads][hd], fp32 (out_f32) or fp16; zero for
  * positions without a page.
  * sal_attention_kv4_f16: q [batch][m][heads][hd] (rotated), out likewise; row i of sequence b sees positions 0..pos[b] + i as far as their
- * pages exist (a row that sees none gets zeros).  Scores and sums in fp32.  workspace: sal_attention_kv4_workspace_bytes of scratch, zero-filled
+ * pages exist (a row that sees none gets zeros).  Scores and sums in fp32; a weight times a value's scale is kept to 22 bits, and to no less
+ * than 2**-31 of the largest weight times the largest scale among the 32 (up to 64 columns m * heads / kv_heads, and heads of 256) or 64
+ * neighbouring positions that it is worked on with.  workspace: sal_attention_kv4_workspace_bytes of scratch, zero-filled
  * once, 16-byte aligned, for calls of up to that many sequences and rows, not shared between streams (nor between graphs that may run at
  * once).  Its first word reports a device-side wait that ran out (SAL_E_TIMEOUT; sal_workspace_status reads and clears it).
  * sal_copy_kv4_pages: page dst[i] becomes a copy of page src[i], in all of `layers` layers (pool [layers][pages][page_bytes]).  src and dst

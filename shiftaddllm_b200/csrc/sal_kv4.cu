@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(ROW_THREADS) read_kv4_kernel(CacheArgs c, cons
 //
 // A score is scale * sum_g (s_g * D_g + low_g * Q_g) with D_g = sum over the group of q * code and Q_g = sum of q; an output is
 // E_g * A_g + sum_t p_t * (low_t + 8 s_t) with A_g = sum over positions of (p * s_g / E_g) * (code - 8).  The codes are 16-bit floats without any error, so D_g and A_g are matrix products of 16-bit operands (m16n8k16, 32-bit sums) in which only the
-// weight p * s is rounded; it goes in as the sum of two 16-bit numbers.  E_g, a power of two not below any scale so far, keeps the weights in
+// weight p * s is rounded; it goes in as the sum of two 16-bit numbers.  E_g, a power of two not below the scales at hand, keeps the weights in
 // their range.  Neither keys nor values are ever formed.
 //
 // Matrix fragments hold keys (or, for the second product, dimensions) as rows and query columns as columns: a lane's part of a row are
@@ -643,6 +643,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) big[g] = 6.1035156e-5f, to_one[g] = W_ONE / big[g];     // 2**-14
+        constexpr uint32_t LOOK = 0xbc00bc00u;                  // -1: no scale is that small, so the next step finds E anew
         uint32_t big_h[(G + 1) / 2];                            // the same as pairs of 16-bit numbers
 #pragma unroll
         for (int i = 0; i < (G + 1) / 2; ++i) big_h[i] = 0x04000400u;
@@ -677,6 +678,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
                     sum_i = 0.f;
                 }
                 set_aside = true;
+                if ((p0 / PG) % (4 * SET_ASIDE) == 0) big_h[0] = LOOK;
             }
             if (alive && sched[(unit0 + pg) & (2 * CHUNK - 1)].x >= 0) {
 #pragma unroll 1
@@ -755,7 +757,10 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
                         }
                     }
                     // A column's weights are powers relative to `ref`, which follows its largest score only when this lane's four would pass 2**8 in
-                    // sum; E likewise follows the scales.  Most keys move neither, which one vote finds out.
+                    // sum; E likewise follows the scales.  Most keys move neither, which one vote finds out.  E comes down again, to the scales of the
+                    // step at hand, behind a step for some of whose positions it jumped, and every 64 pages.  A weight p * s keeps 2**-31 of E, so that
+                    // E would otherwise cost all that follow a few far larger values their digits (4000 positions of weight 2**-16 behind one of 2**16 times
+                    // their scale: 1 to 4 % of the largest value; now the other 31 positions of its step alone).  Asking every step costs 1 to 3 % of the time.
                     float w[2][NT][4], add[NT][2];
                     bool moved = first;
 #pragma unroll
@@ -784,6 +789,8 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
                     }
                     if (__any_sync(0xffffffffu, moved)) {
                         float fg[G];
+                        const bool anew = __any_sync(0xffffffffu, big_h[0] == LOOK);      // each lane's own
+                        bool jumped = false;
 #pragma unroll
                         for (int g = 0; g < G; ++g) {
                             float x = 0.f;
@@ -793,8 +800,9 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
                                 x = fmaxf(x, fmaxf(x0 <= 65504.f ? x0 : 0.f, x1 <= 65504.f ? x1 : 0.f));
                             }
                             const uint32_t u = (__reduce_max_sync(0xffffffffu, __float_as_uint(x)) + 0x7fffffu) & 0x7f800000u;   // up to a power of two
-                            const float grown = fminf(fmaxf(__uint_as_float(u), big[g]), 32768.f);
+                            const float grown = fminf(fmaxf(__uint_as_float(u), anew ? 6.1035156e-5f : big[g]), 32768.f);
                             fg[g] = __fdividef(big[g], grown);
+                            jumped |= 64.f * x < grown && fg[g] <= 0.125f;      // not for this lane's positions
                             big[g] = grown, to_one[g] = __fdividef(W_ONE, grown);
                             const uint32_t h = __half_as_ushort(__float2half_rn(grown));
                             if (G == 1) big_h[0] = h * 0x10001u;
@@ -830,6 +838,7 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
                                     }
                                 }
                             }
+                        if (jumped) big_h[0] = LOOK;
                         first = false;
                     }
 #pragma unroll
