@@ -361,9 +361,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
             if (lane == 0) use(i, place, before);
         }
     };
-    // the first block finds the last kept token of the list
+    // The first block finds the last kept token of the list; false if it is not there.  Rounding cannot push it out of the window (a bin's bounds are
+    // off by 5e-6 where their sum matters, the window is 1e-5 wider), but nothing is made of shared memory that no thread wrote.
+    mass_t prefix;      // the weights of the prefix
     auto settle = [&](bool by_mass, int k, double goal) {
         if (rank == 0) {
+            if (tid == 0) s.found.ties = 0;
+            __syncthreads();
             rank_all([&](int i, int place, mass_t before) {
                 const mass_t w = s.list_w[i];
                 // the last one kept: the k-th, or the one with which the weights pass the goal
@@ -378,8 +382,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
         }
         cluster.sync();
         const Found f = cluster.map_shared_rank(&s, 0)->found;
-        end = f.end, ties = f.ties;
-        return f.mass;
+        if (f.ties == 0) return false;
+        end = f.end, ties = f.ties, prefix = f.mass;
+        return true;
     };
 
     bool done = false;
@@ -517,7 +522,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
                 narrow(false, top_k, 0.);
                 const int in_front = window[0].y;
                 gather(window[0].x, window[1].x, has_p);      // the prefix's weights are what top_p is of
-                total = listed <= LIST ? settle(false, top_k - in_front, 0.) : by_bits(false, top_k, 0.);
+                total = listed <= LIST && settle(false, top_k - in_front, 0.) ? prefix : by_bits(false, top_k, 0.);
             }
             if (has_p) {
                 const float k_end = end;
@@ -536,8 +541,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
                 }
                 narrow(true, 0, goal);
                 gather(window[0].x, window[1].x, true);
-                if (listed <= LIST) settle(true, 0, goal);
-                else (void)by_bits(true, 0, goal);
+                if (listed > LIST || !settle(true, 0, goal)) (void)by_bits(true, 0, goal);
                 if (top_k > 0 && end == k_end) ties = min(ties, k_ties);      // the second prefix is part of the first
             }
         }
