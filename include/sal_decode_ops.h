@@ -155,7 +155,7 @@ int sal_copy_kv4_pages(void *pool, const int32_t *src, const int32_t *dst, int c
 /* The next token of each of `rows` sequences, drawn from its logits (fp32 if logits_f32, else fp16; [rows][vocab], vocab <= 262144) with the
  * random number u[row] (fp32): a token's weight is exp((logit - largest) / temperature); in the order of falling logits, equal ones by
  * index, the first top_k tokens stay (<= 0: all), of these those in front of which less than top_p of their weights lies (>= 1: all;
- * the first always stays), of these those with a weight of at least min_p (the largest is 1; <= 0: all).  The token is the first, by index,
+ * the first always stays), of these those with a weight of at least min_p (the largest is 1; <= 0: all; > 1: as 1).  The token is the first, by index,
  * at which the running sum of the weights that stayed exceeds u times their total.  temperature <= 0 takes the largest logit, the first of
  * equal ones.  NaN and -infinity are never chosen; a row of nothing else gives 0.  temperature, top_k, top_p, min_p: device arrays [rows],
  * or NULL for the one value of all rows that stands in the argument of that name with _all.  Weights are summed in whole numbers of 2**-44:

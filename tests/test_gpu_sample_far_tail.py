@@ -38,3 +38,13 @@ def test_the_border_lies_among_small_weights(vocab, units, spread, share, k_of):
         for got, tokens, run in zip(token.tolist(), kept, runs):
             want = int(np.searchsorted(run, np.floor(number * float(run[-1])), side="right"))
             assert got in tokens[max(0, want - 1): want + 2], (got, want, tokens[want])
+
+
+@pytest.mark.parametrize("min_p", [1.0, 1.5, float("inf")])
+def test_min_p_of_one_and_above_keeps_the_largest(min_p):
+    x = torch.randn(4, 9000, generator=torch.Generator().manual_seed(0)).cuda()
+    x[:, [17, 5000]] = 9.0      # two of them
+    u, token = torch.tensor([0.0, 0.49, 0.51, 1.0], device="cuda"), torch.full((4,), -1, dtype=torch.int64, device="cuda")
+    for kw in (dict(), dict(top_k=50), dict(top_p=0.99)):
+        decode_ops.sample_token(x, u, token.fill_(-1), min_p=min_p, **kw)
+        assert token.tolist() == [17, 17, 5000, 5000]
