@@ -85,9 +85,10 @@ __device__ __forceinline__ uint8_t *record_of(const CacheArgs &c, int b, int p, 
 }
 
 // Writing and reading: a thread has eight neighbouring numbers of a head, 16 bytes of 16-bit numbers or 4 bytes of codes, HD / 8 threads a head.  The
-// other numbers of its rotary pairs are HD / 16 threads on, a group is eight threads.  Writing is bound by instruction issue (conversions, the checks of
-// the rounding, shuffles; about 280 a warp and row): 27 us for 1537 rows of 64 + 8 heads of 128, 57 MB; reading them back 5.7 us; one row of 16
-// sequences 3.1 and 1.9 us, a launch's latency.  Blocks go over a sequence's rows with a stride, threads of a block over the heads of a row.
+// other numbers of its rotary pairs are HD / 16 threads on, a group is eight threads.  Writing takes 27 us for 1537 rows of 64 + 8 heads of 128, 57 MB, a
+// third of the copy rate: 17 million warp instructions (conversions, the checks of the rounding, shuffles) in 62 % of the issue slots, the rest
+// latency of loads and of dependent steps at 23 warps an SM.  Reading them back takes 5.7 us; one row of 16 sequences 3.1 and 1.9 us, a launch's
+// latency.  Blocks go over a sequence's rows with a stride, threads of a block over the heads of a row.
 constexpr int ROW_THREADS = 256;
 
 template <int HD>
@@ -240,8 +241,9 @@ __global__ void __launch_bounds__(ROW_THREADS) read_kv4_kernel(CacheArgs c, cons
 // page of a head is one contiguous record, so its fetch is one bulk copy into a ring of shared memory.  Blocks that share an item leave
 // their part (maximum, sum, unnormalised output) in scratch; the last one to arrive adds them up in the order of the positions.
 //
-// Bound by instruction issue (about 390 a warp for 16 positions; 52 % of the issue slots, 35 % of HBM), not by bytes: 54 us for 159 MB of records
-// (16 sequences of 300 to 4000 positions, 32 heads of 128; 2.9 TB/s), 97 us for 294 MB (three of 70 to 100 thousand, 64 query and 8 kv heads).
+// Bound by the latency of dependent steps at 12 warps an SM, neither by bytes nor by issue (35 % of HBM, 52 % of the issue slots; the 390 instructions a
+// warp for 16 positions would take half the time at full issue): 54 us for 159 MB of records (16 sequences of 300 to 4000 positions, 32 heads
+// of 128; 2.9 TB/s), 97 us for 294 MB (three of 70 to 100 thousand, 64 query and 8 kv heads).
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
@@ -385,7 +387,7 @@ struct AttnShape {
     static constexpr int STAGE = REC + (QUERIES ? COLS * HD * 2 : 0);
     // What an item costs by itself (its first page's wait, the sum over the warps, the output or the part) in pages: 2.8 us against 1.2 us a page
     // with one column and heads of 128.  Counted as 1, 2, 3, 4 pages: 63, 55, 54, 54 us for 16 sequences of 300 to 4000 positions with 32 heads; as
-    // 1 and 3 with 32 columns and heads of 256: 109 and 92 (four sequences, 33 rows behind 1000 to 5000 positions), 152 and 156 (512 rows of one).
+    // 1 and 3 with 32 columns and heads of 256: 111 and 94 (four sequences, 33 rows behind 1000 to 5000 positions), 154 and 158 (512 rows of one).
     static constexpr int ITEM_UNITS = 3;
     static constexpr int MIN_UNITS = ITEM_UNITS + 2;
     static constexpr int STAGES = 4;      // a power of two; so many pages on lie within 32 units, ITEM_UNITS at most being in front of each
@@ -1089,8 +1091,8 @@ __global__ void __launch_bounds__(AttnShape<HD, NT, DUP, WK, PG, WC>::THREADS, A
 //
 // A block takes one item, or one of `splits` equal runs of its pages; the last one to arrive adds the parts up in order.  Items with the most pages are
 // launched first.  Equal runs that may end inside an item, as above, cost more in parts of 128 columns and new starts than they even out: 98 us where this
-// takes 79 (512 rows behind 1536 positions, 32 heads of 128: 15 GFLOP, and half as much again for the second parts).  Bound by instruction issue and latency at
-// 16 warps an SM: 46 % of the issue slots, 1140 instructions a warp and page.  While the tensor core works for one of the two blocks of an SM the other one expands, and within a block the next page's keys are expanded
+// takes 79 (512 rows behind 1536 positions, 32 heads of 128: 15 GFLOP, and half as much again for the second parts).  Bound by latency at
+// 16 warps an SM: 46 % of the issue slots, 1140 instructions a warp and page, most of them once per score and group.  While the tensor core works for one of the two blocks of an SM the other one expands, and within a block the next page's keys are expanded
 // behind the second product's back.
 template <int HD>
 struct WideShape {

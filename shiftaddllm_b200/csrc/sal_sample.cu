@@ -15,9 +15,9 @@
 // Weights are whole numbers in units of 2**-44 (the largest is 2**44, a sum of 2**18 of them fits 63 bits): sums do not depend on their
 // order, so the same inputs give the same token however the work is split, and the running sum meets the total exactly.
 //
-// Bound by instructions over a row's logits (three to four passes over shared memory: 45 % of the issue slots, 1.3 % of HBM) and by about twelve
-// barriers of the cluster, 1 us each: 14.6 us for a row of 32000 with top-k and top-p, 40 us for 64 such rows with all kinds of filters, 122 us for 48 rows of
-// 131071 with top-p.
+// Bound by the latency of four to six passes over a row in shared memory (45 % of the issue slots, 1.3 % of HBM; 230 instructions of a thread per logit
+// with top-p) and of about twelve barriers of the cluster, 1 us each: 14.4 us for a row of 32000 with top-k and top-p, 40 us for 64 such rows with all
+// kinds of filters, 121 us for 48 rows of 131071 with top-p, whose 192 blocks lie two to an SM on 44 of them and one on the others.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
