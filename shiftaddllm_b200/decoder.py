@@ -88,11 +88,11 @@ def _group(lins, x, outs, pdl=True, x_mul=None, atomic=False, swiglu_fixed=False
 
 
 def _capture(model, step):
-    """`step` as a CUDA graph, behind one eager call of it; the model's token and position are put back."""
+    """`step` as a CUDA graph, behind one eager call of it; the model's token, position and logits are put back."""
     stream = torch.cuda.Stream(model.device)
     stream.wait_stream(torch.cuda.current_stream(model.device))      # which may still be at the weights, the token or its position
     with torch.cuda.stream(stream):
-        saved = (model.token.clone(), model.pos.clone())
+        saved = (model.token.clone(), model.pos.clone(), model.logits.clone())
         step()
         torch.cuda.synchronize(model.device)
         model.token.copy_(saved[0])
@@ -102,6 +102,7 @@ def _capture(model, step):
             step()
         model.token.copy_(saved[0])
         model.pos.copy_(saved[1])
+        model.logits.copy_(saved[2])
     torch.cuda.synchronize(model.device)
     model.graph, model._stream = g, stream
     return g

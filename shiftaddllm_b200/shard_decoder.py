@@ -239,7 +239,7 @@ class ColumnParallelDecoder:
         stream = torch.cuda.Stream(self.device)
         stream.wait_stream(torch.cuda.current_stream(self.device))      # which may still be at the weights, the token or its position
         with torch.cuda.stream(stream):
-            saved = (self.token.clone(), self.pos.clone(), self._slot)
+            saved = (self.token.clone(), self.pos.clone(), self._slot, self.logits.clone())
             self.step()
             torch.cuda.synchronize(self.device)
             self.token.copy_(saved[0])
@@ -251,6 +251,7 @@ class ColumnParallelDecoder:
                 self.step()
             self.token.copy_(saved[0])
             self.pos.copy_(saved[1])
+            self.logits.copy_(saved[3])
         torch.cuda.synchronize(self.device)
         self.graph, self._stream = g, stream
         return g

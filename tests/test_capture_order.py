@@ -36,21 +36,32 @@ def log(monkeypatch):
 
 
 def state(log, **more):
-    return SimpleNamespace(device=torch.device("cpu"), token=torch.zeros(1), pos=torch.zeros(1), step=lambda: log.append("step"), **more)
+    model = SimpleNamespace(device=torch.device("cpu"), token=torch.zeros(1), pos=torch.zeros(1), logits=torch.zeros(5), **more)
+
+    def step():
+        log.append("step")
+        for t in (model.token, model.pos, model.logits):
+            t.add_(1)
+
+    model.step = step
+    return model
 
 
-def in_order(log):
+def in_order(log, model):
     assert log[:3] == ["wait", "side stream", "step"] and log[-1] == "synchronize" and log.count("step") == 2
+    assert not model.token.any() and not model.pos.any() and not model.logits.any()
 
 
 def test_decoder(log):
-    decoder.BcqLlamaDecoder.capture(state(log))
-    in_order(log)
+    model = state(log)
+    decoder.BcqLlamaDecoder.capture(model)
+    in_order(log, model)
 
 
 def test_column_parallel_decoder(log):
-    shard_decoder.ColumnParallelDecoder.capture(state(log, _slot=0, blocks=[None] * shard_decoder.NSLOTS))
-    in_order(log)
+    model = state(log, _slot=0, blocks=[None] * shard_decoder.NSLOTS)
+    shard_decoder.ColumnParallelDecoder.capture(model)
+    in_order(log, model)
 
 
 def test_the_benchmark_s_steps(log):

@@ -79,3 +79,16 @@ def test_generating_behind_the_benchmark(like):
     fresh.prefill(ids.t().tolist())
     fresh.generate(8)
     assert torch.equal(model.generate(6), fresh.generate(6)) and torch.equal(model.logits, fresh.logits)
+
+
+@pytest.mark.parametrize("bits", [4, 16])
+def test_a_capture_leaves_the_state_as_it_was(like, bits):
+    """Behind a prompt, not forked and of no whole number of pages, with no wait of the host in between."""
+    model = make(like, bits)
+    if bits == 4:
+        model.prefill(prompts([5, 130, 70]))
+    else:
+        model.feed(torch.tensor(prompts([7] * BATCH)).t())
+    before = [t.clone() for t in (model.token, model.pos, model.logits)]
+    model.capture()
+    assert all(map(torch.equal, before, (model.token, model.pos, model.logits)))
